@@ -14,6 +14,7 @@ from .hip_attn import (BLOCK_K, BLOCK_Q, TileList, attention_backward, attention
                        tiled_flash_attention_qkv)
 from .mesh import adjacency, build_tile_mask, hilbert_order, icosahedral_mesh, khop_mask, mesh_mask
 from .mha import TiledMHA
+from .rms import add_rms_norm, add_rms_norm_q8, quantize_rows, rms_norm, rms_norm_q8
 from .rows import gather_layer_norm, layer_norm_scatter
 from .transformer import MeshBlock, MeshTransformer
 from .tile_cache import cached_khop_tiles, cached_tile_mask

@@ -75,6 +75,13 @@ class RowsDesc(ctypes.Structure):
               ("dtype", ctypes.c_int32), ("eps", ctypes.c_float)]
 
 
+class RmsDesc(ctypes.Structure):
+  _fields_ = [("rows", ctypes.c_int64), ("x_stride", ctypes.c_int64), ("y_stride", ctypes.c_int64),
+              ("channels", ctypes.c_int32), ("dtype", ctypes.c_int32), ("weight_dtype", ctypes.c_int32),
+              ("eps", ctypes.c_float)]
+
+
+RMS_MAX_CHANNELS = 16384  # FWN_RMS_MAX_CHANNELS
 ROWS_MAX_CHANNELS = 4096  # FWN_ROWS_MAX_CHANNELS
 COND_MAX = 64  # FWN_COND_MAX: norms of one fwn_cond_affine_launch
 ROWS_PERM_GRAD, ROWS_PERM_OUT = 1, 2  # FWN_ROWS_PERM_*: what the backward's perm permutes
@@ -86,6 +93,7 @@ _DESC = ctypes.POINTER(AttnDesc)
 _TILES = ctypes.POINTER(Tiles)
 _ROWS = ctypes.POINTER(RowsDesc)
 _DS = ctypes.POINTER(DsMap)
+_RMS = ctypes.POINTER(RmsDesc)
 
 # name -> argtypes, every entry point of include/fwn_attn.h and include/fwn_rows.h
 SIGNATURES = {
@@ -128,6 +136,11 @@ SIGNATURES = {
     "fwn_cond_affine_launch": [_I32, _I32, _I32, _I32, _I32, _P, _P, _P, _P, _P, _P],
     "fwn_rows_norm_bwd_workspace_size": [_ROWS, _P],
     "fwn_rows_norm_bwd_launch": [_ROWS, _P, _P, _I32, _P, _P, _P, _P, _P, _P, _P, _U64, _P],
+    "fwn_rms_norm_launch": [_RMS, _P, _P, _P, _P, _P, _P],
+    "fwn_rms_norm_q8_launch": [_RMS, _P, _P, _P, _P, _P, _P, _P],
+    "fwn_quantize_rows_launch": [_RMS, _P, _P, _P, _P],
+    "fwn_rms_norm_bwd_workspace_size": [_RMS, _P],
+    "fwn_rms_norm_bwd_launch": [_RMS, _P, _P, _P, _P, _P, _P, _P, _U64, _P],
 }
 
 _lock = threading.Lock()

@@ -121,6 +121,46 @@ int fwn_linear_wgrad_workspace_size(int64_t rows, int32_t outs, int32_t ins, uin
 int fwn_linear_wgrad_launch(int64_t rows, int32_t outs, int32_t ins, const void* g, const void* x, void* dw, void* db,
                             void* workspace, uint64_t workspace_bytes, void* stream);
 
+/* Root-mean-square norm of rows, its output in the tensors' dtype or in 8 bits. Rows are `channels`
+ * elements with stride 1; row i of x begins at i * x_stride elements (0: one row for all), of y likewise,
+ * every other tensor is contiguous. Statistics are float32. */
+#define FWN_RMS_MAX_CHANNELS 16384
+
+typedef struct fwn_rms_desc {
+  int64_t rows;
+  int64_t x_stride, y_stride;
+  int32_t channels;      /* 1 to FWN_RMS_MAX_CHANNELS */
+  int32_t dtype;         /* fwn_dtype of x, y, sum, out and the gradients */
+  int32_t weight_dtype;  /* the dtype, or FWN_F32 */
+  float eps;             /* added to the mean square, finite and >= 0 */
+} fwn_rms_desc;
+
+/* With y, sum = x + y (added in float32, rounded once) and the norm is of sum as stored, else y and sum
+ * are NULL and it is of x: out[i, :] = s[i, :] / sqrt(mean(s[i, :]^2) + eps) * weight (NULL: 1). sum and
+ * out must not overlap each other or an input. */
+int fwn_rms_norm_launch(const fwn_rms_desc* d, const void* x, const void* y, const void* weight, void* sum, void* out,
+                        void* stream);
+
+/* The same with the output in 8 bits: for the unrounded values v of a row, scale[i] = max(max |v| / 448,
+ * 2^-126) and q[i, :] the OCP e4m3 codes of v / scale[i], rounded to nearest even. A row with NaN has
+ * scale and codes NaN; one whose largest magnitude is infinite has scale infinity and NaN codes there. */
+int fwn_rms_norm_q8_launch(const fwn_rms_desc* d, const void* x, const void* y, const void* weight, void* sum, uint8_t* q,
+                           float* scale, void* stream);
+
+/* q and scale of the rows of x as they are. */
+int fwn_quantize_rows_launch(const fwn_rms_desc* d, const void* x, uint8_t* q, float* scale, void* stream);
+
+/* Backward of fwn_rms_norm_launch at the contiguous rows s that were normalised (sum, or x):
+ *   gx = g_sum + r (h - s r^2 mean(h s)),  h = g_out weight,  r = 1 / sqrt(mean(s^2) + eps)
+ *   gw = sum over the rows of g_out s r, in weight_dtype
+ * g_sum (NULL: zeros) is the gradient of sum. gx is the gradient of x and of y. gw may be NULL; with it the
+ * launch needs fwn_rms_norm_bwd_workspace_size bytes of workspace (16-byte aligned), whose sums run in a
+ * fixed order. gx must not overlap an input. */
+int fwn_rms_norm_bwd_workspace_size(const fwn_rms_desc* d, uint64_t* bytes);
+int fwn_rms_norm_bwd_launch(const fwn_rms_desc* d, const void* s, const void* weight, const void* g_out,
+                            const void* g_sum, void* gx, void* gw, void* workspace, uint64_t workspace_bytes,
+                            void* stream);
+
 #ifdef __cplusplus
 }  /* extern "C" */
 #endif
