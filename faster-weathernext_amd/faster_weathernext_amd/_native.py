@@ -81,6 +81,14 @@ class RmsDesc(ctypes.Structure):
               ("eps", ctypes.c_float)]
 
 
+class LinearDesc(ctypes.Structure):
+  _fields_ = [("rows", ctypes.c_int64), ("x_stride", ctypes.c_int64), ("w_stride", ctypes.c_int64),
+              ("r_stride", ctypes.c_int64), ("ins", ctypes.c_int32), ("outs", ctypes.c_int32), ("dtype", ctypes.c_int32),
+              ("activation", ctypes.c_int32)]
+
+
+ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}  # FWN_ACT_*
+LINEAR_ACT_MAX = 1 << 20  # FWN_LINEAR_ACT_MAX
 RMS_MAX_CHANNELS = 16384  # FWN_RMS_MAX_CHANNELS
 ROWS_MAX_CHANNELS = 4096  # FWN_ROWS_MAX_CHANNELS
 COND_MAX = 64  # FWN_COND_MAX: norms of one fwn_cond_affine_launch
@@ -94,6 +102,7 @@ _TILES = ctypes.POINTER(Tiles)
 _ROWS = ctypes.POINTER(RowsDesc)
 _DS = ctypes.POINTER(DsMap)
 _RMS = ctypes.POINTER(RmsDesc)
+_LIN = ctypes.POINTER(LinearDesc)
 
 # name -> argtypes, every entry point of include/fwn_attn.h and include/fwn_rows.h
 SIGNATURES = {
@@ -141,6 +150,12 @@ SIGNATURES = {
     "fwn_quantize_rows_launch": [_RMS, _P, _P, _P, _P],
     "fwn_rms_norm_bwd_workspace_size": [_RMS, _P],
     "fwn_rms_norm_bwd_launch": [_RMS, _P, _P, _P, _P, _P, _P, _P, _U64, _P],
+    "fwn_linear_act_workspace_size": [_LIN, _P],
+    "fwn_linear_act_launch": [_LIN, _P, _P, _P, _P, _P, _P, _P, _U64, _P],
+    "fwn_linear_act_bwd_workspace_size": [_LIN, _P],
+    "fwn_linear_act_bwd_launch": [_LIN, _P, _P, _P, _P, _P, _P, _P, _P, _U64, _P],
+    "fwn_linear_act_q8_workspace_size": [_LIN, _P],
+    "fwn_linear_act_q8_launch": [_LIN, _P, _P, _P, _P, _P, _P, _P, _P, _U64, _P],
 }
 
 _lock = threading.Lock()

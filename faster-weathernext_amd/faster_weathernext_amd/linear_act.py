@@ -1,0 +1,186 @@
+"""Linear layers with bias, activation and residual in the epilogue of their matrix product.
+
+    linear_act(x, weight, bias, activation=..., residual=...) = act(x weight^T + bias) + residual
+
+A feed-forward's first layer with its activation, its second with the block's residual, each one product
+whose epilogue does the rest, in the kernels of ``csrc/linear_act.hip``. Products accumulate in float32
+and the output is rounded once; float32 tensors keep float32's precision. ``linear_act`` is
+differentiable in x, weight, bias and residual; ``linear_act_q8`` takes the 8-bit rows of ``rms`` and has
+no derivative.
+"""
+import ctypes
+
+import torch
+
+from . import _native as nat
+from .rms import _Q8, _no_grad, _needs, rows_of
+from .rows import _DTYPES, _addr, _stream, as_torch
+
+
+def _check(x, weight, bias, residual, dtype, lead):
+  if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
+    raise ValueError(f"weight must be [outs, ins] and x [..., ins], got {tuple(weight.shape)} and {tuple(x.shape)}")
+  if not all(1 <= s <= nat.LINEAR_ACT_MAX for s in weight.shape):
+    raise ValueError(f"weight's sizes must be 1 to {nat.LINEAR_ACT_MAX}, got {tuple(weight.shape)}")
+  for t, name, shape in ((bias, "bias", weight.shape[:1]), (residual, "residual", (*lead, weight.shape[0]))):
+    if t is None:
+      continue
+    if not isinstance(t, torch.Tensor) or t.device != x.device or t.shape != shape:
+      raise ValueError(f"{name} must be a tensor of shape {tuple(shape)} on the device of x")
+    if t.dtype != dtype:
+      raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+
+
+def _activation(name):
+  if name not in nat.ACTIVATIONS:
+    raise ValueError(f"unknown activation {name!r} ({', '.join(str(a) for a in nat.ACTIVATIONS)})")
+  return nat.ACTIVATIONS[name]
+
+
+def _workspace(query, d, device):
+  size = ctypes.c_uint64(0)
+  nat.check(query(d, ctypes.byref(size)))
+  return (torch.empty(size.value, dtype=torch.uint8, device=device) if size.value else None), size.value
+
+
+def _forward(x, weight, bias, residual, activation, keep):
+  """(act(x weight^T + bias) + residual, the pre-activation or None), without autograd."""
+  lead, (outs, ins) = x.shape[:-1], weight.shape
+  xr, xs = rows_of(x)
+  wr, ws = rows_of(weight)
+  rr, rs = rows_of(residual) if residual is not None else (None, 0)
+  bias = bias.contiguous() if bias is not None else None
+  L = nat.lib()
+  with torch.cuda.device(x.device):
+    out = torch.empty((*lead, outs), dtype=x.dtype, device=x.device)
+    pre = torch.empty_like(out) if keep else None
+    d = nat.LinearDesc(x.numel() // ins, xs, ws, rs, ins, outs, _DTYPES[x.dtype], activation)
+    work, size = _workspace(L.fwn_linear_act_workspace_size, d, x.device)
+    nat.check(L.fwn_linear_act_launch(d, _addr(xr), _addr(wr), _addr(bias), _addr(rr), _addr(out), _addr(pre),
+                                      _addr(work), size, _stream(x)))
+  return out, pre
+
+
+def _slope(z, activation):
+  """act'(z) of float32 z, as torch operations."""
+  if activation == nat.ACTIVATIONS["relu"]:
+    return (z > 0).to(z.dtype)
+  if activation == nat.ACTIVATIONS["gelu"]:
+    return 0.5 * (1 + torch.erf(z * 0.5 ** 0.5)) + z * torch.exp(-0.5 * z * z) * (0.5 / torch.pi) ** 0.5
+  if activation == nat.ACTIVATIONS["gelu_tanh"]:
+    c = (2 / torch.pi) ** 0.5
+    t = torch.tanh(c * (z + 0.044715 * z ** 3))
+    return 0.5 * (1 + t) + 0.5 * z * (1 - t * t) * c * (1 + 3 * 0.044715 * z * z)
+  if activation == nat.ACTIVATIONS["silu"]:
+    s = torch.sigmoid(z)
+    return s * (1 + z * (1 - s))
+  return torch.ones_like(z)
+
+
+def _backward_torch(x, weight, bias, g, activation, needs):
+  """The gradients of x, weight and bias as torch operations, for backwards under create_graph (which
+  differentiate the pre-activation too: it is formed anew) or of batched gradients."""
+  dz = g.float()
+  if activation:
+    z = torch.mm(x.float(), weight.float().t())
+    dz = dz * _slope(z if bias is None else z + bias.float(), activation)
+  return (torch.mm(dz, weight.float()).to(g.dtype) if needs[0] else None,
+          torch.mm(dz.t(), x.float()).to(g.dtype) if needs[1] else None, dz.sum(0).to(g.dtype) if needs[2] else None)
+
+
+class _LinearAct(torch.autograd.Function):
+  """x [rows, ins]. Without an activation x is kept for the weight's gradient alone and the weight for x's;
+  with one the pre-activation is kept beside them."""
+
+  @staticmethod
+  def forward(ctx, x, weight, bias, residual, activation):
+    need_x, need_w, need_b = ctx.needs_input_grad[:3]
+    act = activation != 0 and (need_x or need_w or need_b)
+    out, pre = _forward(x, weight, bias, residual, activation, act)
+    ctx.save_for_backward(x if need_w or act else None, weight if need_x or act else None, bias if act else None, pre)
+    ctx.sizes, ctx.activation = (x.shape, weight.shape), activation
+    return out
+
+  @staticmethod
+  def backward(ctx, g):
+    x, weight, bias, pre = ctx.saved_tensors
+    (x_shape, w_shape), act = ctx.sizes, ctx.activation
+    needs = need_x, need_w, need_b = ctx.needs_input_grad[:3]
+    g_res = g if ctx.needs_input_grad[3] else None
+    if not any(needs):
+      return None, None, None, g_res, None
+    if as_torch(g):
+      return (*_backward_torch(x, weight, bias, g, act, needs), g_res, None)
+    g = g.contiguous()
+    outs, ins = w_shape
+    xr, xs = rows_of(x) if need_w else (None, 0)
+    wr, ws = rows_of(weight) if need_x else (None, 0)
+    d = nat.LinearDesc(x_shape[0], xs, ws, 0, ins, outs, _DTYPES[g.dtype], act)
+    L = nat.lib()
+    with torch.cuda.device(g.device):
+      gx, gw, gb = (torch.empty(shape, dtype=g.dtype, device=g.device) if need else None
+                    for shape, need in zip((x_shape, w_shape, (outs,)), needs))
+      work, size = _workspace(L.fwn_linear_act_bwd_workspace_size, d, g.device)
+      nat.check(L.fwn_linear_act_bwd_launch(d, _addr(xr), _addr(wr), _addr(pre), _addr(g), _addr(gx), _addr(gw), _addr(gb),
+                                            _addr(work), size, _stream(g)))
+    return gx, gw, gb, g_res, None
+
+
+def linear_act(x, weight, bias=None, *, activation=None, residual=None):
+  """act(x weight^T + bias) + residual for x [..., ins], weight [outs, ins], bias [outs] and residual
+  [..., outs], all float32 or all bfloat16: a Linear layer with its activation (None, "relu", "gelu",
+  "gelu_tanh" or "silu") and the residual's addition in the product's epilogue. Accumulated in float32 and
+  rounded once. Rows of any stride are read where they lie if their channels are contiguous.
+  Differentiable in x, weight, bias and residual."""
+  if not isinstance(x, torch.Tensor) or not x.is_cuda:
+    raise ValueError("x must be a CUDA tensor")
+  if x.dtype not in _DTYPES:
+    raise TypeError(f"x must be float32 or bfloat16, got {x.dtype}")
+  if not isinstance(weight, torch.Tensor) or weight.device != x.device:
+    raise ValueError("weight must be a tensor on the device of x")
+  if weight.dtype != x.dtype:
+    raise TypeError(f"weight must be {x.dtype}, got {weight.dtype}")
+  act = _activation(activation)
+  _check(x, weight, bias, residual, x.dtype, x.shape[:-1])
+  if not _needs(x, weight, bias, residual):
+    return _forward(x, weight, bias, residual, act, False)[0]
+  rows = lambda t: None if t is None else t.reshape(-1, t.shape[-1])
+  return _LinearAct.apply(rows(x), weight, bias, rows(residual), act).view(*x.shape[:-1], weight.shape[0])
+
+
+def linear_act_q8(x, x_scale, weight, weight_scale, bias=None, *, activation=None, residual=None, dtype=torch.bfloat16):
+  """linear_act of 8-bit operands: x [..., ins] and weight [outs, ins] are e4m3 values
+  (torch.float8_e4m3fn) with float32 scales x_scale [...] a row and weight_scale [outs] a column of the
+  output, as ``rms_norm_q8`` and ``quantize_rows`` give them; act((x weight^T) x_scale weight_scale + bias) +
+  residual in `dtype`, which bias and residual have. Forward only."""
+  if not isinstance(x, torch.Tensor) or not x.is_cuda:
+    raise ValueError("x must be a CUDA tensor")
+  if not isinstance(weight, torch.Tensor) or weight.device != x.device:
+    raise ValueError("weight must be a tensor on the device of x")
+  if x.dtype != _Q8 or weight.dtype != _Q8:
+    raise TypeError(f"x and weight must be {_Q8}, got {x.dtype} and {weight.dtype}")
+  if dtype not in _DTYPES:
+    raise TypeError(f"dtype must be float32 or bfloat16, got {dtype}")
+  act = _activation(activation)
+  lead = x.shape[:-1]
+  _check(x, weight, bias, residual, dtype, lead)
+  for t, name, shape in ((x_scale, "x_scale", lead), (weight_scale, "weight_scale", weight.shape[:1])):
+    if not isinstance(t, torch.Tensor) or t.device != x.device or t.shape != shape:
+      raise ValueError(f"{name} must be a tensor of shape {tuple(shape)} on the device of x")
+    if t.dtype != torch.float32:
+      raise TypeError(f"{name} must be float32, got {t.dtype}")
+  _no_grad("linear_act_q8", x_scale, weight_scale, bias, residual)
+  outs, ins = weight.shape
+  xr, xs = rows_of(x)
+  wr, ws = rows_of(weight)
+  rr, rs = rows_of(residual) if residual is not None else (None, 0)
+  bias = bias.contiguous() if bias is not None else None
+  x_scale, weight_scale = x_scale.contiguous(), weight_scale.contiguous()
+  L = nat.lib()
+  with torch.cuda.device(x.device):
+    out = torch.empty((*lead, outs), dtype=dtype, device=x.device)
+    d = nat.LinearDesc(x.numel() // ins, xs, ws, rs, ins, outs, _DTYPES[dtype], act)
+    work, size = _workspace(L.fwn_linear_act_q8_workspace_size, d, x.device)
+    nat.check(L.fwn_linear_act_q8_launch(d, _addr(xr), _addr(x_scale), _addr(wr), _addr(weight_scale), _addr(bias),
+                                         _addr(rr), _addr(out), _addr(work), size, _stream(x)))
+  return out

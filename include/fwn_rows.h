@@ -161,6 +161,50 @@ int fwn_rms_norm_bwd_launch(const fwn_rms_desc* d, const void* s, const void* we
                             const void* g_sum, void* gx, void* gw, void* workspace, uint64_t workspace_bytes,
                             void* stream);
 
+/* Matrix product with bias, activation and residual in its epilogue:
+ *   z = x weight^T + bias,  out = act(z) + residual
+ * x is [rows, ins], weight [outs, ins], residual [rows, outs], with contiguous rows x_stride, w_stride and
+ * r_stride elements apart (0: one row for all); bias [outs], out and pre [rows, outs] are contiguous.
+ * Products accumulate in float32; out, and pre (z for the backward, NULL: not stored) are rounded
+ * once. bias and residual may be NULL. Every tensor is of `dtype`; float32 products keep float32's precision. */
+#define FWN_ACT_NONE 0
+#define FWN_ACT_RELU 1
+#define FWN_ACT_GELU 2      /* z (1 + erf(z / sqrt 2)) / 2 */
+#define FWN_ACT_GELU_TANH 3 /* its tanh form */
+#define FWN_ACT_SILU 4      /* z / (1 + exp(-z)) */
+#define FWN_LINEAR_ACT_MAX (1 << 20) /* of ins and outs */
+
+typedef struct fwn_linear_desc {
+  int64_t rows;
+  int64_t x_stride, w_stride, r_stride;
+  int32_t ins, outs; /* 1 to FWN_LINEAR_ACT_MAX */
+  int32_t dtype;
+  int32_t activation;
+} fwn_linear_desc;
+
+/* Workspaces hold nothing between launches; 256-byte aligned. Launches that can overlap need their own. */
+int fwn_linear_act_workspace_size(const fwn_linear_desc* d, uint64_t* bytes);
+int fwn_linear_act_launch(const fwn_linear_desc* d, const void* x, const void* weight, const void* bias,
+                          const void* residual, void* out, void* pre, void* workspace, uint64_t workspace_bytes,
+                          void* stream);
+
+/* Gradients for the contiguous gradient g [rows, outs] of out: with dz = g act'(pre) (pre is read unless the
+ * activation is FWN_ACT_NONE; dz is rounded to the dtype for the products),
+ *   gx = dz weight [rows, ins],  gw = dz^T x [outs, ins],  gb = column sums of dz [outs]
+ * each contiguous and skipped where NULL. The residual's gradient is g. Sums run in a fixed order. */
+int fwn_linear_act_bwd_workspace_size(const fwn_linear_desc* d, uint64_t* bytes);
+int fwn_linear_act_bwd_launch(const fwn_linear_desc* d, const void* x, const void* weight, const void* pre,
+                              const void* g, void* gx, void* gw, void* gb, void* workspace, uint64_t workspace_bytes,
+                              void* stream);
+
+/* The forward of 8-bit operands: x and weight hold OCP e4m3 codes, z = (x weight^T) x_scale[row]
+ * w_scale[column] + bias with float32 scales (fwn_rms_norm_q8_launch, fwn_quantize_rows_launch). The
+ * descriptor's dtype is that of bias, residual and out. */
+int fwn_linear_act_q8_workspace_size(const fwn_linear_desc* d, uint64_t* bytes);
+int fwn_linear_act_q8_launch(const fwn_linear_desc* d, const uint8_t* x, const float* x_scale, const uint8_t* weight,
+                             const float* w_scale, const void* bias, const void* residual, void* out,
+                             void* workspace, uint64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }  /* extern "C" */
 #endif
