@@ -2,27 +2,72 @@
 //
 //   z = x w^T + b,  out = act(z) + residual;   dz = g act'(z),  gx = dz w,  gw = dz^T x,  gb = sum of dz
 //
-// One kernel for the three products: c[i, j] = sum over k of a(i, k) b(j, k) for operands of any strides.
+// One kernel for the three products c[i, j] = sum over k of a(i, k) b(j, k): an operand whose rows are
+// contiguous in k ("inner": x, w and dz in the first two) is read from LDS row by row, one whose rows are k
+// ("outer": w in gx, dz and x in gw) by transpose reads, and both arrive as the same MFMA operands.
+// float32 operands are laid out as three bf16 parts, 8 bits of the value each, and the product is the sum of
+// the six products of parts above 2^-24 of it, accumulated in float32 on the bf16 matrix units.
+#include "attn_bf16_tiles.h"
 #include "linear_act.h"
-
-#include "fwn_attn.h"
 
 namespace fwn {
 namespace {
 
-__device__ __forceinline__ float as_float(uint32_t u) { return __builtin_bit_cast(float, u); }
+typedef int i32x8 __attribute__((ext_vector_type(8)));
 
-__device__ __forceinline__ float load_one(const void* p, int64_t i, int type) {
-  if (type == kOpF32) return ((const float*)p)[i];
-  if (type == kOpBf16) return as_float((uint32_t)((const uint16_t*)p)[i] << 16);
-  return __builtin_amdgcn_cvt_f32_fp8((int)((const uint8_t*)p)[i], 0);
+__device__ __forceinline__ float as_float(uint32_t u) { return __builtin_bit_cast(float, u); }
+__device__ __forceinline__ uint32_t as_bits(float f) { return __builtin_bit_cast(uint32_t, f); }
+__device__ __forceinline__ uint32_t bf16_bits(float f) { return __builtin_bit_cast(uint16_t, (__bf16)f); }
+
+__device__ __forceinline__ float load_one(const void* p, int64_t i, int dtype) {
+  if (dtype == FWN_F32) return ((const float*)p)[i];
+  return as_float((uint32_t)((const uint16_t*)p)[i] << 16);
 }
 
-__device__ __forceinline__ void store_one(void* p, int64_t i, int type, float v) {
-  if (type == kOpF32)
+__device__ __forceinline__ void store_one(void* p, int64_t i, int dtype, float v) {
+  if (dtype == FWN_F32)
     ((float*)p)[i] = v;
   else
-    ((uint16_t*)p)[i] = __builtin_bit_cast(uint16_t, (__bf16)v);
+    ((uint16_t*)p)[i] = (uint16_t)bf16_bits(v);
+}
+
+// Eight consecutive elements, 16-byte aligned.
+__device__ __forceinline__ void load8(const void* p, int64_t i, int dtype, float (&f)[8]) {
+  if (dtype == FWN_F32) {
+    const u32x4* q = (const u32x4*)((const float*)p + i);
+    const u32x4 v0 = q[0], v1 = q[1];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t a = v0[k], b = v1[k];
+      f[k] = as_float(a);
+      f[4 + k] = as_float(b);
+    }
+  } else {
+    const u32x4 v = *(const u32x4*)((const uint16_t*)p + i);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t u = v[k];
+      f[2 * k] = as_float(u << 16);
+      f[2 * k + 1] = as_float(u & 0xffff0000u);
+    }
+  }
+}
+
+__device__ __forceinline__ u32x4 pack8(const float (&f)[8]) {
+  u32x4 v;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) v[k] = bf16_bits(f[2 * k]) | bf16_bits(f[2 * k + 1]) << 16;
+  return v;
+}
+
+__device__ __forceinline__ void store8(void* p, int64_t i, int dtype, const float (&f)[8]) {
+  if (dtype == FWN_F32) {
+    u32x4* q = (u32x4*)((float*)p + i);
+    q[0] = u32x4{as_bits(f[0]), as_bits(f[1]), as_bits(f[2]), as_bits(f[3])};
+    q[1] = u32x4{as_bits(f[4]), as_bits(f[5]), as_bits(f[6]), as_bits(f[7])};
+  } else {
+    *(u32x4*)((uint16_t*)p + i) = pack8(f);
+  }
 }
 
 __device__ __forceinline__ float activate(float z, int kind) {
@@ -54,69 +99,542 @@ __device__ __forceinline__ float slope(float z, int kind) {
   }
 }
 
-constexpr int TILE = 64, STEP = 16;
+// What the epilogue needs of the columns col .. col + 7.
+struct Columns {
+  float bias[8], scale[8];
 
-// 64 x 64 outputs by 256 threads, 4 x 4 a thread, 16 k at a time through LDS.
-__global__ void __launch_bounds__(256) product_kernel(ProductArgs a) {
-  __shared__ float sa[STEP][TILE + 1], sb[STEP][TILE + 1];
-  const int64_t tiles = (a.n + TILE - 1) / TILE;
-  const int64_t i0 = (int64_t)blockIdx.x / tiles * TILE, j0 = (int64_t)blockIdx.x % tiles * TILE;
-  const int ti = (int)threadIdx.x / 16, tj = (int)threadIdx.x % 16;
-  float acc[4][4] = {};
-  for (int64_t k0 = 0; k0 < a.k; k0 += STEP) {
-    for (int e = threadIdx.x; e < TILE * STEP; e += 256) {
-      const int r = e / STEP, k = e % STEP;
-      const bool in = k0 + k < a.k;
-      sa[k][r] = in && i0 + r < a.m ? load_one(a.a, (i0 + r) * a.a_row + (k0 + k) * a.a_k, a.op) : 0.f;
-      sb[k][r] = in && j0 + r < a.n ? load_one(a.b, (j0 + r) * a.b_row + (k0 + k) * a.b_k, a.op) : 0.f;
+  __device__ __forceinline__ void load(const EpilogueArgs& e, int64_t col) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const bool in = col + k < e.n;
+      bias[k] = e.bias && in ? load_one(e.bias, col + k, e.dtype) : 0.f;
+      scale[k] = e.b_scale && in ? e.b_scale[col + k] : 1.f;
     }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < STEP; ++k)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(sa[k][ti + 16 * i], sb[k][tj + 16 * j], acc[i][j]);
-    __syncthreads();
   }
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j) {
-      const int64_t row = i0 + ti + 16 * i, col = j0 + tj + 16 * j;
-      if (row >= a.m || col >= a.n) continue;
-      float z = acc[i][j];
-      if (a.a_scale) z *= a.a_scale[row] * a.b_scale[col];
-      if (a.bias) z += load_one(a.bias, col, a.dtype);
-      if (a.pre) store_one(a.pre, row * a.n + col, a.dtype, z);
-      z = activate(z, a.activation);
-      if (a.residual) z += load_one(a.residual, row * a.r_row + col, a.dtype);
-      store_one(a.out, row * a.n + col, a.dtype, z);
+};
+
+// The epilogue of z[row, col .. col + 7], row < m; columns from n on are dropped.
+__device__ __forceinline__ void finish(const EpilogueArgs& e, int64_t row, int64_t col, float (&v)[8], const Columns& c) {
+  if (e.a_scale) {
+    const float s = e.a_scale[row];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] *= s * c.scale[k];
+  }
+#pragma unroll
+  for (int k = 0; k < 8; ++k) v[k] += c.bias[k];
+  const int64_t at = row * e.n + col;
+  if (e.vec) {
+    if (col >= e.n) return;
+    if (e.pre) store8(e.pre, at, e.dtype, v);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = activate(v[k], e.activation);
+    if (e.residual) {
+      float r[8];
+      load8(e.residual, row * e.r_row + col, e.dtype, r);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] += r[k];
     }
+    store8(e.out, at, e.dtype, v);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if (col + k >= e.n) break;
+      if (e.pre) store_one(e.pre, at + k, e.dtype, v[k]);
+      float o = activate(v[k], e.activation);
+      if (e.residual) o += load_one(e.residual, row * e.r_row + col + k, e.dtype);
+      store_one(e.out, at + k, e.dtype, o);
+    }
+  }
 }
 
-__global__ void __launch_bounds__(64) slope_kernel(SlopeArgs a) {
-  const int c = (int)blockIdx.x * 64 + (int)threadIdx.x;
-  if (c >= a.outs) return;
-  float sum = 0.f;
-  for (int64_t r = 0; r < a.rows; ++r) {
-    const int64_t at = r * a.outs + c;
-    float dz = load_one(a.g, at, a.dtype);
-    if (a.activation) dz *= slope(load_one(a.pre, at, a.dtype), a.activation);
-    sum += dz;
-    if (a.dz) store_one(a.dz, at, a.dtype, dz);
+// Planes of a and b in each term of a product of parts, a digit a term from the right. The small terms come
+// first, where the accumulator's rounding hurts them least.
+constexpr uint32_t kPlaneA = 0x001102, kPlaneB = 0x010120;
+
+// An operand's float32 value at (row, k) from its three parts.
+template <bool OUTER>
+__device__ __forceinline__ float whole(const char* p, int64_t stride, int64_t plane, int64_t row, int64_t k) {
+  const char* q = OUTER ? p + k * stride + row * 2 : p + row * stride + k * 2;
+  float s = 0.f;
+  for (int i = 2; i >= 0; --i) s += as_float((uint32_t)*(const uint16_t*)(q + i * plane) << 16);
+  return s;
+}
+
+// Outputs of a product of parts that are NaN, formed from whole values: an infinity's parts beside it are
+// zeros, and so are those of a short number, whose product is NaN where the whole one is infinite.
+template <bool OA, bool OB>
+__device__ __forceinline__ void mend(const ProductArgs& g, int64_t row, int64_t col, float (&v)[8]) {
+  bool bad = false;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) bad |= v[e] != v[e] && col + e < g.e.n;
+  if (!bad) return;
+  float s[8] = {};
+  for (int64_t k = 0; k < g.k; ++k) {
+    const float x = whole<OA>(g.a, g.a_stride, g.a_plane, row, k);
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (col + e < g.e.n) s[e] = fmaf(x, whole<OB>(g.b, g.b_stride, g.b_plane, col + e, k), s[e]);
   }
-  if (a.gb) store_one(a.gb, c, a.dtype, sum);
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    if (v[e] != v[e]) v[e] = s[e];
+}
+
+// ------------------------------------------------------------------------------------------
+// Copies of an operand's stages into LDS, 1 KB a wave instruction, two a wave and stage.
+//   inner: 16 rows of 64 bytes; 16-byte chunk c of row r lies at c ^ 2 (r / 4 % 2), so that the eight rows
+//          and two chunks that a ds_read_b128 serves at once lie in sixteen different banks' groups;
+//   outer: 4 rows of k by 128 columns, in the swizzled layout of the transpose reads.
+// Rows and columns past the operand, k past the sum and stages past the range are copied as zeros: their
+// offsets lie past the buffer's end.
+constexpr uint32_t kNowhere = 0x80000000u, kBuffer = 0x7fffffffu;
+
+template <bool OUTER, int WAVES>
+struct Copy {
+  const char* base;  // of the tile
+  int64_t step;      // bytes from one stage to the next
+  int64_t plane;
+  uint32_t off[2], tail[2];  // of this lane's 16 bytes, and kNowhere where they lie past the sum in its last stage
+
+  // Tile from row (or column) `first` of `rows`; `k` elements of `size` bytes in the sum, whose last stage is `last`.
+  __device__ __forceinline__ void init(const char* p, int64_t stride, int64_t plane_bytes, int64_t first, int64_t rows,
+                                       int64_t k, int size, int64_t last, int w, int lane) {
+    plane = plane_bytes;
+    base = p + (OUTER ? first * 2 : first * stride);
+    step = OUTER ? kStageRows * stride : kStageBytes;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int q = w + WAVES * h;
+      if constexpr (OUTER) {
+        const int row = 4 * (q & 7) + lane / 16, chunk = (lane % 16) ^ swz<16>(row), col = (q >> 3) * 128 + chunk * 8;
+        off[h] = first + col < rows ? (uint32_t)row * (uint32_t)stride + (uint32_t)col * 2 : kNowhere;
+        tail[h] = last * kStageRows + row < k ? 0 : kNowhere;
+      } else {
+        const int row = 16 * q + lane / 4, chunk = (lane % 4) ^ (((lane >> 4) & 1) << 1);
+        off[h] = first + row < rows ? (uint32_t)row * (uint32_t)stride + (uint32_t)chunk * 16 : kNowhere;
+        tail[h] = last * kStageBytes + chunk * 16 < k * size ? 0 : kNowhere;
+      }
+    }
+  }
+
+  // Stage `t` of plane `p` to `dst`; `last` all ones: the sum's last stage; `none` kNowhere: zeros.
+  __device__ __forceinline__ void issue(lds_char* dst, int64_t t, int p, uint32_t last, uint32_t none, int w) const {
+    const rsrc_t r = make_rsrc(base + p * plane + t * step, kBuffer);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t o = off[h] | (tail[h] & last) | none;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(dst + (w + WAVES * h) * 1024),
+                                               16, (int)o, 0, 0, 0);
+    }
+  }
+};
+
+// LDS byte offsets of an operand's 32-row blocks for one wave: element [block][half of the 32 k].
+template <bool OUTER, int BLOCKS>
+struct Reads {
+  uint32_t at[BLOCKS][2];
+
+  __device__ __forceinline__ void init(uint32_t region, int first, int lane) {  // first: row or column of the tile
+    const int i = lane & 31, g = lane >> 5;
+#pragma unroll
+    for (int m = 0; m < BLOCKS; ++m) {
+      if constexpr (OUTER) {  // [h]: k 8 g + 4 h .. of a 16-k half; the other half 16 rows on
+        const int G = lane >> 4, t = lane & 15, e = t >> 2, q = t & 3, c0 = first + 32 * m;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int r = 8 * g + 4 * h + e, chunk = 4 * ((c0 & 127) >> 5) + 2 * (G & 1) + (q >> 1);
+          at[m][h] = region + (uint32_t)(c0 >> 7) * 8192 + r * 256 + ((chunk ^ swz<16>(r)) << 4) + (q & 1) * 8;
+        }
+      } else {
+        const int r = first + 32 * m + i;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) at[m][c] = region + r * 64 + (((2 * c + g) ^ (((r >> 2) & 1) << 1)) << 4);
+      }
+    }
+  }
+
+  __device__ __forceinline__ u32x4 read(const lds_char* stage, int m, int c) const {
+    if constexpr (OUTER) {
+      const u32x2 lo = tr_read(stage + c * 4096, at[m][0]), hi = tr_read(stage + c * 4096, at[m][1]);
+      return u32x4{lo[0], lo[1], hi[0], hi[1]};
+    } else {
+      return row_read(stage, at[m][c]);
+    }
+  }
+};
+
+// All but the newest `vm` of this wave's copies have landed and its LDS reads have returned.
+template <int vm>
+__device__ __forceinline__ void stage_barrier() {
+  __builtin_amdgcn_s_waitcnt(0x0070 | vm);
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+constexpr int kStrip = 72;  // floats from one row of a strip to the next: its halves' rows fall in other banks
+
+enum class Form { kBf16, kParts, kE4m3 };
+
+// One BM x BN tile of c over one range of the sum. A wave has 32 MI x 64 of the tile.
+template <bool OA, bool OB, Form FORM, int BM, int BN>
+__global__ void __launch_bounds__(2 * BM, 2) product_kernel(ProductArgs g) {
+  constexpr int WAVES = BM / 32, NI = 2, WN = BN / 64, WM = WAVES / WN, MI = BM / WM / 32;
+  constexpr int STAGE = (BM + BN) * kStageBytes;
+  constexpr bool E4M3 = FORM == Form::kE4m3, PARTS = FORM == Form::kParts;
+  static_assert(WAVES * 2 * 1024 == BM * 64 && BM == BN, "two copies a wave and operand");
+  // One array a stage: the compiler waits for the copies into the array that a read names, and for those alone.
+  __shared__ __align__(16) char lds0[STAGE], lds1[STAGE], lds2[STAGE], lds3[STAGE];
+  lds_char *const s0 = (lds_char*)lds0, *const s1 = (lds_char*)lds1, *const s2 = (lds_char*)lds2,
+           *const s3 = (lds_char*)lds3;
+  const int lane = (int)threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  // Workgroups go to the 8 XCDs in turn: each takes a contiguous range of (range of the sum, tile).
+  const int total = (int)gridDim.x, xcd = (int)blockIdx.x & 7, per = total >> 3, rem = total & 7;
+  const int id = xcd * per + (xcd < rem ? xcd : rem) + ((int)blockIdx.x >> 3);
+  const int tn = (int)((g.e.n + BN - 1) / BN), tiles = (int)((g.e.m + BM - 1) / BM) * tn;
+  const int split = id / tiles, tile = id - split * tiles;
+  const int64_t i0 = (int64_t)(tile / tn) * BM, j0 = (int64_t)(tile % tn) * BN;
+  const int size = E4M3 ? 1 : 2, per_stage = kStageBytes / size;
+  const int64_t stages = (g.k + per_stage - 1) / per_stage, t0 = (int64_t)split * g.chunk;
+  const int64_t t1 = t0 + g.chunk < stages ? t0 + g.chunk : stages;
+  const int steps = (int)(t1 - t0) * (PARTS ? 6 : 1);
+
+  Copy<OA, WAVES> ca;
+  Copy<OB, WAVES> cb;
+  ca.init(g.a, g.a_stride, g.a_plane, i0, g.e.m, g.k, size, stages - 1, w, lane);
+  cb.init(g.b, g.b_stride, g.b_plane, j0, g.e.n, g.k, size, stages - 1, w, lane);
+  int64_t at = t0;  // the stage copied next, and its term
+  uint32_t pa = PARTS ? kPlaneA : 0, pb = PARTS ? kPlaneB : 0;
+  int left = steps;
+  const auto copy = [&](lds_char* stage) {
+    const uint32_t none = left <= 0 ? kNowhere : 0, last = at == stages - 1 ? ~0u : 0;
+    ca.issue(stage, at, pa & 3, last, none, w);
+    cb.issue(stage + BM * kStageBytes, at, pb & 3, last, none, w);
+    --left;
+    if (++at == t1) {
+      at = t0;
+      pa >>= 4;
+      pb >>= 4;
+    }
+  };
+
+  const int wm = w / WN * (32 * MI), wn = w % WN * 64;  // this wave's part of the tile
+  Reads<OA, MI> ra;
+  Reads<OB, NI> rb;
+  ra.init(0, wm, lane);
+  rb.init(BM * kStageBytes, wn, lane);
+  f32x16 acc[MI][NI];
+#pragma unroll
+  for (int m = 0; m < MI; ++m)
+#pragma unroll
+    for (int n = 0; n < NI; ++n) acc[m][n] = zero16();
+  const auto read = [&](const lds_char* stage, int c, u32x4(&fa)[MI], u32x4(&fb)[NI]) {
+#pragma unroll
+    for (int m = 0; m < MI; ++m) fa[m] = ra.read(stage, m, c);
+#pragma unroll
+    for (int n = 0; n < NI; ++n) fb[n] = rb.read(stage, n, c);
+  };
+  u32x4 a0[MI], b0[NI], a1[MI], b1[NI];
+  const auto multiply = [&](const u32x4(&fa)[MI], const u32x4(&fb)[NI]) {
+#pragma unroll
+    for (int m = 0; m < MI; ++m)
+#pragma unroll
+      for (int n = 0; n < NI; ++n) acc[m][n] = mfma_bf16(fa[m], fb[n], acc[m][n]);
+  };
+  // The same for a whole stage of e4m3: 64 k, both halves of the rows' bytes, scales 2^0.
+  const auto multiply8 = [&](const u32x4(&la)[MI], const u32x4(&ha)[MI], const u32x4(&lb)[NI], const u32x4(&hb)[NI]) {
+    const auto join = [](const u32x4& x, const u32x4& y) {
+      return i32x8{(int)x[0], (int)x[1], (int)x[2], (int)x[3], (int)y[0], (int)y[1], (int)y[2], (int)y[3]};
+    };
+#pragma unroll
+    for (int m = 0; m < MI; ++m)
+#pragma unroll
+      for (int n = 0; n < NI; ++n)
+        acc[m][n] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(join(la[m], ha[m]), join(lb[n], hb[n]), acc[m][n], 0, 0,
+                                                                    0, 0x7f7f7f7f, 0, 0x7f7f7f7f);
+  };
+  // Column sums of a, in the workgroups of the first column tile: wave w takes 32 columns.
+  const bool sums = OA && g.sums != nullptr && j0 == 0 && w < BM / 32;
+  float sum = 0.f;
+  Reads<OA, 1> rs;
+  rs.init(0, 32 * (w < BM / 32 ? w : 0), lane);
+  const auto add = [&](const lds_char* stage) {
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const u32x4 v = rs.read(stage, 0, c);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t u = v[k];
+        sum += as_float(u << 16) + as_float(u & 0xffff0000u);
+      }
+    }
+  };
+
+  copy(s0);
+  copy(s1);
+  copy(s2);
+  stage_barrier<8>();  // s0
+  read(s0, 0, a0, b0);
+  const auto step = [&](lds_char* now, lds_char* next, lds_char* last) {
+    // The next stage has landed for every wave, and every wave has read all of the last one, whose place
+    // the stage after the two in flight takes.
+    stage_barrier<4>();
+    copy(last);
+    read(now, 1, a1, b1);
+    if constexpr (E4M3) {
+      multiply8(a0, a1, b0, b1);
+      read(next, 0, a0, b0);
+    } else {
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(a0, b0);
+      if constexpr (OA) {
+        if (sums) add(now);
+      }
+      read(next, 0, a0, b0);
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(a1, b1);
+    }
+  };
+  for (int t = 0; t < steps; t += 4) {  // stages past the last are zeros
+    step(s0, s1, s3);
+    step(s1, s2, s0);
+    step(s2, s3, s1);
+    step(s3, s0, s2);
+  }
+  wait_vmem();  // no copy outlives the stages
+  __syncthreads();
+
+  if constexpr (OA) {
+    if (sums) {
+      sum += __shfl_xor(sum, 32);
+      if (lane < 32 && i0 + 32 * w + lane < g.e.m) g.sums[(int64_t)split * g.e.m + i0 + 32 * w + lane] = sum;
+    }
+  }
+  // Through LDS, 32 rows of the wave's part at a time, to rows of eight columns a lane.
+  constexpr int PER = WAVES / 4;  // waves that share a stage's array
+  lds_char* const own = w / PER == 0 ? s0 : w / PER == 1 ? s1 : w / PER == 2 ? s2 : s3;
+  auto* const strip = (__attribute__((address_space(3))) float*)(own + (w % PER) * (32 * kStrip * 4));
+  const int j = lane & 31, half = lane >> 5;
+  const int64_t col = j0 + wn + 8 * (lane & 7);
+  Columns c;
+  if (!g.part) c.load(g.e, col);
+#pragma unroll
+  for (int m = 0; m < MI; ++m) {
+    if (i0 + wm + 32 * m >= g.e.m) break;
+#pragma unroll
+    for (int n = 0; n < NI; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) strip[(8 * (r >> 2) + 4 * half + (r & 3)) * kStrip + 32 * n + j] = acc[m][n][r];
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+    for (int p = 0; p < 4; ++p) {
+      const int64_t row = i0 + wm + 32 * m + 8 * p + (lane >> 3);
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = strip[(8 * p + (lane >> 3)) * kStrip + 8 * (lane & 7) + k];
+      if (row >= g.e.m || col >= g.e.n) continue;
+      if (g.part) {
+        store8(g.part, ((int64_t)split * g.e.m + row) * g.part_row + col, FWN_F32, v);
+      } else {
+        if constexpr (PARTS) mend<OA, OB>(g, row, col, v);
+        finish(g.e, row, col, v, c);
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+// The partial products added in the order of the splits, then the epilogue: eight columns a thread.
+template <bool OA, bool OB, Form FORM>
+__global__ void __launch_bounds__(256) join_kernel(ProductArgs g) {
+  const int64_t across = g.part_row / 8, id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t row = id / across, col = (id - row * across) * 8;
+  if (row >= g.e.m) return;
+  float v[8] = {};
+#pragma unroll 4
+  for (int s = 0; s < g.splits; ++s) {
+    float p[8];
+    load8(g.part, ((int64_t)s * g.e.m + row) * g.part_row + col, FWN_F32, p);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] += p[k];
+  }
+  Columns c;
+  c.load(g.e, col);
+  if constexpr (FORM == Form::kParts) mend<OA, OB>(g, row, col, v);
+  finish(g.e, row, col, v, c);
+}
+
+template <bool OA, bool OB, Form FORM, int BM, int BN>
+hipError_t launch_tile(const ProductArgs& g, hipStream_t stream) {
+  const int64_t tiles = ((g.e.m + BM - 1) / BM) * ((g.e.n + BN - 1) / BN);
+  hipLaunchKernelGGL((product_kernel<OA, OB, FORM, BM, BN>), dim3((unsigned)(tiles * g.splits)), dim3(2 * BM), 0, stream, g);
+  if (hipError_t e = hipGetLastError(); e != hipSuccess || !g.part) return e;
+  const int64_t threads = g.e.m * (g.part_row / 8);
+  hipLaunchKernelGGL((join_kernel<OA, OB, FORM>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, stream, g);
+  return hipGetLastError();
+}
+
+template <bool OA, bool OB, Form FORM>
+hipError_t launch_operands(int tile, const ProductArgs& g, hipStream_t stream) {
+  if (tile == 0) return launch_tile<OA, OB, FORM, 256, 256>(g, stream);
+  return launch_tile<OA, OB, FORM, 128, 128>(g, stream);
+}
+
+template <Form FORM>
+hipError_t launch_kind(Operands how, int tile, const ProductArgs& g, hipStream_t stream) {
+  if (how == Operands::kInnerInner) return launch_operands<false, false, FORM>(tile, g, stream);
+  if (how == Operands::kInnerOuter) return launch_operands<false, true, FORM>(tile, g, stream);
+  return launch_operands<true, true, FORM>(tile, g, stream);
+}
+
+// ------------------------------------------------------------------------------------------
+// Layouts. A thread forms 16 bytes of each plane of a row.
+
+// Eight values of a row as the product kernel reads them: rounded to bf16, or three parts of 8 bits each.
+__device__ __forceinline__ void store_parts(char* dst, int64_t plane, bool parts, const float (&f)[8]) {
+  if (!parts) {
+    *(u32x4*)dst = pack8(f);
+    return;
+  }
+  u32x4 hi, mid, lo;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    uint32_t h[2], m[2], l[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const float v = f[2 * k + e];
+      const uint32_t u = as_bits(v);
+      if ((u & 0x7f800000u) == 0x7f800000u) {  // an infinity, or a NaN whose bits may all lie in the cut part
+        h[e] = u << 9 ? 0x7fc0u : u >> 16;
+        m[e] = l[e] = 0;
+        continue;
+      }
+      const float r1 = v - as_float(u & 0xffff0000u);
+      const uint32_t u1 = as_bits(r1);
+      const float r2 = r1 - as_float(u1 & 0xffff0000u);
+      h[e] = u >> 16;
+      m[e] = u1 >> 16;
+      l[e] = as_bits(r2) >> 16;
+    }
+    hi[k] = h[0] | h[1] << 16;
+    mid[k] = m[0] | m[1] << 16;
+    lo[k] = l[0] | l[1] << 16;
+  }
+  *(u32x4*)dst = hi;
+  *(u32x4*)(dst + plane) = mid;
+  *(u32x4*)(dst + 2 * plane) = lo;
+}
+
+__global__ void __launch_bounds__(256) layout_kernel(LayoutArgs a) {
+  const int per = a.op == kOpE4m3 ? 16 : 8;  // columns a thread
+  const int64_t across = (a.cols + per - 1) / per, id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t row = id / across, col = (id - row * across) * per;
+  if (row >= a.rows) return;
+  char* dst = a.dst + row * a.dst_stride + (id - row * across) * 16;
+  if (a.op == kOpE4m3) {
+    const uint8_t* p = (const uint8_t*)a.src + row * a.stride + col;
+    uint32_t d[4] = {};
+#pragma unroll
+    for (int k = 0; k < 16; ++k)
+      if (col + k < a.cols) d[k / 4] |= (uint32_t)p[k] << 8 * (k % 4);
+    *(u32x4*)dst = u32x4{d[0], d[1], d[2], d[3]};
+    return;
+  }
+  float f[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k)
+    f[k] = col + k < a.cols ? load_one(a.src, row * a.stride + col + k, a.op == kOpF32 ? FWN_F32 : FWN_BF16) : 0.f;
+  store_parts(dst, a.dst_plane, a.op == kOpF32, f);
+}
+
+// 256 columns by `chunk` rows a workgroup, eight columns of every eighth row a thread.
+__global__ void __launch_bounds__(256) slope_kernel(SlopeArgs a) {
+  __shared__ float red[8][256];
+  const int across = (a.outs + 255) / 256, block = (int)blockIdx.x / across;
+  const int lane = (int)threadIdx.x & 31, own = (int)threadIdx.x >> 5;
+  const int col = ((int)blockIdx.x - block * across) * 256 + 8 * lane;
+  const int64_t r0 = (int64_t)block * a.chunk, r1 = r0 + a.chunk < a.rows ? r0 + a.chunk : a.rows;
+  const bool vec = a.outs % 8 == 0 && (((uintptr_t)a.g | (uintptr_t)a.pre) & 15) == 0;
+  float sum[8] = {};
+  if (col < a.outs) {
+    for (int64_t r = r0 + own; r < r1; r += 8) {
+      const int64_t at = r * a.outs + col;
+      float dz[8], z[8];
+      if (vec) {
+        load8(a.g, at, a.dtype, dz);
+        if (a.activation) load8(a.pre, at, a.dtype, z);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const bool in = col + k < a.outs;
+          dz[k] = in ? load_one(a.g, at + k, a.dtype) : 0.f;
+          z[k] = in && a.activation ? load_one(a.pre, at + k, a.dtype) : 0.f;
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        if (a.activation) dz[k] *= slope(z[k], a.activation);
+        sum[k] += dz[k];
+      }
+      if (a.dz) store_parts(a.dz + r * a.dz_stride + (int64_t)col * 2, a.dz_plane, a.dtype == FWN_F32, dz);
+    }
+  }
+  if (!a.part) return;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) red[own][8 * lane + k] = sum[k];
+  __syncthreads();
+  const int c = (int)threadIdx.x, to = col - 8 * lane + c;
+  if (to >= a.outs) return;
+  float s = red[0][c];
+#pragma unroll
+  for (int k = 1; k < 8; ++k) s += red[k][c];
+  a.part[(int64_t)block * a.outs + to] = s;
+}
+
+constexpr int kGroups = 16;  // shares of the partial rows that a workgroup adds in parallel
+
+__global__ void __launch_bounds__(64 * kGroups) column_sums_kernel(const float* part, int64_t count, int64_t n, void* out,
+                                                                   int dtype) {
+  __shared__ float red[kGroups][64];
+  const int lane = threadIdx.x & 63, grp = (int)threadIdx.x >> 6;
+  const int64_t c = (int64_t)blockIdx.x * 64 + lane;
+  float s = 0.f;
+  if (c < n) {
+#pragma unroll 8
+    for (int64_t b = grp; b < count; b += kGroups) s += part[b * n + c];
+  }
+  red[grp][lane] = s;
+  __syncthreads();
+  if (grp != 0 || c >= n) return;
+#pragma unroll
+  for (int k = 1; k < kGroups; ++k) s += red[k][lane];
+  store_one(out, c, dtype, s);
 }
 
 }  // namespace
 
-hipError_t launch_product(const ProductArgs& a, hipStream_t stream) {
-  const int64_t blocks = ((a.m + TILE - 1) / TILE) * ((a.n + TILE - 1) / TILE);
-  hipLaunchKernelGGL(product_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, a);
+hipError_t launch_product(Operands how, int32_t op, int tile, const ProductArgs& a, hipStream_t stream) {
+  if (op == kOpE4m3) return launch_operands<false, false, Form::kE4m3>(tile, a, stream);
+  return op == kOpF32 ? launch_kind<Form::kParts>(how, tile, a, stream) : launch_kind<Form::kBf16>(how, tile, a, stream);
+}
+
+hipError_t launch_layout(const LayoutArgs& a, hipStream_t stream) {
+  const int per = a.op == kOpE4m3 ? 16 : 8;
+  const int64_t threads = a.rows * ((a.cols + per - 1) / per);
+  if (threads == 0) return hipSuccess;
+  hipLaunchKernelGGL(layout_kernel, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, stream, a);
   return hipGetLastError();
 }
 
 hipError_t launch_slope(const SlopeArgs& a, hipStream_t stream) {
-  hipLaunchKernelGGL(slope_kernel, dim3((unsigned)(a.outs + 63) / 64), dim3(64), 0, stream, a);
+  const unsigned across = (unsigned)(a.outs + 255) / 256;
+  hipLaunchKernelGGL(slope_kernel, dim3(across * (unsigned)a.blocks), dim3(256), 0, stream, a);
+  return hipGetLastError();
+}
+
+hipError_t launch_column_sums(const float* part, int64_t count, int64_t n, void* out, int dtype, hipStream_t stream) {
+  hipLaunchKernelGGL(column_sums_kernel, dim3((unsigned)((n + 63) / 64)), dim3(64 * kGroups), 0, stream, part, count, n,
+                     out, dtype);
   return hipGetLastError();
 }
 

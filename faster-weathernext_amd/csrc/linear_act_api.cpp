@@ -1,4 +1,5 @@
 // C ABI of the linear layers with an epilogue (fwn_rows.h): host-side validation, then the launches.
+#include <algorithm>
 #include <cstdint>
 
 #include <hip/hip_runtime.h>
@@ -26,8 +27,10 @@ int check_desc(const fwn_linear_desc* d, const char* what) {
       d->r_stride > widest)
     return fail(FWN_ERR_INVALID_ARG, "%s: strides %lld, %lld and %lld", what, (long long)d->x_stride,
                 (long long)d->w_stride, (long long)d->r_stride);
-  const int64_t tiles = ((d->rows + 63) / 64) * (((d->outs > d->ins ? d->outs : d->ins) + 63) / 64);
-  if (tiles > (1 << 23)) return fail(FWN_ERR_INVALID_ARG, "%s: too many rows for one launch", what);
+  const int64_t ins = (d->ins + 63) / 64, outs = (d->outs + 63) / 64, rows = (d->rows + 63) / 64, most = 1 << 23;
+  if (rows * ins > most || rows * outs > most || ins * outs > most)
+    return fail(FWN_ERR_INVALID_ARG, "%s: %lld rows, ins %d and outs %d are too many for one launch", what,
+                (long long)d->rows, d->ins, d->outs);
   return FWN_OK;
 }
 
@@ -69,14 +72,137 @@ int status(hipError_t e, const char* what) {
   return e == hipSuccess ? FWN_OK : fail(FWN_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
 }
 
+constexpr int64_t kCus = 256;
+
+int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+int64_t parts(int64_t v, int64_t of) { return (v + of - 1) / of; }
+
+int64_t op_size(int32_t op) { return op == kOpE4m3 ? 1 : op == kOpBf16 ? 2 : 4; }
+
+// Hands out pieces of a workspace (base NULL: only counts them).
+struct Workspace {
+  char* base;
+  uint64_t used = 0;
+  char* take(uint64_t bytes) {
+    char* p = base ? base + used : nullptr;
+    used += (uint64_t)up((int64_t)bytes, 256);
+    return p;
+  }
+};
+
+// A matrix in rows as the product kernel reads it: as it lies where it is bf16 or e4m3 in whole aligned 16
+// bytes, else laid out in the workspace.
+struct Matrix {
+  const void* src;
+  int64_t rows, cols, stride;  // elements
+  int32_t op;
+  char* at;                    // laid out: where
+  int64_t row_bytes, plane;
+  bool laid;
+
+  void place(const void* p, int64_t r, int64_t c, int64_t s, int32_t o, Workspace& ws, bool force = false) {
+    src = p, rows = r, cols = c, stride = s, op = o, plane = 0;
+    const int64_t size = op_size(op);
+    laid = force || op == kOpF32 || ((uintptr_t)p & 15) || c * size % 16 || s * size % 16 || s * size > kMaxStride;
+    if (!laid) {
+      row_bytes = s * size;
+      at = (char*)p;
+      return;
+    }
+    plane = up(c * (op == kOpE4m3 ? 1 : 2), 16);
+    row_bytes = op == kOpF32 ? 3 * plane : plane;
+    at = ws.take((uint64_t)(rows * row_bytes));
+  }
+
+  hipError_t lay_out(hipStream_t stream) const {
+    if (!laid) return hipSuccess;
+    return launch_layout({src, rows, cols, stride, op, at, row_bytes, plane}, stream);
+  }
+};
+
+// The tiles and ranges of the sum of one product. The estimate is the rounds of workgroups over the CUs times
+// the time of one: its share of the matrix units' time (a 128 x 128 tile's stage takes a fifth longer for its area),
+// its start and its end, and for split sums the partial products' trip through memory.
+struct Plan {
+  int tile;
+  int32_t splits, chunk;
+};
+
+Plan plan(int64_t m, int64_t n, int64_t k, int32_t op) {
+  const int64_t stages = std::max<int64_t>(1, parts(k * (op == kOpE4m3 ? 1 : 2), kStageBytes));
+  Plan best{0, 1, (int32_t)stages};
+  double least = 0;
+  for (int t = 0; t < kTileShapes; ++t) {
+    const int64_t tiles = parts(m, kTiles[t].m) * parts(n, kTiles[t].n);
+    const double per_stage = (t == 0 ? 0.5 : 0.15) * (op == kOpF32 ? 6 : 1), ends = t == 0 ? 6.0 : 3.0;  // us
+    for (int64_t want = 1; want <= 64; want *= 2) {
+      const int64_t chunk = parts(stages, want), splits = parts(stages, chunk);
+      if (splits != want && want > 1) continue;
+      if (want > 1 && chunk < 4) break;
+      const double join = splits > 1 ? 4.0 + (double)(splits + 1) * m * n * 4 / 4e6 : 0;
+      const double time = (double)parts(tiles * splits, kCus) * (per_stage * chunk + ends) + join;
+      if ((t == 0 && want == 1) || time < least) {
+        least = time;
+        best = {t, (int32_t)splits, (int32_t)chunk};
+      }
+    }
+  }
+  return best;
+}
+
+// One product's launch: its plan, operands and workspace.
+struct Product {
+  ProductArgs g{};
+  Operands how;
+  int32_t op;
+  Plan p;
+
+  // Sizes and plan; `sums`: the column sums of a are wanted.
+  void shape(Operands h, int64_t m, int64_t n, int64_t k, int32_t o, bool sums, Workspace& ws) {
+    how = h, op = o;
+    p = plan(m, n, k, op);
+    g.k = k;
+    g.splits = p.splits;
+    g.chunk = p.chunk;
+    g.e.m = m;
+    g.e.n = n;
+    g.part_row = up(n, 8);
+    g.part = p.splits > 1 ? (float*)ws.take((uint64_t)p.splits * m * g.part_row * sizeof(float)) : nullptr;
+    g.sums = sums ? (float*)ws.take((uint64_t)p.splits * m * sizeof(float)) : nullptr;
+  }
+  hipError_t launch(const Matrix& a, const Matrix& b, hipStream_t stream) {
+    g.a = a.at, g.a_stride = a.row_bytes, g.a_plane = a.plane;
+    g.b = b.at, g.b_stride = b.row_bytes, g.b_plane = b.plane;
+    const EpilogueArgs& e = g.e;
+    g.e.vec = e.n % 8 == 0 && (!e.residual || e.r_row % 8 == 0) &&
+              (((uintptr_t)e.out | (uintptr_t)e.pre | (uintptr_t)e.residual) & 15) == 0;
+    return launch_product(how, op, p.tile, g, stream);
+  }
+};
+
+// Where everything of one forward launch lies; without a workspace, how large that has to be.
+struct Forward {
+  Matrix x, w;
+  Product z;
+  uint64_t bytes;
+
+  Forward(const fwn_linear_desc* d, int32_t op, const void* xp, const void* wp, void* workspace) {
+    Workspace ws{(char*)workspace};
+    x.place(xp, d->rows, d->ins, d->x_stride, op, ws);
+    w.place(wp, d->outs, d->ins, d->w_stride, op, ws);
+    z.shape(Operands::kInnerInner, d->rows, d->outs, d->ins, op, false, ws);
+    bytes = ws.used;
+  }
+};
+
 int forward(const fwn_linear_desc* d, int32_t op, const void* x, const float* x_scale, const void* weight,
-            const float* w_scale, const void* bias, const void* residual, void* out, void* pre, void* stream,
-            const char* what) {
+            const float* w_scale, const void* bias, const void* residual, void* out, void* pre, void* workspace,
+            uint64_t workspace_bytes, void* stream, const char* what) {
   if (int rc = check_desc(d, what)) return rc;
   if (d->rows == 0) return FWN_OK;
   if (!x || !weight || !out || (op == kOpE4m3 && (!x_scale || !w_scale)))
     return fail(FWN_ERR_INVALID_ARG, "%s: null argument", what);
-  const uint64_t size = size_of(d->dtype), in_size = op == kOpE4m3 ? 1 : size;
+  const uint64_t size = size_of(d->dtype), in_size = (uint64_t)op_size(op);
   if (misaligned(x, in_size) || misaligned(weight, in_size) || misaligned(x_scale, 4) || misaligned(w_scale, 4) ||
       misaligned(bias, size) || misaligned(residual, size) || misaligned(out, size) || misaligned(pre, size))
     return fail(FWN_ERR_INVALID_ARG, "%s: a tensor is not aligned to its elements", what);
@@ -85,31 +211,61 @@ int forward(const fwn_linear_desc* d, int32_t op, const void* x, const float* x_
                       span(residual, d->rows, d->r_stride, d->outs, size)};
   const Span outs[] = {span(out, d->rows, d->outs, d->outs, size), span(pre, d->rows, d->outs, d->outs, size)};
   if (int rc = check_overlap(ins, outs, what)) return rc;
-  ProductArgs a{};
-  a.a = x;
-  a.b = weight;
-  a.a_row = d->x_stride;
-  a.b_row = d->w_stride;
-  a.a_k = a.b_k = 1;
-  a.m = d->rows;
-  a.n = d->outs;
-  a.k = d->ins;
-  a.op = op;
-  a.dtype = d->dtype;
-  a.a_scale = x_scale;
-  a.b_scale = w_scale;
-  a.bias = bias;
-  a.residual = residual;
-  a.r_row = d->r_stride;
-  a.out = out;
-  a.pre = pre;
-  a.activation = d->activation;
-  return status(launch_product(a, (hipStream_t)stream), what);
+  Forward f(d, op, x, weight, workspace);
+  if (int rc = check_workspace(workspace, workspace_bytes, f.bytes, what)) return rc;
+  EpilogueArgs& e = f.z.g.e;
+  e.a_scale = x_scale;
+  e.b_scale = w_scale;
+  e.bias = bias;
+  e.residual = residual;
+  e.r_row = d->r_stride;
+  e.out = out;
+  e.pre = pre;
+  e.dtype = d->dtype;
+  e.activation = d->activation;
+  const hipStream_t s = (hipStream_t)stream;
+  if (int rc = status(f.x.lay_out(s), what)) return rc;
+  if (int rc = status(f.w.lay_out(s), what)) return rc;
+  return status(f.z.launch(f.x, f.w, s), what);
 }
 
-uint64_t bwd_bytes(const fwn_linear_desc* d) {
-  return d->activation == FWN_ACT_NONE ? 0 : (uint64_t)d->rows * (uint64_t)d->outs * size_of(d->dtype);
+// Workgroups by rows of the dz pass: about four workgroups a CU, 32 rows at least.
+int64_t slope_chunk(int64_t rows, int64_t outs) {
+  const int64_t blocks = std::max<int64_t>(1, std::min(4 * kCus / parts(outs, 256), parts(rows, 32)));
+  return std::max<int64_t>(1, parts(rows, blocks));
 }
+
+// The backward: dz (g itself where it is bf16 without an activation), its column sums, and the two products. The
+// sums come from the weight gradient's product where that reads g itself, else from the pass that forms dz.
+struct Backward {
+  Matrix dz, w, x;
+  Product to_x, to_w;
+  SlopeArgs slope{};
+  bool formed, sums_in_product;
+  uint64_t bytes;
+
+  Backward(const fwn_linear_desc* d, const void* xp, const void* wp, const void* gp, bool need_x, bool need_w, bool need_b,
+           void* workspace) {
+    Workspace ws{(char*)workspace};
+    const int32_t op = d->dtype == FWN_F32 ? kOpF32 : kOpBf16;
+    const bool act = d->activation != FWN_ACT_NONE, products = need_x || need_w;
+    dz.place(gp, d->rows, d->outs, d->outs, op, ws, act);
+    formed = products && dz.laid;
+    sums_in_product = need_b && need_w && !formed;
+    slope.chunk = slope_chunk(d->rows, d->outs);
+    slope.blocks = (int32_t)std::max<int64_t>(1, parts(d->rows, slope.chunk));
+    if (need_b && !sums_in_product) slope.part = (float*)ws.take((uint64_t)slope.blocks * d->outs * sizeof(float));
+    if (need_x) {
+      w.place(wp, d->outs, d->ins, d->w_stride, op, ws);
+      to_x.shape(Operands::kInnerOuter, d->rows, d->ins, d->outs, op, false, ws);
+    }
+    if (need_w) {
+      x.place(xp, d->rows, d->ins, d->x_stride, op, ws);
+      to_w.shape(Operands::kOuterOuter, d->outs, d->ins, d->rows, op, sums_in_product, ws);
+    }
+    bytes = ws.used;
+  }
+};
 
 int size_query(const fwn_linear_desc* d, uint64_t* bytes, const char* what) {
   clear_error();
@@ -123,8 +279,11 @@ int size_query(const fwn_linear_desc* d, uint64_t* bytes, const char* what) {
 
 extern "C" {
 
-int fwn_linear_act_workspace_size(const fwn_linear_desc* d, uint64_t* bytes) {
-  return fwn::size_query(d, bytes, "fwn_linear_act_workspace_size");
+int fwn_linear_act_workspace_size(const fwn_linear_desc* d, const void* x, const void* weight, uint64_t* bytes) {
+  using namespace fwn;
+  if (int rc = size_query(d, bytes, "fwn_linear_act_workspace_size")) return rc;
+  *bytes = Forward(d, d->dtype == FWN_F32 ? kOpF32 : kOpBf16, x, weight, nullptr).bytes;
+  return FWN_OK;
 }
 
 int fwn_linear_act_launch(const fwn_linear_desc* d, const void* x, const void* weight, const void* bias,
@@ -132,13 +291,15 @@ int fwn_linear_act_launch(const fwn_linear_desc* d, const void* x, const void* w
                           void* stream) {
   using namespace fwn;
   clear_error();
-  (void)workspace, (void)workspace_bytes;
   return forward(d, d && d->dtype == FWN_F32 ? kOpF32 : kOpBf16, x, nullptr, weight, nullptr, bias, residual, out, pre,
-                 stream, "fwn_linear_act_launch");
+                 workspace, workspace_bytes, stream, "fwn_linear_act_launch");
 }
 
-int fwn_linear_act_q8_workspace_size(const fwn_linear_desc* d, uint64_t* bytes) {
-  return fwn::size_query(d, bytes, "fwn_linear_act_q8_workspace_size");
+int fwn_linear_act_q8_workspace_size(const fwn_linear_desc* d, const uint8_t* x, const uint8_t* weight, uint64_t* bytes) {
+  using namespace fwn;
+  if (int rc = size_query(d, bytes, "fwn_linear_act_q8_workspace_size")) return rc;
+  *bytes = Forward(d, kOpE4m3, x, weight, nullptr).bytes;
+  return FWN_OK;
 }
 
 int fwn_linear_act_q8_launch(const fwn_linear_desc* d, const uint8_t* x, const float* x_scale, const uint8_t* weight,
@@ -146,15 +307,15 @@ int fwn_linear_act_q8_launch(const fwn_linear_desc* d, const uint8_t* x, const f
                              void* workspace, uint64_t workspace_bytes, void* stream) {
   using namespace fwn;
   clear_error();
-  (void)workspace, (void)workspace_bytes;
-  return forward(d, kOpE4m3, x, x_scale, weight, w_scale, bias, residual, out, nullptr, stream,
-                 "fwn_linear_act_q8_launch");
+  return forward(d, kOpE4m3, x, x_scale, weight, w_scale, bias, residual, out, nullptr, workspace, workspace_bytes,
+                 stream, "fwn_linear_act_q8_launch");
 }
 
-int fwn_linear_act_bwd_workspace_size(const fwn_linear_desc* d, uint64_t* bytes) {
+int fwn_linear_act_bwd_workspace_size(const fwn_linear_desc* d, const void* x, const void* weight, const void* g,
+                                      const void* gx, const void* gw, const void* gb, uint64_t* bytes) {
   using namespace fwn;
   if (int rc = size_query(d, bytes, "fwn_linear_act_bwd_workspace_size")) return rc;
-  *bytes = bwd_bytes(d);
+  *bytes = Backward(d, x, weight, g, gx && d->rows > 0, gw != nullptr, gb != nullptr, nullptr).bytes;
   return FWN_OK;
 }
 
@@ -176,47 +337,37 @@ int fwn_linear_act_bwd_launch(const fwn_linear_desc* d, const void* x, const voi
   const Span outs[] = {span(gx, d->rows, d->ins, d->ins, size), span(gw, d->outs, d->ins, d->ins, size),
                        span(gb, 1, 0, d->outs, size)};
   if (int rc = check_overlap(ins, outs, what)) return rc;
-  if (int rc = check_workspace(workspace, workspace_bytes, bwd_bytes(d), what)) return rc;
+  Backward b(d, x, weight, g, gx && d->rows > 0, gw != nullptr, gb != nullptr, workspace);
+  if (int rc = check_workspace(workspace, workspace_bytes, b.bytes, what)) return rc;
   const hipStream_t s = (hipStream_t)stream;
-  if (gb || act) {
-    SlopeArgs a{};
+  if (b.formed || (gb && !b.sums_in_product)) {
+    SlopeArgs& a = b.slope;
     a.g = g;
     a.pre = pre;
-    a.dz = act ? workspace : nullptr;
-    a.gb = gb;
+    a.dz = b.formed ? b.dz.at : nullptr;
+    a.dz_stride = b.dz.row_bytes;
+    a.dz_plane = b.dz.plane;
     a.rows = d->rows;
     a.outs = d->outs;
     a.dtype = d->dtype;
     a.activation = d->activation;
     if (int rc = status(launch_slope(a, s), what)) return rc;
+    if (gb)
+      if (int rc = status(launch_column_sums(a.part, a.blocks, d->outs, gb, d->dtype, s), what)) return rc;
   }
-  ProductArgs a{};
-  a.a = act ? workspace : g;
-  a.op = d->dtype == FWN_F32 ? kOpF32 : kOpBf16;
-  a.dtype = d->dtype;
   if (gx && d->rows > 0) {
-    a.b = weight;
-    a.a_row = d->outs;
-    a.a_k = 1;
-    a.b_row = 1;
-    a.b_k = d->w_stride;
-    a.m = d->rows;
-    a.n = d->ins;
-    a.k = d->outs;
-    a.out = gx;
-    if (int rc = status(launch_product(a, s), what)) return rc;
+    if (int rc = status(b.w.lay_out(s), what)) return rc;
+    b.to_x.g.e.out = gx;
+    b.to_x.g.e.dtype = d->dtype;
+    if (int rc = status(b.to_x.launch(b.dz, b.w, s), what)) return rc;
   }
   if (gw) {
-    a.b = x;
-    a.a_row = 1;
-    a.a_k = d->outs;
-    a.b_row = 1;
-    a.b_k = d->x_stride;
-    a.m = d->outs;
-    a.n = d->ins;
-    a.k = d->rows;
-    a.out = gw;
-    if (int rc = status(launch_product(a, s), what)) return rc;
+    if (int rc = status(b.x.lay_out(s), what)) return rc;
+    b.to_w.g.e.out = gw;
+    b.to_w.g.e.dtype = d->dtype;
+    if (int rc = status(b.to_w.launch(b.dz, b.x, s), what)) return rc;
+    if (b.sums_in_product)
+      if (int rc = status(launch_column_sums(b.to_w.g.sums, b.to_w.p.splits, d->outs, gb, d->dtype, s), what)) return rc;
   }
   return FWN_OK;
 }

@@ -150,11 +150,11 @@ SIGNATURES = {
     "fwn_quantize_rows_launch": [_RMS, _P, _P, _P, _P],
     "fwn_rms_norm_bwd_workspace_size": [_RMS, _P],
     "fwn_rms_norm_bwd_launch": [_RMS, _P, _P, _P, _P, _P, _P, _P, _U64, _P],
-    "fwn_linear_act_workspace_size": [_LIN, _P],
+    "fwn_linear_act_workspace_size": [_LIN, _P, _P, _P],
     "fwn_linear_act_launch": [_LIN, _P, _P, _P, _P, _P, _P, _P, _U64, _P],
-    "fwn_linear_act_bwd_workspace_size": [_LIN, _P],
+    "fwn_linear_act_bwd_workspace_size": [_LIN, _P, _P, _P, _P, _P, _P, _P],
     "fwn_linear_act_bwd_launch": [_LIN, _P, _P, _P, _P, _P, _P, _P, _P, _U64, _P],
-    "fwn_linear_act_q8_workspace_size": [_LIN, _P],
+    "fwn_linear_act_q8_workspace_size": [_LIN, _P, _P, _P],
     "fwn_linear_act_q8_launch": [_LIN, _P, _P, _P, _P, _P, _P, _P, _P, _U64, _P],
 }
 

@@ -37,9 +37,9 @@ def _activation(name):
   return nat.ACTIVATIONS[name]
 
 
-def _workspace(query, d, device):
+def _workspace(query, d, device, *tensors):
   size = ctypes.c_uint64(0)
-  nat.check(query(d, ctypes.byref(size)))
+  nat.check(query(d, *(_addr(t) for t in tensors), ctypes.byref(size)))
   return (torch.empty(size.value, dtype=torch.uint8, device=device) if size.value else None), size.value
 
 
@@ -55,7 +55,7 @@ def _forward(x, weight, bias, residual, activation, keep):
     out = torch.empty((*lead, outs), dtype=x.dtype, device=x.device)
     pre = torch.empty_like(out) if keep else None
     d = nat.LinearDesc(x.numel() // ins, xs, ws, rs, ins, outs, _DTYPES[x.dtype], activation)
-    work, size = _workspace(L.fwn_linear_act_workspace_size, d, x.device)
+    work, size = _workspace(L.fwn_linear_act_workspace_size, d, x.device, xr, wr)
     nat.check(L.fwn_linear_act_launch(d, _addr(xr), _addr(wr), _addr(bias), _addr(rr), _addr(out), _addr(pre),
                                       _addr(work), size, _stream(x)))
   return out, pre
@@ -120,7 +120,7 @@ class _LinearAct(torch.autograd.Function):
     with torch.cuda.device(g.device):
       gx, gw, gb = (torch.empty(shape, dtype=g.dtype, device=g.device) if need else None
                     for shape, need in zip((x_shape, w_shape, (outs,)), needs))
-      work, size = _workspace(L.fwn_linear_act_bwd_workspace_size, d, g.device)
+      work, size = _workspace(L.fwn_linear_act_bwd_workspace_size, d, g.device, xr, wr, g, gx, gw, gb)
       nat.check(L.fwn_linear_act_bwd_launch(d, _addr(xr), _addr(wr), _addr(pre), _addr(g), _addr(gx), _addr(gw), _addr(gb),
                                             _addr(work), size, _stream(g)))
     return gx, gw, gb, g_res, None
@@ -180,7 +180,7 @@ def linear_act_q8(x, x_scale, weight, weight_scale, bias=None, *, activation=Non
   with torch.cuda.device(x.device):
     out = torch.empty((*lead, outs), dtype=dtype, device=x.device)
     d = nat.LinearDesc(x.numel() // ins, xs, ws, rs, ins, outs, _DTYPES[dtype], act)
-    work, size = _workspace(L.fwn_linear_act_q8_workspace_size, d, x.device)
+    work, size = _workspace(L.fwn_linear_act_q8_workspace_size, d, x.device, xr, wr)
     nat.check(L.fwn_linear_act_q8_launch(d, _addr(xr), _addr(x_scale), _addr(wr), _addr(weight_scale), _addr(bias),
                                          _addr(rr), _addr(out), _addr(work), size, _stream(x)))
   return out

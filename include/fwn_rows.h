@@ -182,8 +182,9 @@ typedef struct fwn_linear_desc {
   int32_t activation;
 } fwn_linear_desc;
 
-/* Workspaces hold nothing between launches; 256-byte aligned. Launches that can overlap need their own. */
-int fwn_linear_act_workspace_size(const fwn_linear_desc* d, uint64_t* bytes);
+/* Workspaces hold nothing between launches and are 256-byte aligned; launches that can overlap need their
+ * own. Their sizes are asked with the pointers of the launch, of which only NULL and the alignment matter. */
+int fwn_linear_act_workspace_size(const fwn_linear_desc* d, const void* x, const void* weight, uint64_t* bytes);
 int fwn_linear_act_launch(const fwn_linear_desc* d, const void* x, const void* weight, const void* bias,
                           const void* residual, void* out, void* pre, void* workspace, uint64_t workspace_bytes,
                           void* stream);
@@ -192,7 +193,8 @@ int fwn_linear_act_launch(const fwn_linear_desc* d, const void* x, const void* w
  * activation is FWN_ACT_NONE; dz is rounded to the dtype for the products),
  *   gx = dz weight [rows, ins],  gw = dz^T x [outs, ins],  gb = column sums of dz [outs]
  * each contiguous and skipped where NULL. The residual's gradient is g. Sums run in a fixed order. */
-int fwn_linear_act_bwd_workspace_size(const fwn_linear_desc* d, uint64_t* bytes);
+int fwn_linear_act_bwd_workspace_size(const fwn_linear_desc* d, const void* x, const void* weight, const void* g,
+                                      const void* gx, const void* gw, const void* gb, uint64_t* bytes);
 int fwn_linear_act_bwd_launch(const fwn_linear_desc* d, const void* x, const void* weight, const void* pre,
                               const void* g, void* gx, void* gw, void* gb, void* workspace, uint64_t workspace_bytes,
                               void* stream);
@@ -200,7 +202,7 @@ int fwn_linear_act_bwd_launch(const fwn_linear_desc* d, const void* x, const voi
 /* The forward of 8-bit operands: x and weight hold OCP e4m3 codes, z = (x weight^T) x_scale[row]
  * w_scale[column] + bias with float32 scales (fwn_rms_norm_q8_launch, fwn_quantize_rows_launch). The
  * descriptor's dtype is that of bias, residual and out. */
-int fwn_linear_act_q8_workspace_size(const fwn_linear_desc* d, uint64_t* bytes);
+int fwn_linear_act_q8_workspace_size(const fwn_linear_desc* d, const uint8_t* x, const uint8_t* weight, uint64_t* bytes);
 int fwn_linear_act_q8_launch(const fwn_linear_desc* d, const uint8_t* x, const float* x_scale, const uint8_t* weight,
                              const float* w_scale, const void* bias, const void* residual, void* out,
                              void* workspace, uint64_t workspace_bytes, void* stream);

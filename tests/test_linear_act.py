@@ -449,14 +449,15 @@ def _desc(rows=4, ins=64, outs=32, x_stride=64, w_stride=64, r_stride=32, dtype=
 
 
 @pytest.mark.parametrize("bad,code", [(dict(rows=-1), 1), (dict(rows=1 << 40), 1), (dict(ins=0), 1), (dict(outs=0), 1),
-                                      (dict(ins=(1 << 20) + 1), 1), (dict(x_stride=-1), 1), (dict(w_stride=1 << 40), 1),
+                                      (dict(ins=(1 << 20) + 1), 1), (dict(ins=1 << 20, outs=1 << 20), 1), (dict(rows=1 << 31, outs=4096), 1), (dict(x_stride=-1), 1), (dict(w_stride=1 << 40), 1),
                                       (dict(r_stride=-5), 1), (dict(dtype=2), 2), (dict(activation=5), 2),
                                       (dict(activation=-1), 2)])
 def test_bad_descriptors(bad, code):
   L, d = nat.lib(), _desc(**bad)
   size = ctypes.c_uint64()
-  for query in (L.fwn_linear_act_workspace_size, L.fwn_linear_act_bwd_workspace_size, L.fwn_linear_act_q8_workspace_size):
-    assert query(d, ctypes.byref(size)) == code
+  for query in (L.fwn_linear_act_workspace_size, L.fwn_linear_act_q8_workspace_size):
+    assert query(d, F, 2 * F, ctypes.byref(size)) == code
+  assert L.fwn_linear_act_bwd_workspace_size(d, F, 2 * F, 3 * F, 4 * F, 5 * F, 6 * F, ctypes.byref(size)) == code
   assert L.fwn_linear_act_launch(d, F, 2 * F, None, None, 3 * F, None, None, 0, None) == code
   assert L.fwn_linear_act_q8_launch(d, F, 2 * F, 3 * F, 4 * F, None, None, 5 * F, None, 0, None) == code
   assert L.fwn_linear_act_bwd_launch(d, F, 2 * F, None, 3 * F, 4 * F, 5 * F, 6 * F, None, 0, None) == code
@@ -466,8 +467,19 @@ def test_bad_pointers():
   L, d = nat.lib(), _desc()
   fwd, q8, bwd = L.fwn_linear_act_launch, L.fwn_linear_act_q8_launch, L.fwn_linear_act_bwd_launch
   act = _desc(activation=2)
-  for query in (L.fwn_linear_act_workspace_size, L.fwn_linear_act_bwd_workspace_size, L.fwn_linear_act_q8_workspace_size):
-    assert query(d, None) == nat.ERR_INVALID_ARG
+  for query in (L.fwn_linear_act_workspace_size, L.fwn_linear_act_q8_workspace_size):
+    assert query(d, F, 2 * F, None) == nat.ERR_INVALID_ARG
+  assert L.fwn_linear_act_bwd_workspace_size(d, F, 2 * F, 3 * F, 4 * F, 5 * F, 6 * F, None) == nat.ERR_INVALID_ARG
+  size = ctypes.c_uint64()
+  odd = _desc(ins=100, x_stride=100)  # x is laid out: no workspace is an error
+  assert L.fwn_linear_act_workspace_size(odd, F, 2 * F, ctypes.byref(size)) == nat.OK and size.value >= 4 * 208
+  assert fwd(odd, F, 2 * F, None, None, 3 * F, None, None, 0, None) == nat.ERR_INVALID_ARG
+  assert fwd(odd, F, 2 * F, None, None, 3 * F, None, 4 * F, size.value - 1, None) == nat.ERR_INVALID_ARG
+  assert fwd(odd, F, 2 * F, None, None, 3 * F, None, 4 * F + 16, size.value, None) == nat.ERR_INVALID_ARG
+  # Aligned whole rows are read where they lie: nothing is kept for them; misaligned ones are laid out.
+  wide = _desc(rows=4096, ins=4096, outs=4096, x_stride=4096, w_stride=4096)
+  assert L.fwn_linear_act_workspace_size(wide, F, 2 * F, ctypes.byref(size)) == nat.OK and size.value == 0
+  assert L.fwn_linear_act_workspace_size(wide, F + 2, 2 * F, ctypes.byref(size)) == nat.OK and size.value == 4096 * 8192
   for rc in (fwd(None, F, 2 * F, None, None, 3 * F, None, None, 0, None), fwd(d, None, 2 * F, None, None, 3 * F, None, None, 0, None),
              fwd(d, F, None, None, None, 3 * F, None, None, 0, None), fwd(d, F, 2 * F, None, None, None, None, None, 0, None),
              fwd(d, F, 2 * F, None, None, F + 256, None, None, 0, None), fwd(d, F, 2 * F, None, None, 3 * F, 3 * F, None, 0, None),
