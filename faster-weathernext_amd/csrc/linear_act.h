@@ -48,8 +48,8 @@ struct ProductArgs {
 };
 
 constexpr int64_t kMaxStride = 1 << 22;
-constexpr int kStageBytes = 64;  // of an operand row in one pipeline stage
-constexpr int kStageRows = 32;   // of an operand whose rows are k
+constexpr int kStageBytes = 128;  // of an operand row in one pipeline stage
+constexpr int kStageRows = 64;   // of an operand whose rows are k
 
 enum class Operands { kInnerInner, kInnerOuter, kOuterOuter };  // how a and b lie
 

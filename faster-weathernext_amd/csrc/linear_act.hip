@@ -181,20 +181,23 @@ __device__ __forceinline__ void mend(const ProductArgs& g, int64_t row, int64_t 
 }
 
 // ------------------------------------------------------------------------------------------
-// Copies of an operand's stages into LDS, 1 KB a wave instruction, two a wave and stage.
-//   inner: 16 rows of 64 bytes; 16-byte chunk c of row r lies at c ^ 2 (r / 4 % 2), so that the eight rows
-//          and two chunks that a ds_read_b128 serves at once lie in sixteen different banks' groups;
+// Copies of an operand's stages into LDS, 1 KB a wave instruction, four a wave and stage.
+//   inner: 8 rows of 128 bytes; 16-byte chunk c of row r lies at c ^ (r / 2 % 8), so that a chunk of sixteen
+//          rows, which a ds_read_b128 serves at once, lies in sixteen different parts of a 256-byte line (4 clocks
+//          a read measured, 256 bytes a clock). Whole 128-byte lines: with 64-byte rows each line was fetched
+//          twice, the L1 holding less than a stage, and the product ran at two thirds of its rate;
 //   outer: 4 rows of k by 128 columns, in the swizzled layout of the transpose reads.
 // Rows and columns past the operand, k past the sum and stages past the range are copied as zeros: their
 // offsets lie past the buffer's end.
 constexpr uint32_t kNowhere = 0x80000000u, kBuffer = 0x7fffffffu;
+constexpr int kCopies = 4;
 
 template <bool OUTER, int WAVES>
 struct Copy {
   const char* base;  // of the tile
   int64_t step;      // bytes from one stage to the next
   int64_t plane;
-  uint32_t off[2], tail[2];  // of this lane's 16 bytes, and kNowhere where they lie past the sum in its last stage
+  uint32_t off[kCopies], tail[kCopies];  // of this lane's 16 bytes, and kNowhere where they lie past the sum in its last stage
 
   // Tile from row (or column) `first` of `rows`; `k` elements of `size` bytes in the sum, whose last stage is `last`.
   __device__ __forceinline__ void init(const char* p, int64_t stride, int64_t plane_bytes, int64_t first, int64_t rows,
@@ -203,14 +206,14 @@ struct Copy {
     base = p + (OUTER ? first * 2 : first * stride);
     step = OUTER ? kStageRows * stride : kStageBytes;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    for (int h = 0; h < kCopies; ++h) {
       const int q = w + WAVES * h;
       if constexpr (OUTER) {
-        const int row = 4 * (q & 7) + lane / 16, chunk = (lane % 16) ^ swz<16>(row), col = (q >> 3) * 128 + chunk * 8;
+        const int row = 4 * (q & 15) + lane / 16, chunk = (lane % 16) ^ swz<16>(row), col = (q >> 4) * 128 + chunk * 8;
         off[h] = first + col < rows ? (uint32_t)row * (uint32_t)stride + (uint32_t)col * 2 : kNowhere;
         tail[h] = last * kStageRows + row < k ? 0 : kNowhere;
       } else {
-        const int row = 16 * q + lane / 4, chunk = (lane % 4) ^ (((lane >> 4) & 1) << 1);
+        const int row = 8 * q + lane / 8, chunk = (lane % 8) ^ (row / 2 % 8);
         off[h] = first + row < rows ? (uint32_t)row * (uint32_t)stride + (uint32_t)chunk * 16 : kNowhere;
         tail[h] = last * kStageBytes + chunk * 16 < k * size ? 0 : kNowhere;
       }
@@ -221,7 +224,7 @@ struct Copy {
   __device__ __forceinline__ void issue(lds_char* dst, int64_t t, int p, uint32_t last, uint32_t none, int w) const {
     const rsrc_t r = make_rsrc(base + p * plane + t * step, kBuffer);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    for (int h = 0; h < kCopies; ++h) {
       const uint32_t o = off[h] | (tail[h] & last) | none;
       __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(dst + (w + WAVES * h) * 1024),
                                                16, (int)o, 0, 0, 0);
@@ -229,49 +232,50 @@ struct Copy {
   }
 };
 
-// LDS byte offsets of an operand's 32-row blocks for one wave: element [block][half of the 32 k].
+// LDS byte offsets of an operand's 32-row blocks for one wave: quarter c of a stage is 16 bf16 k.
 template <bool OUTER, int BLOCKS>
 struct Reads {
-  uint32_t at[BLOCKS][2];
+  uint32_t at[OUTER ? 2 * BLOCKS : 4];
 
   __device__ __forceinline__ void init(uint32_t region, int first, int lane) {  // first: row or column of the tile
     const int i = lane & 31, g = lane >> 5;
+    if constexpr (OUTER) {  // k 8 g + 4 h .. of a quarter
+      const int G = lane >> 4, t = lane & 15, e = t >> 2, q = t & 3;
 #pragma unroll
-    for (int m = 0; m < BLOCKS; ++m) {
-      if constexpr (OUTER) {  // [h]: k 8 g + 4 h .. of a 16-k half; the other half 16 rows on
-        const int G = lane >> 4, t = lane & 15, e = t >> 2, q = t & 3, c0 = first + 32 * m;
+      for (int m = 0; m < BLOCKS; ++m) {
+        const int c0 = first + 32 * m;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int r = 8 * g + 4 * h + e, chunk = 4 * ((c0 & 127) >> 5) + 2 * (G & 1) + (q >> 1);
-          at[m][h] = region + (uint32_t)(c0 >> 7) * 8192 + r * 256 + ((chunk ^ swz<16>(r)) << 4) + (q & 1) * 8;
+          at[2 * m + h] = region + (uint32_t)(c0 >> 7) * 16384 + r * 256 + ((chunk ^ swz<16>(r)) << 4) + (q & 1) * 8;
         }
-      } else {
-        const int r = first + 32 * m + i;
-#pragma unroll
-        for (int c = 0; c < 2; ++c) at[m][c] = region + r * 64 + (((2 * c + g) ^ (((r >> 2) & 1) << 1)) << 4);
       }
+    } else {
+      const int r = first + i;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) at[c] = region + r * 128 + (((2 * c + g) ^ (r / 2 % 8)) << 4);
     }
   }
 
   __device__ __forceinline__ u32x4 read(const lds_char* stage, int m, int c) const {
     if constexpr (OUTER) {
-      const u32x2 lo = tr_read(stage + c * 4096, at[m][0]), hi = tr_read(stage + c * 4096, at[m][1]);
+      const u32x2 lo = tr_read(stage + c * 4096, at[2 * m]), hi = tr_read(stage + c * 4096, at[2 * m + 1]);
       return u32x4{lo[0], lo[1], hi[0], hi[1]};
     } else {
-      return row_read(stage, at[m][c]);
+      return row_read(stage + m * 4096, at[c]);
     }
   }
 };
 
-// All but the newest `vm` of this wave's copies have landed and its LDS reads have returned.
-template <int vm>
+// This wave's copies have landed and its LDS reads have returned, and so have every other wave's.
 __device__ __forceinline__ void stage_barrier() {
-  __builtin_amdgcn_s_waitcnt(0x0070 | vm);
+  __builtin_amdgcn_s_waitcnt(0x0070);
   asm volatile("" ::: "memory");
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 }
 
+constexpr int kBand = 8;
 constexpr int kStrip = 72;  // floats from one row of a strip to the next: its halves' rows fall in other banks
 
 enum class Form { kBf16, kParts, kE4m3 };
@@ -282,18 +286,20 @@ __global__ void __launch_bounds__(2 * BM, 2) product_kernel(ProductArgs g) {
   constexpr int WAVES = BM / 32, NI = 2, WN = BN / 64, WM = WAVES / WN, MI = BM / WM / 32;
   constexpr int STAGE = (BM + BN) * kStageBytes;
   constexpr bool E4M3 = FORM == Form::kE4m3, PARTS = FORM == Form::kParts;
-  static_assert(WAVES * 2 * 1024 == BM * 64 && BM == BN, "two copies a wave and operand");
+  static_assert(WAVES * kCopies * 1024 == BM * kStageBytes && BM == BN, "copies a wave and operand");
   // One array a stage: the compiler waits for the copies into the array that a read names, and for those alone.
-  __shared__ __align__(16) char lds0[STAGE], lds1[STAGE], lds2[STAGE], lds3[STAGE];
-  lds_char *const s0 = (lds_char*)lds0, *const s1 = (lds_char*)lds1, *const s2 = (lds_char*)lds2,
-           *const s3 = (lds_char*)lds3;
+  __shared__ __align__(256) char lds0[STAGE], lds1[STAGE];
+  lds_char *const s0 = (lds_char*)lds0, *const s1 = (lds_char*)lds1;
   const int lane = (int)threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   // Workgroups go to the 8 XCDs in turn: each takes a contiguous range of (range of the sum, tile).
   const int total = (int)gridDim.x, xcd = (int)blockIdx.x & 7, per = total >> 3, rem = total & 7;
   const int id = xcd * per + (xcd < rem ? xcd : rem) + ((int)blockIdx.x >> 3);
   const int tn = (int)((g.e.n + BN - 1) / BN), tiles = (int)((g.e.m + BM - 1) / BM) * tn;
   const int split = id / tiles, tile = id - split * tiles;
-  const int64_t i0 = (int64_t)(tile / tn) * BM, j0 = (int64_t)(tile % tn) * BN;
+  // Bands of kBand rows of tiles, column by column: what runs at once on an XCD shares rows of both operands.
+  const int tm = tiles / tn, band = tile / (kBand * tn), in = tile - band * (kBand * tn);
+  const int high = tm - band * kBand < kBand ? tm - band * kBand : kBand;
+  const int64_t i0 = (int64_t)(band * kBand + in % high) * BM, j0 = (int64_t)(in / high) * BN;
   const int size = E4M3 ? 1 : 2, per_stage = kStageBytes / size;
   const int64_t stages = (g.k + per_stage - 1) / per_stage, t0 = (int64_t)split * g.chunk;
   const int64_t t1 = t0 + g.chunk < stages ? t0 + g.chunk : stages;
@@ -328,21 +334,22 @@ __global__ void __launch_bounds__(2 * BM, 2) product_kernel(ProductArgs g) {
   for (int m = 0; m < MI; ++m)
 #pragma unroll
     for (int n = 0; n < NI; ++n) acc[m][n] = zero16();
-  const auto read = [&](const lds_char* stage, int c, u32x4(&fa)[MI], u32x4(&fb)[NI]) {
+  constexpr int SETS = E4M3 ? 4 : 2;  // operands in registers: those multiplied and those being read
+  u32x4 fa[SETS][MI], fb[SETS][NI];
+  const auto read = [&](const lds_char* stage, int c, int set) {
 #pragma unroll
-    for (int m = 0; m < MI; ++m) fa[m] = ra.read(stage, m, c);
+    for (int m = 0; m < MI; ++m) fa[set][m] = ra.read(stage, m, c);
 #pragma unroll
-    for (int n = 0; n < NI; ++n) fb[n] = rb.read(stage, n, c);
+    for (int n = 0; n < NI; ++n) fb[set][n] = rb.read(stage, n, c);
   };
-  u32x4 a0[MI], b0[NI], a1[MI], b1[NI];
-  const auto multiply = [&](const u32x4(&fa)[MI], const u32x4(&fb)[NI]) {
+  const auto multiply = [&](int set) {
 #pragma unroll
     for (int m = 0; m < MI; ++m)
 #pragma unroll
-      for (int n = 0; n < NI; ++n) acc[m][n] = mfma_bf16(fa[m], fb[n], acc[m][n]);
+      for (int n = 0; n < NI; ++n) acc[m][n] = mfma_bf16(fa[set][m], fb[set][n], acc[m][n]);
   };
-  // The same for a whole stage of e4m3: 64 k, both halves of the rows' bytes, scales 2^0.
-  const auto multiply8 = [&](const u32x4(&la)[MI], const u32x4(&ha)[MI], const u32x4(&lb)[NI], const u32x4(&hb)[NI]) {
+  // The same for half a stage of e4m3: 64 k, the bytes of two quarters, scales 2^0.
+  const auto multiply8 = [&](int set) {
     const auto join = [](const u32x4& x, const u32x4& y) {
       return i32x8{(int)x[0], (int)x[1], (int)x[2], (int)x[3], (int)y[0], (int)y[1], (int)y[2], (int)y[3]};
     };
@@ -350,8 +357,9 @@ __global__ void __launch_bounds__(2 * BM, 2) product_kernel(ProductArgs g) {
     for (int m = 0; m < MI; ++m)
 #pragma unroll
       for (int n = 0; n < NI; ++n)
-        acc[m][n] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(join(la[m], ha[m]), join(lb[n], hb[n]), acc[m][n], 0, 0,
-                                                                    0, 0x7f7f7f7f, 0, 0x7f7f7f7f);
+        acc[m][n] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(join(fa[set][m], fa[set + 1][m]),
+                                                                    join(fb[set][n], fb[set + 1][n]), acc[m][n], 0, 0, 0,
+                                                                    0x7f7f7f7f, 0, 0x7f7f7f7f);
   };
   // Column sums of a, in the workgroups of the first column tile: wave w takes 32 columns.
   const bool sums = OA && g.sums != nullptr && j0 == 0 && w < BM / 32;
@@ -360,7 +368,7 @@ __global__ void __launch_bounds__(2 * BM, 2) product_kernel(ProductArgs g) {
   rs.init(0, 32 * (w < BM / 32 ? w : 0), lane);
   const auto add = [&](const lds_char* stage) {
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
+    for (int c = 0; c < 4; ++c) {
       const u32x4 v = rs.read(stage, 0, c);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
@@ -371,35 +379,44 @@ __global__ void __launch_bounds__(2 * BM, 2) product_kernel(ProductArgs g) {
   };
 
   copy(s0);
+  stage_barrier();
   copy(s1);
-  copy(s2);
-  stage_barrier<8>();  // s0
-  read(s0, 0, a0, b0);
-  const auto step = [&](lds_char* now, lds_char* next, lds_char* last) {
-    // The next stage has landed for every wave, and every wave has read all of the last one, whose place
-    // the stage after the two in flight takes.
-    stage_barrier<4>();
-    copy(last);
-    read(now, 1, a1, b1);
+  read(s0, 0, 0);
+  if constexpr (E4M3) read(s0, 1, 1);
+  const auto step = [&](lds_char* now, lds_char* next) {
     if constexpr (E4M3) {
-      multiply8(a0, a1, b0, b1);
-      read(next, 0, a0, b0);
+      read(now, 2, 2);
+      read(now, 3, 3);
+      multiply8(0);
     } else {
+      read(now, 1, 1);
       __builtin_amdgcn_sched_barrier(0);
-      multiply(a0, b0);
+      multiply(0);
       if constexpr (OA) {
         if (sums) add(now);
       }
-      read(next, 0, a0, b0);
+      read(now, 2, 0);
       __builtin_amdgcn_sched_barrier(0);
-      multiply(a1, b1);
+      multiply(1);
+      read(now, 3, 1);
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(0);
+    }
+    // Every wave has read all of this stage, whose place the stage after the next takes, and the next has landed.
+    stage_barrier();
+    copy(now);
+    read(next, 0, 0);
+    if constexpr (E4M3) {
+      read(next, 1, 1);
+      multiply8(2);
+    } else {
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(1);
     }
   };
-  for (int t = 0; t < steps; t += 4) {  // stages past the last are zeros
-    step(s0, s1, s3);
-    step(s1, s2, s0);
-    step(s2, s3, s1);
-    step(s3, s0, s2);
+  for (int t = 0; t < steps; t += 2) {  // a stage past the last is zeros
+    step(s0, s1);
+    step(s1, s0);
   }
   wait_vmem();  // no copy outlives the stages
   __syncthreads();
@@ -411,9 +428,8 @@ __global__ void __launch_bounds__(2 * BM, 2) product_kernel(ProductArgs g) {
     }
   }
   // Through LDS, 32 rows of the wave's part at a time, to rows of eight columns a lane.
-  constexpr int PER = WAVES / 4;  // waves that share a stage's array
-  lds_char* const own = w / PER == 0 ? s0 : w / PER == 1 ? s1 : w / PER == 2 ? s2 : s3;
-  auto* const strip = (__attribute__((address_space(3))) float*)(own + (w % PER) * (32 * kStrip * 4));
+  constexpr int PER = WAVES / 2;  // waves that share a stage's array
+  auto* const strip = (__attribute__((address_space(3))) float*)((w < PER ? s0 : s1) + (w % PER) * (32 * kStrip * 4));
   const int j = lane & 31, half = lane >> 5;
   const int64_t col = j0 + wn + 8 * (lane & 7);
   Columns c;

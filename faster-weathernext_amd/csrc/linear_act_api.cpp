@@ -134,11 +134,11 @@ Plan plan(int64_t m, int64_t n, int64_t k, int32_t op) {
   double least = 0;
   for (int t = 0; t < kTileShapes; ++t) {
     const int64_t tiles = parts(m, kTiles[t].m) * parts(n, kTiles[t].n);
-    const double per_stage = (t == 0 ? 0.5 : 0.15) * (op == kOpF32 ? 6 : 1), ends = t == 0 ? 6.0 : 3.0;  // us
+    const double per_stage = (t == 0 ? 1.0 : 0.3) * (op == kOpF32 ? 6 : 1), ends = t == 0 ? 6.0 : 3.0;  // us
     for (int64_t want = 1; want <= 64; want *= 2) {
       const int64_t chunk = parts(stages, want), splits = parts(stages, chunk);
       if (splits != want && want > 1) continue;
-      if (want > 1 && chunk < 4) break;
+      if (want > 1 && chunk < 2) break;
       const double join = splits > 1 ? 4.0 + (double)(splits + 1) * m * n * 4 / 4e6 : 0;
       const double time = (double)parts(tiles * splits, kCus) * (per_stage * chunk + ends) + join;
       if ((t == 0 && want == 1) || time < least) {
