@@ -22,7 +22,7 @@ struct EpilogueArgs {
   int64_t r_row;
   int64_t m, n;
   int32_t dtype, activation;
-  bool vec;  // n and r_row are multiples of 8 and every tensor is 16-byte aligned
+  bool vec;  // n and r_row are multiples of 8 (r_row at most FWN_LINEAR_ACT_MAX), every tensor is 16-byte aligned
 };
 
 // c[i, j] = sum over k of a(i, k) b(j, k). Each operand is either rows of contiguous k (`inner`) or k rows of

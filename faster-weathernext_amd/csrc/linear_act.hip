@@ -70,32 +70,66 @@ __device__ __forceinline__ void store8(void* p, int64_t i, int dtype, const floa
   }
 }
 
-__device__ __forceinline__ float activate(float z, int kind) {
-  constexpr float c = 0.7978845608028654f;
-  switch (kind) {
-    case FWN_ACT_RELU: return z > 0.f || z != z ? z : 0.f;
-    case FWN_ACT_GELU: return 0.5f * z * (1.f + erff(z * 0.7071067811865476f));
-    case FWN_ACT_GELU_TANH: return 0.5f * z * (1.f + tanhf(c * (z + 0.044715f * z * z * z)));
-    case FWN_ACT_SILU: return z / (1.f + expf(-z));
-    default: return z;
-  }
+// e^x and 1 / x on the transcendental unit, within two units in the last place.
+__device__ __forceinline__ float fast_exp(float x) { return fast_exp2(x * LOG2E); }
+__device__ __forceinline__ float fast_rcp(float x) { return __builtin_amdgcn_rcpf(x); }
+
+// erf by Abramowitz and Stegun's 7.1.26, off by at most 1.5e-7 (a value times z / 2 here).
+__device__ __forceinline__ float erf_of(float x) {
+  const float y = __builtin_fabsf(x), t = fast_rcp(fmaf(0.3275911f, y, 1.f));
+  float p = fmaf(1.061405429f, t, -1.453152027f);
+  p = fmaf(p, t, 1.421413741f);
+  p = fmaf(p, t, -0.284496736f);
+  p = fmaf(p, t, 0.254829592f);
+  return __builtin_copysignf(1.f - p * t * fast_exp(-y * y), x);
 }
 
-__device__ __forceinline__ float slope(float z, int kind) {
-  constexpr float c = 0.7978845608028654f;
+constexpr float kTanh = 0.7978845608028654f, kCube = 0.044715f;  // gelu_tanh: u = kTanh (z + kCube z^3)
+
+// act(z). The tanh form is z / (1 + e^(-2u)).
+template <int KIND>
+__device__ __forceinline__ float activate(float z) {
+  if constexpr (KIND == FWN_ACT_RELU) return z > 0.f || z != z ? z : 0.f;
+  if constexpr (KIND == FWN_ACT_GELU) return 0.5f * z * (1.f + erf_of(z * 0.7071067811865476f));
+  if constexpr (KIND == FWN_ACT_GELU_TANH)
+    return z * fast_rcp(1.f + fast_exp2(z * fmaf(z * z, -2.f * kTanh * kCube * LOG2E, -2.f * kTanh * LOG2E)));
+  if constexpr (KIND == FWN_ACT_SILU) return z * fast_rcp(1.f + fast_exp(-z));
+  return z;
+}
+
+// act'(z).
+template <int KIND>
+__device__ __forceinline__ float slope(float z) {
+  if constexpr (KIND == FWN_ACT_RELU) return z > 0.f ? 1.f : 0.f;
+  if constexpr (KIND == FWN_ACT_GELU)
+    return 0.5f * (1.f + erf_of(z * 0.7071067811865476f)) + z * fast_exp(-0.5f * z * z) * 0.3989422804014327f;
+  if constexpr (KIND == FWN_ACT_GELU_TANH) {
+    // p = 1 / (1 + e^(-2u)), p + 2 z p (1 - p) u'; beyond 12 it is 0 or 1, and a large z^2 would meet that 0.
+    const float y = z > 12.f ? 12.f : z < -12.f ? -12.f : z, q = y * y;
+    const float p = fast_rcp(1.f + fast_exp2(y * fmaf(q, -2.f * kTanh * kCube * LOG2E, -2.f * kTanh * LOG2E)));
+    return fmaf(2.f * y * p * (1.f - p), fmaf(q, 3.f * kTanh * kCube, kTanh), p);
+  }
+  if constexpr (KIND == FWN_ACT_SILU) {
+    const float p = fast_rcp(1.f + fast_exp(-z)), y = p > 0.f ? z : 0.f;
+    return p * fmaf(y, 1.f - p, 1.f);
+  }
+  return 1.f;
+}
+
+// Calls f with the activation as a compile-time constant.
+template <int KIND>
+struct Act {
+  static constexpr int kind = KIND;
+};
+template <bool PLAIN, typename F>
+__device__ __forceinline__ void with_activation(int kind, F&& f) {
+  if constexpr (PLAIN) return f(Act<FWN_ACT_NONE>());
   switch (kind) {
-    case FWN_ACT_RELU: return z > 0.f ? 1.f : 0.f;
-    case FWN_ACT_GELU:
-      return 0.5f * (1.f + erff(z * 0.7071067811865476f)) + z * expf(-0.5f * z * z) * 0.3989422804014327f;
-    case FWN_ACT_GELU_TANH: {
-      const float t = tanhf(c * (z + 0.044715f * z * z * z));
-      return 0.5f * (1.f + t) + 0.5f * z * (1.f - t * t) * c * (1.f + 3.f * 0.044715f * z * z);
-    }
-    case FWN_ACT_SILU: {
-      const float s = 1.f / (1.f + expf(-z));
-      return s * (1.f + z * (1.f - s));
-    }
-    default: return 1.f;
+    case FWN_ACT_RELU: return f(Act<FWN_ACT_RELU>());
+    case FWN_ACT_GELU: return f(Act<FWN_ACT_GELU>());
+    case FWN_ACT_GELU_TANH: return f(Act<FWN_ACT_GELU_TANH>());
+    case FWN_ACT_SILU: return f(Act<FWN_ACT_SILU>());
+    default: return f(Act<FWN_ACT_NONE>());
   }
 }
 
@@ -114,6 +148,7 @@ struct Columns {
 };
 
 // The epilogue of z[row, col .. col + 7], row < m; columns from n on are dropped.
+template <int KIND>
 __device__ __forceinline__ void finish(const EpilogueArgs& e, int64_t row, int64_t col, float (&v)[8], const Columns& c) {
   if (e.a_scale) {
     const float s = e.a_scale[row];
@@ -127,7 +162,7 @@ __device__ __forceinline__ void finish(const EpilogueArgs& e, int64_t row, int64
     if (col >= e.n) return;
     if (e.pre) store8(e.pre, at, e.dtype, v);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = activate(v[k], e.activation);
+    for (int k = 0; k < 8; ++k) v[k] = activate<KIND>(v[k]);
     if (e.residual) {
       float r[8];
       load8(e.residual, row * e.r_row + col, e.dtype, r);
@@ -140,7 +175,7 @@ __device__ __forceinline__ void finish(const EpilogueArgs& e, int64_t row, int64
     for (int k = 0; k < 8; ++k) {
       if (col + k >= e.n) break;
       if (e.pre) store_one(e.pre, at + k, e.dtype, v[k]);
-      float o = activate(v[k], e.activation);
+      float o = activate<KIND>(v[k]);
       if (e.residual) o += load_one(e.residual, row * e.r_row + col + k, e.dtype);
       store_one(e.out, at + k, e.dtype, o);
     }
@@ -286,6 +321,7 @@ __global__ void __launch_bounds__(2 * BM, 2) product_kernel(ProductArgs g) {
   constexpr int WAVES = BM / 32, NI = 2, WN = BN / 64, WM = WAVES / WN, MI = BM / WM / 32;
   constexpr int STAGE = (BM + BN) * kStageBytes;
   constexpr bool E4M3 = FORM == Form::kE4m3, PARTS = FORM == Form::kParts;
+  constexpr bool PLAIN = OB;  // a gradient: no epilogue but the rounding
   static_assert(WAVES * kCopies * 1024 == BM * kStageBytes && BM == BN, "copies a wave and operand");
   // One array a stage: the compiler waits for the copies into the array that a read names, and for those alone.
   __shared__ __align__(256) char lds0[STAGE], lds1[STAGE];
@@ -431,33 +467,118 @@ __global__ void __launch_bounds__(2 * BM, 2) product_kernel(ProductArgs g) {
   constexpr int PER = WAVES / 2;  // waves that share a stage's array
   auto* const strip = (__attribute__((address_space(3))) float*)((w < PER ? s0 : s1) + (w % PER) * (32 * kStrip * 4));
   const int j = lane & 31, half = lane >> 5;
-  const int64_t col = j0 + wn + 8 * (lane & 7);
-  Columns c;
-  if (!g.part) c.load(g.e, col);
-#pragma unroll
-  for (int m = 0; m < MI; ++m) {
-    if (i0 + wm + 32 * m >= g.e.m) break;
+  const auto to_strip = [&](int m) {
 #pragma unroll
     for (int n = 0; n < NI; ++n)
 #pragma unroll
       for (int r = 0; r < 16; ++r) strip[(8 * (r >> 2) + 4 * half + (r & 3)) * kStrip + 32 * n + j] = acc[m][n][r];
-    __builtin_amdgcn_wave_barrier();
-#pragma unroll 1
-    for (int p = 0; p < 4; ++p) {
-      const int64_t row = i0 + wm + 32 * m + 8 * p + (lane >> 3);
-      float v[8];
+  };
+  const int sub = lane >> 3, at_col = wn + 8 * (lane & 7);  // this lane's row of eight and its columns of the tile
+  const int64_t col = j0 + at_col;
+  const auto from_strip = [&](int p, float(&v)[8]) {
+    const auto* q = (const __attribute__((address_space(3))) f32x4*)(strip + (8 * p + sub) * kStrip + 8 * (lane & 7));
+    const f32x4 lo = q[0], hi = q[1];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = strip[(8 * p + (lane >> 3)) * kStrip + 8 * (lane & 7) + k];
-      if (row >= g.e.m || col >= g.e.n) continue;
-      if (g.part) {
-        store8(g.part, ((int64_t)split * g.e.m + row) * g.part_row + col, FWN_F32, v);
-      } else {
-        if constexpr (PARTS) mend<OA, OB>(g, row, col, v);
-        finish(g.e, row, col, v, c);
-      }
+    for (int k = 0; k < 4; ++k) {
+      const float x = lo[k], y = hi[k];
+      v[k] = x;
+      v[4 + k] = y;
     }
-    __builtin_amdgcn_wave_barrier();
+  };
+  const EpilogueArgs& e = g.e;
+  const int rows = (int)(e.m - i0 < BM ? e.m - i0 : BM);  // of the tile
+  if (g.part || (e.vec && !PARTS)) {
+    // Offsets in the tile, past the buffers' ends for rows and columns outside.
+    const bool f32 = g.part || (E4M3 && e.dtype == FWN_F32);
+    const int64_t width = g.part ? g.part_row : e.n;
+    const uint32_t shift = f32 ? 2 : 1;
+    char* const to = g.part ? (char*)(g.part + (int64_t)split * e.m * g.part_row) : (char*)e.out;
+    const rsrc_t ro = make_rsrc(to + ((i0 * width + j0) << shift), kBuffer);
+    const rsrc_t rp = make_rsrc((char*)e.pre + ((i0 * width + j0) << shift), kBuffer);
+    const rsrc_t rr = make_rsrc((const char*)e.residual + ((i0 * e.r_row + j0) << shift), kBuffer);
+    const bool scaled = E4M3 && !g.part, pre = !PLAIN && !g.part && e.pre,
+               residual = !PLAIN && !g.part && e.residual;
+    const uint32_t nowhere = col < e.n ? 0 : kNowhere;
+    Columns c;
+    if (!PLAIN && !g.part) c.load(e, col);
+    const auto load = [&](rsrc_t r, uint32_t o, float(&f)[8]) {
+      const u32x4 lo = bload16(r, o), hi = f32 ? bload16(r, o + 16) : lo;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t x = lo[k], y = hi[k];
+        if (f32) {
+          f[k] = as_float(x);
+          f[4 + k] = as_float(y);
+        } else {
+          f[2 * k] = as_float(x << 16);
+          f[2 * k + 1] = as_float(x & 0xffff0000u);
+        }
+      }
+    };
+    const auto store = [&](rsrc_t r, uint32_t o, const float(&f)[8]) {
+      if (f32) {
+        __builtin_amdgcn_raw_buffer_store_b128(u32x4{as_bits(f[0]), as_bits(f[1]), as_bits(f[2]), as_bits(f[3])}, r, (int)o, 0, 0);
+        __builtin_amdgcn_raw_buffer_store_b128(u32x4{as_bits(f[4]), as_bits(f[5]), as_bits(f[6]), as_bits(f[7])}, r, (int)(o + 16), 0, 0);
+      } else {
+        __builtin_amdgcn_raw_buffer_store_b128(pack8(f), r, (int)o, 0, 0);
+      }
+    };
+    with_activation<PLAIN>(g.part ? FWN_ACT_NONE : e.activation, [&](auto act) {
+#pragma unroll
+      for (int m = 0; m < MI; ++m) {
+        to_strip(m);
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+          const int row = wm + 32 * m + 8 * p + sub;
+          const uint32_t out = (row < rows ? 0 : kNowhere) | nowhere;
+          const uint32_t o = out | (((uint32_t)row * (uint32_t)width + (uint32_t)at_col) << shift);
+          float v[8], r[8];
+          if (residual) load(rr, out | (((uint32_t)row * (uint32_t)e.r_row + (uint32_t)at_col) << shift), r);
+          from_strip(p, v);
+          if (scaled) {
+            const float s = row < rows ? e.a_scale[i0 + row] : 0.f;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] *= s * c.scale[k];
+          }
+          if (!PLAIN && !g.part) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] += c.bias[k];
+            if (pre) store(rp, o, v);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = activate<decltype(act)::kind>(v[k]);
+            if (residual) {
+#pragma unroll
+              for (int k = 0; k < 8; ++k) v[k] += r[k];
+            }
+          }
+          store(ro, o, v);
+        }
+        __builtin_amdgcn_wave_barrier();
+      }
+    });
+    return;
   }
+  // Outputs that are not whole aligned eights, and those of parts, which may need their wholes.
+  Columns c;
+  c.load(e, col);
+  with_activation<PLAIN>(e.activation, [&](auto act) {
+#pragma unroll
+    for (int m = 0; m < MI; ++m) {
+      to_strip(m);
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+      for (int p = 0; p < 4; ++p) {
+        const int row = wm + 32 * m + 8 * p + sub;
+        if (row >= rows || col >= e.n) continue;
+        float v[8];
+        from_strip(p, v);
+        if constexpr (PARTS) mend<OA, OB>(g, i0 + row, col, v);
+        finish<decltype(act)::kind>(e, i0 + row, col, v, c);
+      }
+      __builtin_amdgcn_wave_barrier();
+    }
+  });
 }
 
 // The partial products added in the order of the splits, then the epilogue: eight columns a thread.
@@ -477,7 +598,7 @@ __global__ void __launch_bounds__(256) join_kernel(ProductArgs g) {
   Columns c;
   c.load(g.e, col);
   if constexpr (FORM == Form::kParts) mend<OA, OB>(g, row, col, v);
-  finish(g.e, row, col, v, c);
+  with_activation<OB>(g.e.activation, [&](auto act) { finish<decltype(act)::kind>(g.e, row, col, v, c); });
 }
 
 template <bool OA, bool OB, Form FORM, int BM, int BN>
@@ -564,6 +685,7 @@ __global__ void __launch_bounds__(256) layout_kernel(LayoutArgs a) {
 }
 
 // 256 columns by `chunk` rows a workgroup, eight columns of every eighth row a thread.
+template <int KIND>
 __global__ void __launch_bounds__(256) slope_kernel(SlopeArgs a) {
   __shared__ float red[8][256];
   const int across = (a.outs + 255) / 256, block = (int)blockIdx.x / across;
@@ -578,18 +700,18 @@ __global__ void __launch_bounds__(256) slope_kernel(SlopeArgs a) {
       float dz[8], z[8];
       if (vec) {
         load8(a.g, at, a.dtype, dz);
-        if (a.activation) load8(a.pre, at, a.dtype, z);
+        if (KIND != FWN_ACT_NONE) load8(a.pre, at, a.dtype, z);
       } else {
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           const bool in = col + k < a.outs;
           dz[k] = in ? load_one(a.g, at + k, a.dtype) : 0.f;
-          z[k] = in && a.activation ? load_one(a.pre, at + k, a.dtype) : 0.f;
+          z[k] = in && KIND != FWN_ACT_NONE ? load_one(a.pre, at + k, a.dtype) : 0.f;
         }
       }
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        if (a.activation) dz[k] *= slope(z[k], a.activation);
+        if constexpr (KIND != FWN_ACT_NONE) dz[k] *= slope<KIND>(z[k]);
         sum[k] += dz[k];
       }
       if (a.dz) store_parts(a.dz + r * a.dz_stride + (int64_t)col * 2, a.dz_plane, a.dtype == FWN_F32, dz);
@@ -644,7 +766,14 @@ hipError_t launch_layout(const LayoutArgs& a, hipStream_t stream) {
 
 hipError_t launch_slope(const SlopeArgs& a, hipStream_t stream) {
   const unsigned across = (unsigned)(a.outs + 255) / 256;
-  hipLaunchKernelGGL(slope_kernel, dim3(across * (unsigned)a.blocks), dim3(256), 0, stream, a);
+  const dim3 grid(across * (unsigned)a.blocks), block(256);
+  switch (a.activation) {
+    case FWN_ACT_RELU: hipLaunchKernelGGL(slope_kernel<FWN_ACT_RELU>, grid, block, 0, stream, a); break;
+    case FWN_ACT_GELU: hipLaunchKernelGGL(slope_kernel<FWN_ACT_GELU>, grid, block, 0, stream, a); break;
+    case FWN_ACT_GELU_TANH: hipLaunchKernelGGL(slope_kernel<FWN_ACT_GELU_TANH>, grid, block, 0, stream, a); break;
+    case FWN_ACT_SILU: hipLaunchKernelGGL(slope_kernel<FWN_ACT_SILU>, grid, block, 0, stream, a); break;
+    default: hipLaunchKernelGGL(slope_kernel<FWN_ACT_NONE>, grid, block, 0, stream, a);
+  }
   return hipGetLastError();
 }
 

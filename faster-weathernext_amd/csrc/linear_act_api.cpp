@@ -174,7 +174,7 @@ struct Product {
     g.a = a.at, g.a_stride = a.row_bytes, g.a_plane = a.plane;
     g.b = b.at, g.b_stride = b.row_bytes, g.b_plane = b.plane;
     const EpilogueArgs& e = g.e;
-    g.e.vec = e.n % 8 == 0 && (!e.residual || e.r_row % 8 == 0) &&
+    g.e.vec = e.n % 8 == 0 && (!e.residual || (e.r_row % 8 == 0 && e.r_row <= FWN_LINEAR_ACT_MAX)) &&
               (((uintptr_t)e.out | (uintptr_t)e.pre | (uintptr_t)e.residual) & 15) == 0;
     return launch_product(how, op, p.tile, g, stream);
   }
