@@ -57,8 +57,8 @@ enum class Operands { kInnerInner, kInnerOuter, kOuterOuter };  // how a and b l
 struct TileShape {
   int m, n;
 };
-constexpr TileShape kTiles[] = {{256, 256}, {128, 128}};
-constexpr int kTileShapes = 2;
+constexpr TileShape kTiles[] = {{256, 256}, {192, 128}, {128, 128}};
+constexpr int kTileShapes = 3;
 
 // One product, by tiles of kTiles[tile]. `op` is what the operands hold: bf16, float32 as planes, or e4m3
 // (kInnerInner alone).

@@ -216,7 +216,7 @@ __device__ __forceinline__ void mend(const ProductArgs& g, int64_t row, int64_t 
 }
 
 // ------------------------------------------------------------------------------------------
-// Copies of an operand's stages into LDS, 1 KB a wave instruction, four a wave and stage.
+// Copies of an operand's stages into LDS, 1 KB a wave instruction, a few a wave and stage.
 //   inner: 8 rows of 128 bytes; 16-byte chunk c of row r lies at c ^ (r / 2 % 8), so that a chunk of sixteen
 //          rows, which a ds_read_b128 serves at once, lies in sixteen different parts of a 256-byte line (4 clocks
 //          a read measured, 256 bytes a clock). Whole 128-byte lines: with 64-byte rows each line was fetched
@@ -225,14 +225,12 @@ __device__ __forceinline__ void mend(const ProductArgs& g, int64_t row, int64_t 
 // Rows and columns past the operand, k past the sum and stages past the range are copied as zeros: their
 // offsets lie past the buffer's end.
 constexpr uint32_t kNowhere = 0x80000000u, kBuffer = 0x7fffffffu;
-constexpr int kCopies = 4;
-
-template <bool OUTER, int WAVES>
+template <bool OUTER, int WAVES, int COUNT>
 struct Copy {
   const char* base;  // of the tile
   int64_t step;      // bytes from one stage to the next
   int64_t plane;
-  uint32_t off[kCopies], tail[kCopies];  // of this lane's 16 bytes, and kNowhere where they lie past the sum in its last stage
+  uint32_t off[COUNT], tail[COUNT];  // of this lane's 16 bytes, and kNowhere where they lie past the sum in its last stage
 
   // Tile from row (or column) `first` of `rows`; `k` elements of `size` bytes in the sum, whose last stage is `last`.
   __device__ __forceinline__ void init(const char* p, int64_t stride, int64_t plane_bytes, int64_t first, int64_t rows,
@@ -241,7 +239,7 @@ struct Copy {
     base = p + (OUTER ? first * 2 : first * stride);
     step = OUTER ? kStageRows * stride : kStageBytes;
 #pragma unroll
-    for (int h = 0; h < kCopies; ++h) {
+    for (int h = 0; h < COUNT; ++h) {
       const int q = w + WAVES * h;
       if constexpr (OUTER) {
         const int row = 4 * (q & 15) + lane / 16, chunk = (lane % 16) ^ swz<16>(row), col = (q >> 4) * 128 + chunk * 8;
@@ -259,7 +257,7 @@ struct Copy {
   __device__ __forceinline__ void issue(lds_char* dst, int64_t t, int p, uint32_t last, uint32_t none, int w) const {
     const rsrc_t r = make_rsrc(base + p * plane + t * step, kBuffer);
 #pragma unroll
-    for (int h = 0; h < kCopies; ++h) {
+    for (int h = 0; h < COUNT; ++h) {
       const uint32_t o = off[h] | (tail[h] & last) | none;
       __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(dst + (w + WAVES * h) * 1024),
                                                16, (int)o, 0, 0, 0);
@@ -313,16 +311,20 @@ __device__ __forceinline__ void stage_barrier() {
 constexpr int kBand = 8;
 constexpr int kStrip = 72;  // floats from one row of a strip to the next: its halves' rows fall in other banks
 
+constexpr int threads_of(int bm, int bn) { return bm * bn > 192 * 128 ? 512 : 256; }
+
 enum class Form { kBf16, kParts, kE4m3 };
 
 // One BM x BN tile of c over one range of the sum. A wave has 32 MI x 64 of the tile.
 template <bool OA, bool OB, Form FORM, int BM, int BN>
-__global__ void __launch_bounds__(2 * BM, 2) product_kernel(ProductArgs g) {
-  constexpr int WAVES = BM / 32, NI = 2, WN = BN / 64, WM = WAVES / WN, MI = BM / WM / 32;
+__global__ void __launch_bounds__((threads_of(BM, BN)), 2) product_kernel(ProductArgs g) {
+  constexpr int WAVES = (threads_of(BM, BN)) / 64, NI = 2, WN = BN / 64, WM = WAVES / WN, MI = BM / WM / 32;
   constexpr int STAGE = (BM + BN) * kStageBytes;
   constexpr bool E4M3 = FORM == Form::kE4m3, PARTS = FORM == Form::kParts;
   constexpr bool PLAIN = OB;  // a gradient: no epilogue but the rounding
-  static_assert(WAVES * kCopies * 1024 == BM * kStageBytes && BM == BN, "copies a wave and operand");
+  constexpr int CA = BM / 8 / WAVES, CB = BN / 8 / WAVES;  // copies a wave and operand
+  static_assert(CA * WAVES * 8 == BM && CB * WAVES * 8 == BN && WM * MI * 32 == BM, "whole copies and blocks");
+  static_assert((!OA || BM % 128 == 0) && (!OB || BN % 128 == 0), "outer operands lie in 128 columns");
   // One array a stage: the compiler waits for the copies into the array that a read names, and for those alone.
   __shared__ __align__(256) char lds0[STAGE], lds1[STAGE];
   lds_char *const s0 = (lds_char*)lds0, *const s1 = (lds_char*)lds1;
@@ -341,8 +343,8 @@ __global__ void __launch_bounds__(2 * BM, 2) product_kernel(ProductArgs g) {
   const int64_t t1 = t0 + g.chunk < stages ? t0 + g.chunk : stages;
   const int steps = (int)(t1 - t0) * (PARTS ? 6 : 1);
 
-  Copy<OA, WAVES> ca;
-  Copy<OB, WAVES> cb;
+  Copy<OA, WAVES, CA> ca;
+  Copy<OB, WAVES, CB> cb;
   ca.init(g.a, g.a_stride, g.a_plane, i0, g.e.m, g.k, size, stages - 1, w, lane);
   cb.init(g.b, g.b_stride, g.b_plane, j0, g.e.n, g.k, size, stages - 1, w, lane);
   int64_t at = t0;  // the stage copied next, and its term
@@ -604,7 +606,7 @@ __global__ void __launch_bounds__(256) join_kernel(ProductArgs g) {
 template <bool OA, bool OB, Form FORM, int BM, int BN>
 hipError_t launch_tile(const ProductArgs& g, hipStream_t stream) {
   const int64_t tiles = ((g.e.m + BM - 1) / BM) * ((g.e.n + BN - 1) / BN);
-  hipLaunchKernelGGL((product_kernel<OA, OB, FORM, BM, BN>), dim3((unsigned)(tiles * g.splits)), dim3(2 * BM), 0, stream, g);
+  hipLaunchKernelGGL((product_kernel<OA, OB, FORM, BM, BN>), dim3((unsigned)(tiles * g.splits)), dim3((threads_of(BM, BN))), 0, stream, g);
   if (hipError_t e = hipGetLastError(); e != hipSuccess || !g.part) return e;
   const int64_t threads = g.e.m * (g.part_row / 8);
   hipLaunchKernelGGL((join_kernel<OA, OB, FORM>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, stream, g);
@@ -614,6 +616,9 @@ hipError_t launch_tile(const ProductArgs& g, hipStream_t stream) {
 template <bool OA, bool OB, Form FORM>
 hipError_t launch_operands(int tile, const ProductArgs& g, hipStream_t stream) {
   if (tile == 0) return launch_tile<OA, OB, FORM, 256, 256>(g, stream);
+  if constexpr (!OA) {
+    if (tile == 1) return launch_tile<OA, OB, FORM, 192, 128>(g, stream);
+  }
   return launch_tile<OA, OB, FORM, 128, 128>(g, stream);
 }
 

@@ -128,20 +128,21 @@ struct Plan {
   int32_t splits, chunk;
 };
 
-Plan plan(int64_t m, int64_t n, int64_t k, int32_t op) {
+Plan plan(int64_t m, int64_t n, int64_t k, int32_t op, bool outer) {
   const int64_t stages = std::max<int64_t>(1, parts(k * (op == kOpE4m3 ? 1 : 2), kStageBytes));
   Plan best{0, 1, (int32_t)stages};
   double least = 0;
   for (int t = 0; t < kTileShapes; ++t) {
+    if (t == 1) continue;
     const int64_t tiles = parts(m, kTiles[t].m) * parts(n, kTiles[t].n);
     const double per_stage = (t == 0 ? 1.0 : 0.3) * (op == kOpF32 ? 6 : 1), ends = t == 0 ? 6.0 : 3.0;  // us
-    for (int64_t want = 1; want <= 64; want *= 2) {
+    for (int64_t want = 1; want <= 64; ++want) {
       const int64_t chunk = parts(stages, want), splits = parts(stages, chunk);
       if (splits != want && want > 1) continue;
       if (want > 1 && chunk < 2) break;
       const double join = splits > 1 ? 4.0 + (double)(splits + 1) * m * n * 4 / 4e6 : 0;
       const double time = (double)parts(tiles * splits, kCus) * (per_stage * chunk + ends) + join;
-      if ((t == 0 && want == 1) || time < least) {
+      if (least == 0 || time < least) {
         least = time;
         best = {t, (int32_t)splits, (int32_t)chunk};
       }
@@ -160,7 +161,7 @@ struct Product {
   // Sizes and plan; `sums`: the column sums of a are wanted.
   void shape(Operands h, int64_t m, int64_t n, int64_t k, int32_t o, bool sums, Workspace& ws) {
     how = h, op = o;
-    p = plan(m, n, k, op);
+    p = plan(m, n, k, op, how == Operands::kOuterOuter);
     g.k = k;
     g.splits = p.splits;
     g.chunk = p.chunk;

@@ -13,8 +13,8 @@ import ctypes
 import torch
 
 from . import _native as nat
-from .rms import _Q8, _no_grad, _needs, rows_of
-from .rows import _DTYPES, _addr, _stream, as_torch
+from .rms import _Q8, _needs, _no_grad, launch, rows_of
+from .rows import _DTYPES, _addr, as_torch
 
 
 def _check(x, weight, bias, residual, dtype, lead):
@@ -51,13 +51,12 @@ def _forward(x, weight, bias, residual, activation, keep):
   rr, rs = rows_of(residual) if residual is not None else (None, 0)
   bias = bias.contiguous() if bias is not None else None
   L = nat.lib()
-  with torch.cuda.device(x.device):
-    out = torch.empty((*lead, outs), dtype=x.dtype, device=x.device)
-    pre = torch.empty_like(out) if keep else None
-    d = nat.LinearDesc(x.numel() // ins, xs, ws, rs, ins, outs, _DTYPES[x.dtype], activation)
-    work, size = _workspace(L.fwn_linear_act_workspace_size, d, x.device, xr, wr)
-    nat.check(L.fwn_linear_act_launch(d, _addr(xr), _addr(wr), _addr(bias), _addr(rr), _addr(out), _addr(pre),
-                                      _addr(work), size, _stream(x)))
+  out = torch.empty((*lead, outs), dtype=x.dtype, device=x.device)
+  pre = torch.empty_like(out) if keep else None
+  d = nat.LinearDesc(x.numel() // ins, xs, ws, rs, ins, outs, _DTYPES[x.dtype], activation)
+  work, size = _workspace(L.fwn_linear_act_workspace_size, d, x.device, xr, wr)
+  launch(x, L.fwn_linear_act_launch, d, _addr(xr), _addr(wr), _addr(bias), _addr(rr), _addr(out), _addr(pre), _addr(work),
+         size)
   return out, pre
 
 
@@ -117,12 +116,11 @@ class _LinearAct(torch.autograd.Function):
     wr, ws = rows_of(weight) if need_x else (None, 0)
     d = nat.LinearDesc(x_shape[0], xs, ws, 0, ins, outs, _DTYPES[g.dtype], act)
     L = nat.lib()
-    with torch.cuda.device(g.device):
-      gx, gw, gb = (torch.empty(shape, dtype=g.dtype, device=g.device) if need else None
-                    for shape, need in zip((x_shape, w_shape, (outs,)), needs))
-      work, size = _workspace(L.fwn_linear_act_bwd_workspace_size, d, g.device, xr, wr, g, gx, gw, gb)
-      nat.check(L.fwn_linear_act_bwd_launch(d, _addr(xr), _addr(wr), _addr(pre), _addr(g), _addr(gx), _addr(gw), _addr(gb),
-                                            _addr(work), size, _stream(g)))
+    gx, gw, gb = (torch.empty(shape, dtype=g.dtype, device=g.device) if need else None
+                  for shape, need in zip((x_shape, w_shape, (outs,)), needs))
+    work, size = _workspace(L.fwn_linear_act_bwd_workspace_size, d, g.device, xr, wr, g, gx, gw, gb)
+    launch(g, L.fwn_linear_act_bwd_launch, d, _addr(xr), _addr(wr), _addr(pre), _addr(g), _addr(gx), _addr(gw), _addr(gb),
+           _addr(work), size)
     return gx, gw, gb, g_res, None
 
 
@@ -177,10 +175,9 @@ def linear_act_q8(x, x_scale, weight, weight_scale, bias=None, *, activation=Non
   bias = bias.contiguous() if bias is not None else None
   x_scale, weight_scale = x_scale.contiguous(), weight_scale.contiguous()
   L = nat.lib()
-  with torch.cuda.device(x.device):
-    out = torch.empty((*lead, outs), dtype=dtype, device=x.device)
-    d = nat.LinearDesc(x.numel() // ins, xs, ws, rs, ins, outs, _DTYPES[dtype], act)
-    work, size = _workspace(L.fwn_linear_act_q8_workspace_size, d, x.device, xr, wr)
-    nat.check(L.fwn_linear_act_q8_launch(d, _addr(xr), _addr(x_scale), _addr(wr), _addr(weight_scale), _addr(bias),
-                                         _addr(rr), _addr(out), _addr(work), size, _stream(x)))
+  out = torch.empty((*lead, outs), dtype=dtype, device=x.device)
+  d = nat.LinearDesc(x.numel() // ins, xs, ws, rs, ins, outs, _DTYPES[dtype], act)
+  work, size = _workspace(L.fwn_linear_act_q8_workspace_size, d, x.device, xr, wr)
+  launch(x, L.fwn_linear_act_q8_launch, d, _addr(xr), _addr(x_scale), _addr(wr), _addr(weight_scale), _addr(bias), _addr(rr),
+         _addr(out), _addr(work), size)
   return out
