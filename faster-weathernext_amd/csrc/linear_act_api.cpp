@@ -90,61 +90,68 @@ struct Workspace {
   }
 };
 
-// A matrix in rows as the product kernel reads it: as it lies where it is bf16 or e4m3 in whole aligned 16
-// bytes, else laid out in the workspace.
+// A matrix in rows as the product kernels read it: as it lies where it is bf16 or e4m3 in whole aligned 16 bytes or
+// float32, else laid out in the workspace.
 struct Matrix {
   const void* src;
   int64_t rows, cols, stride;  // elements
   int32_t op;
-  char* at;                    // laid out: where
-  int64_t row_bytes, plane;
-  bool laid;
+  char* at;
+  int64_t row_bytes;
+  bool laid, vec;
 
   void place(const void* p, int64_t r, int64_t c, int64_t s, int32_t o, Workspace& ws, bool force = false) {
-    src = p, rows = r, cols = c, stride = s, op = o, plane = 0;
+    src = p, rows = r, cols = c, stride = s, op = o;
     const int64_t size = op_size(op);
-    laid = force || op == kOpF32 || ((uintptr_t)p & 15) || c * size % 16 || s * size % 16 || s * size > kMaxStride;
-    if (!laid) {
-      row_bytes = s * size;
-      at = (char*)p;
-      return;
-    }
-    plane = up(c * (op == kOpE4m3 ? 1 : 2), 16);
-    row_bytes = op == kOpF32 ? 3 * plane : plane;
+    vec = !(((uintptr_t)p & 15) || c * size % 16 || s * size % 16);
+    laid = force || s * size > kMaxStride || (op != kOpF32 && !vec);
+    row_bytes = s * size;
+    at = (char*)p;
+    if (!laid) return;
+    vec = true;
+    row_bytes = up(c, 8) * size;
+    if (row_bytes % 16) row_bytes = up(row_bytes, 16);
     at = ws.take((uint64_t)(rows * row_bytes));
   }
 
   hipError_t lay_out(hipStream_t stream) const {
     if (!laid) return hipSuccess;
-    return launch_layout({src, rows, cols, stride, op, at, row_bytes, plane}, stream);
+    return launch_layout({src, rows, cols, stride, op, at, row_bytes}, stream);
   }
 };
 
-// The tiles and ranges of the sum of one product. The estimate is the rounds of workgroups over the CUs times
-// the time of one: its share of the matrix units' time (a 128 x 128 tile's stage takes a fifth longer for its area),
-// its start and its end, and for split sums the partial products' trip through memory.
+// The tiles and ranges of the sum of one product, by an estimate of its time in us: a CU takes its share of the
+// workgroups one after the other, or two at a time where that fills it, each its stages and its ends (the
+// first loads and the epilogue); split sums add the partial products' trip through memory.
 struct Plan {
   int tile;
   int32_t splits, chunk;
 };
 
-Plan plan(int64_t m, int64_t n, int64_t k, int32_t op, bool outer) {
-  const int64_t stages = std::max<int64_t>(1, parts(k * (op == kOpE4m3 ? 1 : 2), kStageBytes));
-  Plan best{0, 1, (int32_t)stages};
-  double least = 0;
-  for (int t = 0; t < kTileShapes; ++t) {
-    if (t == 1) continue;
-    const int64_t tiles = parts(m, kTiles[t].m) * parts(n, kTiles[t].n);
-    const double per_stage = (t == 0 ? 1.0 : 0.3) * (op == kOpF32 ? 6 : 1), ends = t == 0 ? 6.0 : 3.0;  // us
+struct Cost {
+  int tile;
+  double alone, full, ends;  // a stage of the one workgroup on a CU, of one among those that fill it, a workgroup's ends
+};
+
+Plan plan(int64_t m, int64_t n, int64_t k, int32_t op) {
+  constexpr Cost bf16[] = {{256, 1.55, 1.55, 6.0}, {128, 0.6, 0.5, 2.2}}, f32[] = {{128, 1.3, 0.95, 2.5}};
+  const int64_t of = op == kOpF32 ? kStageF32 : op == kOpE4m3 ? kStageBytes : kStageRows;
+  const int64_t stages = std::max<int64_t>(1, parts(k, of));
+  Plan best{128, 1, (int32_t)stages};
+  double least = -1;
+  for (int t = 0; t < (op == kOpF32 ? 1 : 2); ++t) {
+    const Cost& c = op == kOpF32 ? f32[t] : bf16[t];
+    const int64_t tiles = parts(m, c.tile) * parts(n, c.tile);
     for (int64_t want = 1; want <= 64; ++want) {
       const int64_t chunk = parts(stages, want), splits = parts(stages, chunk);
-      if (splits != want && want > 1) continue;
-      if (want > 1 && chunk < 2) break;
+      if (splits != want) continue;
+      if (want > 1 && (chunk < 2 || tiles * want > 4 * kCus)) break;
+      const int64_t load = parts(tiles * splits, kCus);
       const double join = splits > 1 ? 4.0 + (double)(splits + 1) * m * n * 4 / 4e6 : 0;
-      const double time = (double)parts(tiles * splits, kCus) * (per_stage * chunk + ends) + join;
-      if (least == 0 || time < least) {
+      const double time = load * (chunk * (load == 1 ? c.alone : c.full) + c.ends) + join;
+      if (least < 0 || time < least) {
         least = time;
-        best = {t, (int32_t)splits, (int32_t)chunk};
+        best = {c.tile, (int32_t)splits, (int32_t)chunk};
       }
     }
   }
@@ -158,10 +165,10 @@ struct Product {
   int32_t op;
   Plan p;
 
-  // Sizes and plan; `sums`: the column sums of a are wanted.
+  // `sums`: the column sums of a are wanted.
   void shape(Operands h, int64_t m, int64_t n, int64_t k, int32_t o, bool sums, Workspace& ws) {
     how = h, op = o;
-    p = plan(m, n, k, op, how == Operands::kOuterOuter);
+    p = plan(m, n, k, op);
     g.k = k;
     g.splits = p.splits;
     g.chunk = p.chunk;
@@ -171,9 +178,10 @@ struct Product {
     g.part = p.splits > 1 ? (float*)ws.take((uint64_t)p.splits * m * g.part_row * sizeof(float)) : nullptr;
     g.sums = sums ? (float*)ws.take((uint64_t)p.splits * m * sizeof(float)) : nullptr;
   }
+
   hipError_t launch(const Matrix& a, const Matrix& b, hipStream_t stream) {
-    g.a = a.at, g.a_stride = a.row_bytes, g.a_plane = a.plane;
-    g.b = b.at, g.b_stride = b.row_bytes, g.b_plane = b.plane;
+    g.a = a.at, g.a_stride = a.row_bytes, g.a_vec = a.vec;
+    g.b = b.at, g.b_stride = b.row_bytes, g.b_vec = b.vec;
     const EpilogueArgs& e = g.e;
     g.e.vec = e.n % 8 == 0 && (!e.residual || (e.r_row % 8 == 0 && e.r_row <= FWN_LINEAR_ACT_MAX)) &&
               (((uintptr_t)e.out | (uintptr_t)e.pre | (uintptr_t)e.residual) & 15) == 0;
@@ -252,7 +260,7 @@ struct Backward {
     const bool act = d->activation != FWN_ACT_NONE, products = need_x || need_w;
     dz.place(gp, d->rows, d->outs, d->outs, op, ws, act);
     formed = products && dz.laid;
-    sums_in_product = need_b && need_w && !formed;
+    sums_in_product = need_b && need_w && !formed && op == kOpBf16;
     slope.chunk = slope_chunk(d->rows, d->outs);
     slope.blocks = (int32_t)std::max<int64_t>(1, parts(d->rows, slope.chunk));
     if (need_b && !sums_in_product) slope.part = (float*)ws.take((uint64_t)slope.blocks * d->outs * sizeof(float));
@@ -347,7 +355,6 @@ int fwn_linear_act_bwd_launch(const fwn_linear_desc* d, const void* x, const voi
     a.pre = pre;
     a.dz = b.formed ? b.dz.at : nullptr;
     a.dz_stride = b.dz.row_bytes;
-    a.dz_plane = b.dz.plane;
     a.rows = d->rows;
     a.outs = d->outs;
     a.dtype = d->dtype;

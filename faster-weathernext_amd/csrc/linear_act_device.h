@@ -1,0 +1,399 @@
+// Device-side building blocks of the linear layers' kernels: elements, activations, the epilogue of a product's
+// tile and the order of the tiles (gfx950).
+#pragma once
+
+#include "attn_bf16_tiles.h"
+#include "linear_act.h"
+
+namespace fwn {
+namespace {
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+__device__ __forceinline__ float as_float(uint32_t u) { return __builtin_bit_cast(float, u); }
+__device__ __forceinline__ uint32_t as_bits(float f) { return __builtin_bit_cast(uint32_t, f); }
+__device__ __forceinline__ uint32_t bf16_bits(float f) { return __builtin_bit_cast(uint16_t, (__bf16)f); }
+
+__device__ __forceinline__ float load_one(const void* p, int64_t i, int dtype) {
+  if (dtype == FWN_F32) return ((const float*)p)[i];
+  return as_float((uint32_t)((const uint16_t*)p)[i] << 16);
+}
+
+__device__ __forceinline__ void store_one(void* p, int64_t i, int dtype, float v) {
+  if (dtype == FWN_F32)
+    ((float*)p)[i] = v;
+  else
+    ((uint16_t*)p)[i] = (uint16_t)bf16_bits(v);
+}
+
+// Eight consecutive elements, 16-byte aligned.
+__device__ __forceinline__ void load8(const void* p, int64_t i, int dtype, float (&f)[8]) {
+  if (dtype == FWN_F32) {
+    const u32x4* q = (const u32x4*)((const float*)p + i);
+    const u32x4 v0 = q[0], v1 = q[1];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t a = v0[k], b = v1[k];
+      f[k] = as_float(a);
+      f[4 + k] = as_float(b);
+    }
+  } else {
+    const u32x4 v = *(const u32x4*)((const uint16_t*)p + i);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t u = v[k];
+      f[2 * k] = as_float(u << 16);
+      f[2 * k + 1] = as_float(u & 0xffff0000u);
+    }
+  }
+}
+
+__device__ __forceinline__ u32x4 pack8(const float (&f)[8]) {
+  u32x4 v;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) v[k] = bf16_bits(f[2 * k]) | bf16_bits(f[2 * k + 1]) << 16;
+  return v;
+}
+
+__device__ __forceinline__ void store8(void* p, int64_t i, int dtype, const float (&f)[8]) {
+  if (dtype == FWN_F32) {
+    u32x4* q = (u32x4*)((float*)p + i);
+    q[0] = u32x4{as_bits(f[0]), as_bits(f[1]), as_bits(f[2]), as_bits(f[3])};
+    q[1] = u32x4{as_bits(f[4]), as_bits(f[5]), as_bits(f[6]), as_bits(f[7])};
+  } else {
+    *(u32x4*)((uint16_t*)p + i) = pack8(f);
+  }
+}
+
+// e^x and 1 / x on the transcendental unit, within two units in the last place.
+__device__ __forceinline__ float fast_exp(float x) { return fast_exp2(x * LOG2E); }
+__device__ __forceinline__ float fast_rcp(float x) { return __builtin_amdgcn_rcpf(x); }
+
+// erf by Abramowitz and Stegun's 7.1.26, off by at most 1.5e-7 (a value times z / 2 here).
+__device__ __forceinline__ float erf_of(float x) {
+  const float y = __builtin_fabsf(x), t = fast_rcp(fmaf(0.3275911f, y, 1.f));
+  float p = fmaf(1.061405429f, t, -1.453152027f);
+  p = fmaf(p, t, 1.421413741f);
+  p = fmaf(p, t, -0.284496736f);
+  p = fmaf(p, t, 0.254829592f);
+  return __builtin_copysignf(1.f - p * t * fast_exp(-y * y), x);
+}
+
+constexpr float kTanh = 0.7978845608028654f, kCube = 0.044715f;  // gelu_tanh: u = kTanh (z + kCube z^3)
+
+// act(z). The tanh form is z / (1 + e^(-2u)).
+template <int KIND>
+__device__ __forceinline__ float activate(float z) {
+  if constexpr (KIND == FWN_ACT_RELU) return z > 0.f || z != z ? z : 0.f;
+  if constexpr (KIND == FWN_ACT_GELU) return 0.5f * z * (1.f + erf_of(z * 0.7071067811865476f));
+  if constexpr (KIND == FWN_ACT_GELU_TANH)
+    return z * fast_rcp(1.f + fast_exp2(z * fmaf(z * z, -2.f * kTanh * kCube * LOG2E, -2.f * kTanh * LOG2E)));
+  if constexpr (KIND == FWN_ACT_SILU) return z * fast_rcp(1.f + fast_exp(-z));
+  return z;
+}
+
+// act'(z).
+template <int KIND>
+__device__ __forceinline__ float slope(float z) {
+  if constexpr (KIND == FWN_ACT_RELU) return z > 0.f ? 1.f : 0.f;
+  if constexpr (KIND == FWN_ACT_GELU)
+    return 0.5f * (1.f + erf_of(z * 0.7071067811865476f)) + z * fast_exp(-0.5f * z * z) * 0.3989422804014327f;
+  if constexpr (KIND == FWN_ACT_GELU_TANH) {
+    // p = 1 / (1 + e^(-2u)), p + 2 z p (1 - p) u'; beyond 12 it is 0 or 1, and a large z^2 would meet that 0.
+    const float y = z > 12.f ? 12.f : z < -12.f ? -12.f : z, q = y * y;
+    const float p = fast_rcp(1.f + fast_exp2(y * fmaf(q, -2.f * kTanh * kCube * LOG2E, -2.f * kTanh * LOG2E)));
+    return fmaf(2.f * y * p * (1.f - p), fmaf(q, 3.f * kTanh * kCube, kTanh), p);
+  }
+  if constexpr (KIND == FWN_ACT_SILU) {
+    const float p = fast_rcp(1.f + fast_exp(-z)), y = p > 0.f ? z : 0.f;
+    return p * fmaf(y, 1.f - p, 1.f);
+  }
+  return 1.f;
+}
+
+// Calls f with the activation as a compile-time constant.
+template <int KIND>
+struct Act {
+  static constexpr int kind = KIND;
+};
+template <bool PLAIN, typename F>
+__device__ __forceinline__ void with_activation(int kind, F&& f) {
+  if constexpr (PLAIN) return f(Act<FWN_ACT_NONE>());
+  switch (kind) {
+    case FWN_ACT_RELU: return f(Act<FWN_ACT_RELU>());
+    case FWN_ACT_GELU: return f(Act<FWN_ACT_GELU>());
+    case FWN_ACT_GELU_TANH: return f(Act<FWN_ACT_GELU_TANH>());
+    case FWN_ACT_SILU: return f(Act<FWN_ACT_SILU>());
+    default: return f(Act<FWN_ACT_NONE>());
+  }
+}
+
+// What the epilogue needs of the columns col .. col + 7.
+struct Columns {
+  float bias[8], scale[8];
+
+  __device__ __forceinline__ void load(const EpilogueArgs& e, int64_t col) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const bool in = col + k < e.n;
+      bias[k] = e.bias && in ? load_one(e.bias, col + k, e.dtype) : 0.f;
+      scale[k] = e.b_scale && in ? e.b_scale[col + k] : 1.f;
+    }
+  }
+};
+
+// The epilogue of z[row, col .. col + 7], row < m; columns from n on are dropped.
+template <int KIND>
+__device__ __forceinline__ void finish(const EpilogueArgs& e, int64_t row, int64_t col, float (&v)[8], const Columns& c) {
+  if (e.a_scale) {
+    const float s = e.a_scale[row];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] *= s * c.scale[k];
+  }
+#pragma unroll
+  for (int k = 0; k < 8; ++k) v[k] += c.bias[k];
+  const int64_t at = row * e.n + col;
+  if (e.vec) {
+    if (col >= e.n) return;
+    if (e.pre) store8(e.pre, at, e.dtype, v);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = activate<KIND>(v[k]);
+    if (e.residual) {
+      float r[8];
+      load8(e.residual, row * e.r_row + col, e.dtype, r);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] += r[k];
+    }
+    store8(e.out, at, e.dtype, v);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if (col + k >= e.n) break;
+      if (e.pre) store_one(e.pre, at + k, e.dtype, v[k]);
+      float o = activate<KIND>(v[k]);
+      if (e.residual) o += load_one(e.residual, row * e.r_row + col + k, e.dtype);
+      store_one(e.out, at + k, e.dtype, o);
+    }
+  }
+}
+
+// Offsets with the top bit set lie past every buffer's end: loads give zeros and stores are dropped.
+constexpr uint32_t kNowhere = 0x80000000u, kBuffer = 0x7fffffffu;
+
+// What a workgroup computes: a tile of c and a range of the sum.
+struct Work {
+  int split;
+  int64_t i0, j0;
+};
+
+constexpr int kBand = 8;
+
+// Workgroups go to the 8 XCDs in turn: each takes a contiguous range of (range of the sum, tile). Tiles run in
+// bands of kBand rows of them, column by column: what runs at once on an XCD shares rows of both operands.
+template <int BM, int BN>
+__device__ __forceinline__ Work work_of(const EpilogueArgs& e) {
+  const int total = (int)gridDim.x, xcd = (int)blockIdx.x & 7, per = total >> 3, rem = total & 7;
+  const int id = xcd * per + (xcd < rem ? xcd : rem) + ((int)blockIdx.x >> 3);
+  const int tn = (int)((e.n + BN - 1) / BN), tm = (int)((e.m + BM - 1) / BM), tiles = tm * tn;
+  Work k;
+  k.split = id / tiles;
+  const int tile = id - k.split * tiles, band = tile / (kBand * tn), in = tile - band * (kBand * tn);
+  const int high = tm - band * kBand < kBand ? tm - band * kBand : kBand;
+  k.i0 = (int64_t)(band * kBand + in % high) * BM;
+  k.j0 = (int64_t)(in / high) * BN;
+  return k;
+}
+
+typedef __attribute__((address_space(3))) float* strip_ptr;
+constexpr int kStrip = 72;                      // floats from one row of a strip to the next: its halves' rows fall in other banks
+constexpr int kStripBytes = 32 * kStrip * 4;  // of LDS, for each wave
+
+// The epilogue of a wave's 32 MI x 64 part (from row wm and column wn) of a BM-row tile: 32 rows at a time through
+// the wave's strip of LDS to rows of eight columns a lane, or of one column a lane where rows are not whole aligned
+// eights. PLAIN: no epilogue but the rounding (gradients). F32: 1 the outputs are float32, 0 bf16, -1 either.
+// mend(row, col, v) may put right outputs before the epilogue.
+template <int BM, int MI, bool PLAIN, int F32, bool SCALED, typename Mend>
+__device__ __forceinline__ void write_tile(const ProductArgs& g, const Work& k, const f32x16 (&acc)[MI][2], strip_ptr strip,
+                                           int wm, int wn, int lane, const Mend& mend) {
+  const int j = lane & 31, half = lane >> 5;
+  const auto to_strip = [&](int m) {
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) strip[(8 * (r >> 2) + 4 * half + (r & 3)) * kStrip + 32 * n + j] = acc[m][n][r];
+    __builtin_amdgcn_wave_barrier();
+  };
+  const EpilogueArgs& e = g.e;
+  const int rows = (int)(e.m - k.i0 < BM ? e.m - k.i0 : BM);  // of the tile
+  if (g.part || e.vec) {
+    // Offsets in the tile.
+    const bool f32 = g.part || F32 == 1 || (F32 == -1 && e.dtype == FWN_F32);
+    const int64_t width = g.part ? g.part_row : e.n;
+    const uint32_t shift = f32 ? 2 : 1;
+    char* const to = g.part ? (char*)(g.part + (int64_t)k.split * e.m * g.part_row) : (char*)e.out;
+    const rsrc_t ro = make_rsrc(to + ((k.i0 * width + k.j0) << shift), kBuffer);
+    const rsrc_t rp = make_rsrc((char*)e.pre + ((k.i0 * width + k.j0) << shift), kBuffer);
+    const rsrc_t rr = make_rsrc((const char*)e.residual + ((k.i0 * e.r_row + k.j0) << shift), kBuffer);
+    const bool pre = !PLAIN && !g.part && e.pre, residual = !PLAIN && !g.part && e.residual;
+    const int sub = lane >> 3, at_col = wn + 8 * (lane & 7);  // this lane's row of eight and its columns of the tile
+    const int64_t col = k.j0 + at_col;
+    const uint32_t nowhere = col < e.n ? 0 : kNowhere;
+    Columns c;
+    if (!PLAIN && !g.part) c.load(e, col);
+    const auto load = [&](rsrc_t r, uint32_t o, float(&f)[8]) {
+      const u32x4 lo = bload16(r, o), hi = f32 ? bload16(r, o + 16) : lo;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t x = lo[i], y = hi[i];
+        if (f32) {
+          f[i] = as_float(x);
+          f[4 + i] = as_float(y);
+        } else {
+          f[2 * i] = as_float(x << 16);
+          f[2 * i + 1] = as_float(x & 0xffff0000u);
+        }
+      }
+    };
+    const auto store = [&](rsrc_t r, uint32_t o, const float(&f)[8]) {
+      if (f32) {
+        __builtin_amdgcn_raw_buffer_store_b128(u32x4{as_bits(f[0]), as_bits(f[1]), as_bits(f[2]), as_bits(f[3])}, r, (int)o, 0, 0);
+        __builtin_amdgcn_raw_buffer_store_b128(u32x4{as_bits(f[4]), as_bits(f[5]), as_bits(f[6]), as_bits(f[7])}, r, (int)(o + 16), 0, 0);
+      } else {
+        __builtin_amdgcn_raw_buffer_store_b128(pack8(f), r, (int)o, 0, 0);
+      }
+    };
+    with_activation<PLAIN>(g.part ? FWN_ACT_NONE : e.activation, [&](auto act) {
+#pragma unroll
+      for (int m = 0; m < MI; ++m) {
+        to_strip(m);
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+          const int row = wm + 32 * m + 8 * p + sub;
+          const uint32_t out = (row < rows ? 0 : kNowhere) | nowhere;
+          const uint32_t o = out | (((uint32_t)row * (uint32_t)width + (uint32_t)at_col) << shift);
+          float v[8], r[8];
+          if (residual) load(rr, out | (((uint32_t)row * (uint32_t)e.r_row + (uint32_t)at_col) << shift), r);
+          const auto* q = (const __attribute__((address_space(3))) f32x4*)(strip + (8 * p + sub) * kStrip + 8 * (lane & 7));
+          const f32x4 lo = q[0], hi = q[1];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float x = lo[i], y = hi[i];
+            v[i] = x;
+            v[4 + i] = y;
+          }
+          if (!g.part) {
+            if (out == 0) mend(k.i0 + row, col, v);
+            if (SCALED) {
+              const float s = row < rows ? e.a_scale[k.i0 + row] : 0.f;
+#pragma unroll
+              for (int i = 0; i < 8; ++i) v[i] *= s * c.scale[i];
+            }
+            if (!PLAIN) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) v[i] += c.bias[i];
+              if (pre) store(rp, o, v);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) v[i] = activate<decltype(act)::kind>(v[i]);
+              if (residual) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] += r[i];
+              }
+            }
+          }
+          store(ro, o, v);
+        }
+        __builtin_amdgcn_wave_barrier();
+      }
+    });
+    return;
+  }
+  const int64_t col = k.j0 + wn + lane;
+  const bool in = col < e.n;
+  const float bias = !PLAIN && e.bias && in ? load_one(e.bias, col, e.dtype) : 0.f;
+  const float scale = SCALED && in ? e.b_scale[col] : 1.f;
+  with_activation<PLAIN>(e.activation, [&](auto act) {
+#pragma unroll
+    for (int m = 0; m < MI; ++m) {
+      to_strip(m);
+      const int from = wm + 32 * m, count = rows - from < 32 ? rows - from : 32;
+      if (in) {
+#pragma unroll 4
+        for (int r = 0; r < count; ++r) {
+          const int64_t row = k.i0 + from + r, at = row * e.n + col;
+          float v[1] = {strip[r * kStrip + lane]};
+          mend(row, col, v);
+          float z = v[0];
+          if (SCALED) z *= e.a_scale[row] * scale;
+          if (!PLAIN) {
+            z += bias;
+            if (e.pre) store_one(e.pre, at, e.dtype, z);
+            z = activate<decltype(act)::kind>(z);
+            if (e.residual) z += load_one(e.residual, row * e.r_row + col, e.dtype);
+          }
+          store_one(e.out, at, e.dtype, z);
+        }
+      }
+      __builtin_amdgcn_wave_barrier();
+    }
+  });
+}
+
+// float32 products are formed of three bf16 parts a value, an infinity's beside it zeros or NaN: outputs that came
+// out NaN are formed anew of the whole values. OUTER: the operand's rows are k.
+template <bool OA, bool OB>
+struct MendParts {
+  const ProductArgs& g;
+
+  template <bool OUTER>
+  __device__ __forceinline__ static float value(const char* p, int64_t stride, int64_t i, int64_t k) {
+    return *(const float*)(OUTER ? p + k * stride + i * 4 : p + i * stride + k * 4);
+  }
+
+  template <int N>
+  __device__ __forceinline__ void operator()(int64_t row, int64_t col, float (&v)[N]) const {
+    bool bad = false;
+#pragma unroll
+    for (int e = 0; e < N; ++e) bad |= v[e] != v[e];
+    if (!bad) return;
+    float s[N] = {};
+    for (int64_t k = 0; k < g.k; ++k) {
+      const float x = value<OA>(g.a, g.a_stride, row, k);
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        if (col + e < g.e.n) s[e] = fmaf(x, value<OB>(g.b, g.b_stride, col + e, k), s[e]);
+    }
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      if (v[e] != v[e]) v[e] = s[e];
+  }
+};
+
+struct MendNothing {
+  template <int N>
+  __device__ __forceinline__ void operator()(int64_t, int64_t, float (&)[N]) const {}
+};
+
+// The partial products added in the order of the splits, then the epilogue: eight columns a thread.
+template <bool PLAIN, typename Mend>
+__device__ __forceinline__ void join(const ProductArgs& g, const Mend& mend) {
+  const int64_t across = g.part_row / 8, id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t row = id / across, col = (id - row * across) * 8;
+  if (row >= g.e.m) return;
+  float v[8] = {};
+#pragma unroll 4
+  for (int s = 0; s < g.splits; ++s) {
+    float p[8];
+    load8(g.part, ((int64_t)s * g.e.m + row) * g.part_row + col, FWN_F32, p);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] += p[k];
+  }
+  Columns c;
+  c.load(g.e, col);
+  mend(row, col, v);
+  with_activation<PLAIN>(g.e.activation, [&](auto act) { finish<decltype(act)::kind>(g.e, row, col, v, c); });
+}
+
+inline dim3 join_grid(const ProductArgs& g) { return dim3((unsigned)((g.e.m * (g.part_row / 8) + 255) / 256)); }
+
+}  // namespace
+}  // namespace fwn

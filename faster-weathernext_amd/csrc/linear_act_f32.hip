@@ -1,0 +1,196 @@
+// The linear layers' products of float32 operands (gfx950), at float32's precision on the bf16 matrix units.
+//
+// A value is the exact sum of three bf16 parts: its top 8 significant bits, the next 8 and the last. Of the nine
+// products of parts the six above 2^-24 of the whole are formed and accumulated in float32, small ones first:
+// six bf16 MFMAs do what eight times as many clocks of float32 MFMAs do. The parts are formed on the way from memory to
+// LDS, so an operand of any strides and alignment is read where it lies, once a tile.
+//
+// A workgroup is 4 waves on a 128 x 128 tile, a wave 64 x 64: per 16 k it reads 12 KB of LDS for 24 MFMAs. One
+// stage of 32 k is 48 KB of parts, so that three workgroups share a CU: while one splits and writes its next stage,
+// loaded a stage ahead into registers, the others multiply.
+#include "linear_act_device.h"
+
+namespace fwn {
+namespace {
+
+constexpr int TILE = 128, STEP = 32, PLANE = TILE * STEP * 2, OPERAND = 3 * PLANE;
+
+// One operand's stages: 128 rows of 32 k ("inner") or 32 rows of k of 128 columns ("outer"), 16 values a thread.
+// In LDS a part is 128 rows of 64 bytes or 32 of 256, 16-byte chunks swizzled as for the bf16 kernels.
+template <bool OUTER>
+struct Operand {
+  const char* base;
+  int64_t step;      // bytes from one stage to the next
+  uint32_t off[4];   // of this thread's four fours of values
+  uint32_t lds[4];
+  int first_k[4], limit;  // inner: k in the stage; outer: the same, and columns of the four inside the operand
+  bool vec;          // fours of values are 16-byte aligned and whole
+  uint32_t at[OUTER ? 4 : 2];  // this lane's reads
+
+  __device__ __forceinline__ void init(const char* p, int64_t stride, int64_t first, int64_t rows, int64_t k, bool aligned,
+                                       int wave_first, int lane) {
+    base = p + (OUTER ? first * 4 : first * stride);
+    step = OUTER ? STEP * stride : STEP * 4;
+    vec = aligned;
+    const int t = (int)threadIdx.x;
+    limit = 4;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (OUTER) {
+        const int row = t / 32 + 8 * i, col = t % 32 * 4;
+        off[i] = first + col < rows ? (uint32_t)row * (uint32_t)stride + (uint32_t)col * 4 : kNowhere;
+        if (rows - first - col < 4) limit = (int)(rows - first - col);
+        first_k[i] = row;
+        lds[i] = row * 256 + (((col / 8) ^ swz<16>(row)) << 4) + (col % 8) * 2;
+      } else {
+        const int row = t / 8 + 32 * i, c = t % 8 * 4;
+        off[i] = first + row < rows ? (uint32_t)row * (uint32_t)stride + (uint32_t)c * 4 : kNowhere;
+        first_k[i] = c;
+        lds[i] = row * 64 + (((c / 8) ^ (row / 4 % 4)) << 4) + (c % 8) * 2;
+      }
+    }
+    const int i = lane & 31, g = lane >> 5;
+    if constexpr (OUTER) {
+      const int G = lane >> 4, u = lane & 15, e = u >> 2, q = u & 3;
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int r = 8 * g + 4 * h + e, chunk = 4 * ((wave_first + 32 * m) >> 5) + 2 * (G & 1) + (q >> 1);
+          at[2 * m + h] = r * 256 + ((chunk ^ swz<16>(r)) << 4) + (q & 1) * 8;
+        }
+    } else {
+      const int r = wave_first + i;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) at[c] = r * 64 + (((2 * c + g) ^ (r / 4 % 4)) << 4);
+    }
+  }
+
+  // Stage t's values; `left`: k from its first to the sum's end (what lies past it is zeros).
+  __device__ __forceinline__ void load(int64_t t, int64_t left, u32x4 (&v)[4]) const {
+    const rsrc_t r = make_rsrc(base + t * step, kBuffer);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (vec) {
+        v[i] = bload16(r, off[i] | (first_k[i] < left ? 0 : kNowhere));
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const bool in = OUTER ? e < limit && first_k[i] < left : first_k[i] + e < left;
+          v[i][e] = __builtin_amdgcn_raw_buffer_load_b32(r, (int)((off[i] + 4 * e) | (in ? 0 : kNowhere)), 0, 0);
+        }
+      }
+    }
+  }
+
+  // Their parts to LDS. An infinity or NaN gives NaN in the middle part, and so in every output that it feeds.
+  __device__ __forceinline__ void split(lds_char* to, const u32x4 (&v)[4]) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t part[3][4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t u = v[i][e];
+        const uint32_t u1 = as_bits(as_float(u) - as_float(u & 0xffff0000u));
+        part[0][e] = u;
+        part[1][e] = u1;
+        part[2][e] = as_bits(as_float(u1) - as_float(u1 & 0xffff0000u));
+      }
+#pragma unroll
+      for (int p = 0; p < 3; ++p)
+        *(__attribute__((address_space(3))) u32x2*)(to + p * PLANE + lds[i]) =
+            u32x2{__builtin_amdgcn_perm(part[p][1], part[p][0], 0x07060302), __builtin_amdgcn_perm(part[p][3], part[p][2], 0x07060302)};
+    }
+  }
+
+  // Block m's operand of half c of the stage in the part at `part`.
+  __device__ __forceinline__ u32x4 read(const lds_char* part, int m, int c) const {
+    if constexpr (OUTER) {
+      const u32x2 lo = tr_read(part + c * 4096, at[2 * m]), hi = tr_read(part + c * 4096, at[2 * m + 1]);
+      return u32x4{lo[0], lo[1], hi[0], hi[1]};
+    } else {
+      return row_read(part + m * 2048, at[c]);
+    }
+  }
+};
+
+template <bool OA, bool OB>
+__global__ void __launch_bounds__(256, 2) product_f32_kernel(ProductArgs g) {
+  __shared__ __align__(256) char lds[2 * OPERAND];
+  static_assert(sizeof(lds) >= 4 * kStripBytes, "the waves' strips");
+  lds_char* const sa = (lds_char*)lds;
+  lds_char* const sb = sa + OPERAND;
+  const int lane = (int)threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const Work k = work_of<TILE, TILE>(g.e);
+  const int64_t stages = (g.k + STEP - 1) / STEP, t0 = (int64_t)k.split * g.chunk;
+  const int64_t t1 = t0 + g.chunk < stages ? t0 + g.chunk : stages;
+  const int wm = w / 2 * 64, wn = w % 2 * 64;
+  Operand<OA> a;
+  Operand<OB> b;
+  a.init(g.a, g.a_stride, k.i0, g.e.m, g.k, g.a_vec, wm, lane);
+  b.init(g.b, g.b_stride, k.j0, g.e.n, g.k, g.b_vec, wn, lane);
+  f32x16 acc[2][2];
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int n = 0; n < 2; ++n) acc[m][n] = zero16();
+  u32x4 va[4], vb[4];
+  if (t0 < t1) {
+    a.load(t0, g.k - t0 * STEP, va);
+    b.load(t0, g.k - t0 * STEP, vb);
+  }
+  for (int64_t t = t0; t < t1; ++t) {
+    lds_barrier();  // every wave has read the last stage
+    a.split(sa, va);
+    b.split(sb, vb);
+    if (t + 1 < t1) {
+      a.load(t + 1, g.k - (t + 1) * STEP, va);
+      b.load(t + 1, g.k - (t + 1) * STEP, vb);
+    }
+    lds_barrier();
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      u32x4 fa[3][2], fb[3][2];
+#pragma unroll
+      for (int p = 2; p >= 0; --p)
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+          fa[p][m] = a.read(sa + p * PLANE, m, c);
+          fb[p][m] = b.read(sb + p * PLANE, m, c);
+        }
+      constexpr int pa[6] = {2, 0, 1, 1, 0, 0}, pb[6] = {0, 2, 1, 0, 1, 0};
+#pragma unroll
+      for (int i = 0; i < 6; ++i)
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+          for (int n = 0; n < 2; ++n) acc[m][n] = mfma_bf16(fa[pa[i]][m], fb[pb[i]][n], acc[m][n]);
+    }
+  }
+  __syncthreads();
+  write_tile<TILE, 2, OB, 1, false>(g, k, acc, (strip_ptr)(sa + w * kStripBytes), wm, wn, lane, MendParts<OA, OB>{g});
+}
+
+template <bool OA, bool OB>
+__global__ void __launch_bounds__(256) join_f32_kernel(ProductArgs g) {
+  join<OB>(g, MendParts<OA, OB>{g});
+}
+
+template <bool OA, bool OB>
+hipError_t launch(const ProductArgs& g, hipStream_t stream) {
+  const int64_t tiles = ((g.e.m + TILE - 1) / TILE) * ((g.e.n + TILE - 1) / TILE);
+  hipLaunchKernelGGL((product_f32_kernel<OA, OB>), dim3((unsigned)(tiles * g.splits)), dim3(256), 0, stream, g);
+  if (hipError_t e = hipGetLastError(); e != hipSuccess || !g.part) return e;
+  hipLaunchKernelGGL((join_f32_kernel<OA, OB>), join_grid(g), dim3(256), 0, stream, g);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_product_f32(Operands how, const ProductArgs& g, hipStream_t stream) {
+  if (how == Operands::kInnerInner) return launch<false, false>(g, stream);
+  if (how == Operands::kInnerOuter) return launch<false, true>(g, stream);
+  return launch<true, true>(g, stream);
+}
+
+}  // namespace fwn

@@ -1,0 +1,133 @@
+// Passes around the products of the linear layers (gfx950): operands laid out for them, dz = g act'(z) with its
+// column sums, and the sums of partial rows.
+#include "linear_act_device.h"
+
+namespace fwn {
+namespace {
+
+// Rows padded with zeros to 16 bytes, 16 bytes a thread.
+__global__ void __launch_bounds__(256) layout_kernel(LayoutArgs a) {
+  const int per = a.op == kOpE4m3 ? 16 : a.op == kOpBf16 ? 8 : 4;  // columns a thread
+  const int64_t across = (a.cols + per - 1) / per, id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t row = id / across, col = (id - row * across) * per;
+  if (row >= a.rows) return;
+  char* dst = a.dst + row * a.dst_stride + (id - row * across) * 16;
+  if (a.op == kOpE4m3) {
+    const uint8_t* p = (const uint8_t*)a.src + row * a.stride + col;
+    uint32_t d[4] = {};
+#pragma unroll
+    for (int k = 0; k < 16; ++k)
+      if (col + k < a.cols) d[k / 4] |= (uint32_t)p[k] << 8 * (k % 4);
+    *(u32x4*)dst = u32x4{d[0], d[1], d[2], d[3]};
+    return;
+  }
+  uint32_t d[4] = {};
+  if (a.op == kOpBf16) {
+    const uint16_t* p = (const uint16_t*)a.src + row * a.stride + col;
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (col + k < a.cols) d[k / 2] |= (uint32_t)p[k] << 16 * (k % 2);
+  } else {
+    const uint32_t* p = (const uint32_t*)a.src + row * a.stride + col;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (col + k < a.cols) d[k] = p[k];
+  }
+  *(u32x4*)dst = u32x4{d[0], d[1], d[2], d[3]};
+}
+
+// 256 columns by `chunk` rows a workgroup, eight columns of every eighth row a thread.
+template <int KIND>
+__global__ void __launch_bounds__(256) slope_kernel(SlopeArgs a) {
+  __shared__ float red[8][256];
+  const int across = (a.outs + 255) / 256, block = (int)blockIdx.x / across;
+  const int lane = (int)threadIdx.x & 31, own = (int)threadIdx.x >> 5;
+  const int col = ((int)blockIdx.x - block * across) * 256 + 8 * lane;
+  const int64_t r0 = (int64_t)block * a.chunk, r1 = r0 + a.chunk < a.rows ? r0 + a.chunk : a.rows;
+  const bool vec = a.outs % 8 == 0 && (((uintptr_t)a.g | (uintptr_t)a.pre) & 15) == 0;
+  float sum[8] = {};
+  if (col < a.outs) {
+    for (int64_t r = r0 + own; r < r1; r += 8) {
+      const int64_t at = r * a.outs + col;
+      float dz[8], z[8];
+      if (vec) {
+        load8(a.g, at, a.dtype, dz);
+        if (KIND != FWN_ACT_NONE) load8(a.pre, at, a.dtype, z);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const bool in = col + k < a.outs;
+          dz[k] = in ? load_one(a.g, at + k, a.dtype) : 0.f;
+          z[k] = in && KIND != FWN_ACT_NONE ? load_one(a.pre, at + k, a.dtype) : 0.f;
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        if constexpr (KIND != FWN_ACT_NONE) dz[k] *= slope<KIND>(z[k]);
+        sum[k] += dz[k];
+      }
+      if (a.dz) store8(a.dz + r * a.dz_stride, col, a.dtype, dz);
+    }
+  }
+  if (!a.part) return;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) red[own][8 * lane + k] = sum[k];
+  __syncthreads();
+  const int c = (int)threadIdx.x, to = col - 8 * lane + c;
+  if (to >= a.outs) return;
+  float s = red[0][c];
+#pragma unroll
+  for (int k = 1; k < 8; ++k) s += red[k][c];
+  a.part[(int64_t)block * a.outs + to] = s;
+}
+
+constexpr int kGroups = 16;  // shares of the partial rows that a workgroup adds in parallel
+
+__global__ void __launch_bounds__(64 * kGroups) column_sums_kernel(const float* part, int64_t count, int64_t n, void* out,
+                                                                   int dtype) {
+  __shared__ float red[kGroups][64];
+  const int lane = threadIdx.x & 63, grp = (int)threadIdx.x >> 6;
+  const int64_t c = (int64_t)blockIdx.x * 64 + lane;
+  float s = 0.f;
+  if (c < n) {
+#pragma unroll 8
+    for (int64_t b = grp; b < count; b += kGroups) s += part[b * n + c];
+  }
+  red[grp][lane] = s;
+  __syncthreads();
+  if (grp != 0 || c >= n) return;
+#pragma unroll
+  for (int k = 1; k < kGroups; ++k) s += red[k][lane];
+  store_one(out, c, dtype, s);
+}
+
+}  // namespace
+
+hipError_t launch_layout(const LayoutArgs& a, hipStream_t stream) {
+  const int per = a.op == kOpE4m3 ? 16 : a.op == kOpBf16 ? 8 : 4;
+  const int64_t threads = a.rows * ((a.cols + per - 1) / per);
+  if (threads == 0) return hipSuccess;
+  hipLaunchKernelGGL(layout_kernel, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, stream, a);
+  return hipGetLastError();
+}
+
+hipError_t launch_slope(const SlopeArgs& a, hipStream_t stream) {
+  const unsigned across = (unsigned)(a.outs + 255) / 256;
+  const dim3 grid(across * (unsigned)a.blocks), block(256);
+  switch (a.activation) {
+    case FWN_ACT_RELU: hipLaunchKernelGGL(slope_kernel<FWN_ACT_RELU>, grid, block, 0, stream, a); break;
+    case FWN_ACT_GELU: hipLaunchKernelGGL(slope_kernel<FWN_ACT_GELU>, grid, block, 0, stream, a); break;
+    case FWN_ACT_GELU_TANH: hipLaunchKernelGGL(slope_kernel<FWN_ACT_GELU_TANH>, grid, block, 0, stream, a); break;
+    case FWN_ACT_SILU: hipLaunchKernelGGL(slope_kernel<FWN_ACT_SILU>, grid, block, 0, stream, a); break;
+    default: hipLaunchKernelGGL(slope_kernel<FWN_ACT_NONE>, grid, block, 0, stream, a);
+  }
+  return hipGetLastError();
+}
+
+hipError_t launch_column_sums(const float* part, int64_t count, int64_t n, void* out, int dtype, hipStream_t stream) {
+  hipLaunchKernelGGL(column_sums_kernel, dim3((unsigned)((n + 63) / 64)), dim3(64 * kGroups), 0, stream, part, count, n,
+                     out, dtype);
+  return hipGetLastError();
+}
+
+}  // namespace fwn
