@@ -32,7 +32,6 @@ struct ProductArgs {
   const char* a;
   const char* b;
   int64_t a_stride, b_stride;  // bytes between rows, at most kMaxStride
-  bool a_vec, b_vec;           // float32 operands: aligned likewise
   int64_t k;
   int32_t splits;              // ranges of the sum, each `chunk` stages (the last may be shorter)
   int32_t chunk;

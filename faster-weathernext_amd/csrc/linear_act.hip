@@ -241,9 +241,9 @@ __global__ void __launch_bounds__((threads_of(BM)), 2) product_kernel(ProductArg
                                               lane, MendNothing());
 }
 
-template <bool PLAIN>
+template <bool PLAIN, int N>
 __global__ void __launch_bounds__(256) join_kernel(ProductArgs g) {
-  join<PLAIN>(g, MendNothing());
+  join<PLAIN, N>(g, MendNothing());
 }
 
 template <bool OA, bool OB, bool E4M3, int TILE>
@@ -252,7 +252,10 @@ hipError_t launch_tile(const ProductArgs& g, hipStream_t stream) {
   hipLaunchKernelGGL((product_kernel<OA, OB, E4M3, TILE, TILE>), dim3((unsigned)(tiles * g.splits)), dim3(threads_of(TILE)), 0,
                      stream, g);
   if (hipError_t e = hipGetLastError(); e != hipSuccess || !g.part) return e;
-  hipLaunchKernelGGL(join_kernel<OB>, join_grid(g), dim3(256), 0, stream, g);
+  if (g.e.vec)
+    hipLaunchKernelGGL((join_kernel<OB, 8>), join_grid(g), dim3(256), 0, stream, g);
+  else
+    hipLaunchKernelGGL((join_kernel<OB, 1>), join_grid(g), dim3(256), 0, stream, g);
   return hipGetLastError();
 }
 

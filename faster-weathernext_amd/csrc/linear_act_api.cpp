@@ -24,7 +24,7 @@ int check_desc(const fwn_linear_desc* d, const char* what) {
   if (d->rows < 0 || d->rows > (INT64_C(1) << 31)) return fail(FWN_ERR_INVALID_ARG, "%s: %lld rows", what, (long long)d->rows);
   const int64_t widest = INT64_C(1) << 30;
   if (d->x_stride < 0 || d->w_stride < 0 || d->r_stride < 0 || d->x_stride > widest || d->w_stride > widest ||
-      d->r_stride > widest)
+      d->r_stride > FWN_LINEAR_ACT_MAX)
     return fail(FWN_ERR_INVALID_ARG, "%s: strides %lld, %lld and %lld", what, (long long)d->x_stride,
                 (long long)d->w_stride, (long long)d->r_stride);
   const int64_t ins = (d->ins + 63) / 64, outs = (d->outs + 63) / 64, rows = (d->rows + 63) / 64, most = 1 << 23;
@@ -98,17 +98,15 @@ struct Matrix {
   int32_t op;
   char* at;
   int64_t row_bytes;
-  bool laid, vec;
+  bool laid;
 
   void place(const void* p, int64_t r, int64_t c, int64_t s, int32_t o, Workspace& ws, bool force = false) {
     src = p, rows = r, cols = c, stride = s, op = o;
     const int64_t size = op_size(op);
-    vec = !(((uintptr_t)p & 15) || c * size % 16 || s * size % 16);
-    laid = force || s * size > kMaxStride || (op != kOpF32 && !vec);
+    laid = force || s * size > kMaxStride || (op != kOpF32 && (((uintptr_t)p & 15) || c * size % 16 || s * size % 16));
     row_bytes = s * size;
     at = (char*)p;
     if (!laid) return;
-    vec = true;
     row_bytes = up(c, 8) * size;
     if (row_bytes % 16) row_bytes = up(row_bytes, 16);
     at = ws.take((uint64_t)(rows * row_bytes));
@@ -180,10 +178,10 @@ struct Product {
   }
 
   hipError_t launch(const Matrix& a, const Matrix& b, hipStream_t stream) {
-    g.a = a.at, g.a_stride = a.row_bytes, g.a_vec = a.vec;
-    g.b = b.at, g.b_stride = b.row_bytes, g.b_vec = b.vec;
+    g.a = a.at, g.a_stride = a.row_bytes;
+    g.b = b.at, g.b_stride = b.row_bytes;
     const EpilogueArgs& e = g.e;
-    g.e.vec = e.n % 8 == 0 && (!e.residual || (e.r_row % 8 == 0 && e.r_row <= FWN_LINEAR_ACT_MAX)) &&
+    g.e.vec = e.n % 8 == 0 && (!e.residual || e.r_row % 8 == 0) &&
               (((uintptr_t)e.out | (uintptr_t)e.pre | (uintptr_t)e.residual) & 15) == 0;
     return launch_product(how, op, p.tile, g, stream);
   }

@@ -142,7 +142,7 @@ struct Columns {
   }
 };
 
-// The epilogue of z[row, col .. col + 7], row < m; columns from n on are dropped.
+// The epilogue of z[row, col .. col + 7] in rows of whole aligned eights.
 template <int KIND>
 __device__ __forceinline__ void finish(const EpilogueArgs& e, int64_t row, int64_t col, float (&v)[8], const Columns& c) {
   if (e.a_scale) {
@@ -153,28 +153,16 @@ __device__ __forceinline__ void finish(const EpilogueArgs& e, int64_t row, int64
 #pragma unroll
   for (int k = 0; k < 8; ++k) v[k] += c.bias[k];
   const int64_t at = row * e.n + col;
-  if (e.vec) {
-    if (col >= e.n) return;
-    if (e.pre) store8(e.pre, at, e.dtype, v);
+  if (e.pre) store8(e.pre, at, e.dtype, v);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = activate<KIND>(v[k]);
-    if (e.residual) {
-      float r[8];
-      load8(e.residual, row * e.r_row + col, e.dtype, r);
+  for (int k = 0; k < 8; ++k) v[k] = activate<KIND>(v[k]);
+  if (e.residual) {
+    float r[8];
+    load8(e.residual, row * e.r_row + col, e.dtype, r);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] += r[k];
-    }
-    store8(e.out, at, e.dtype, v);
-  } else {
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      if (col + k >= e.n) break;
-      if (e.pre) store_one(e.pre, at + k, e.dtype, v[k]);
-      float o = activate<KIND>(v[k]);
-      if (e.residual) o += load_one(e.residual, row * e.r_row + col + k, e.dtype);
-      store_one(e.out, at + k, e.dtype, o);
-    }
+    for (int k = 0; k < 8; ++k) v[k] += r[k];
   }
+  store8(e.out, at, e.dtype, v);
 }
 
 // Offsets with the top bit set lie past every buffer's end: loads give zeros and stores are dropped.
@@ -311,26 +299,51 @@ __device__ __forceinline__ void write_tile(const ProductArgs& g, const Work& k, 
   const bool in = col < e.n;
   const float bias = !PLAIN && e.bias && in ? load_one(e.bias, col, e.dtype) : 0.f;
   const float scale = SCALED && in ? e.b_scale[col] : 1.f;
+  const bool f32 = F32 == 1 || (F32 == -1 && e.dtype == FWN_F32);
+  const uint32_t shift = f32 ? 2 : 1;
+  const rsrc_t ro = make_rsrc((char*)e.out + ((k.i0 * e.n + k.j0) << shift), kBuffer);
+  const rsrc_t rp = make_rsrc((char*)e.pre + ((k.i0 * e.n + k.j0) << shift), kBuffer);
+  const rsrc_t rr = make_rsrc((const char*)e.residual + ((k.i0 * e.r_row + k.j0) << shift), kBuffer);
+  const auto store = [&](rsrc_t r, uint32_t o, float v) {
+    if (f32)
+      __builtin_amdgcn_raw_buffer_store_b32(as_bits(v), r, (int)o, 0, 0);
+    else
+      __builtin_amdgcn_raw_buffer_store_b16((uint16_t)bf16_bits(v), r, (int)o, 0, 0);
+  };
   with_activation<PLAIN>(e.activation, [&](auto act) {
 #pragma unroll
     for (int m = 0; m < MI; ++m) {
       to_strip(m);
-      const int from = wm + 32 * m, count = rows - from < 32 ? rows - from : 32;
-      if (in) {
-#pragma unroll 4
-        for (int r = 0; r < count; ++r) {
-          const int64_t row = k.i0 + from + r, at = row * e.n + col;
-          float v[1] = {strip[r * kStrip + lane]};
-          mend(row, col, v);
-          float z = v[0];
-          if (SCALED) z *= e.a_scale[row] * scale;
-          if (!PLAIN) {
-            z += bias;
-            if (e.pre) store_one(e.pre, at, e.dtype, z);
-            z = activate<decltype(act)::kind>(z);
-            if (e.residual) z += load_one(e.residual, row * e.r_row + col, e.dtype);
+#pragma unroll 1
+      for (int r0 = 0; r0 < 32; r0 += 8) {  // eight rows' residuals are on their way at once
+        uint32_t out[8];
+        float z[8], res[8];
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          const int row = wm + 32 * m + r0 + r;
+          out[r] = in && row < rows ? 0 : kNowhere;
+          res[r] = 0.f;
+          if (!PLAIN && e.residual) {
+            const uint32_t o = out[r] | (((uint32_t)row * (uint32_t)e.r_row + (uint32_t)(wn + lane)) << shift);
+            res[r] = f32 ? as_float(__builtin_amdgcn_raw_buffer_load_b32(rr, (int)o, 0, 0))
+                         : as_float((uint32_t)__builtin_amdgcn_raw_buffer_load_b16(rr, (int)o, 0, 0) << 16);
           }
-          store_one(e.out, at, e.dtype, z);
+          z[r] = strip[(r0 + r) * kStrip + lane];
+        }
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          const int row = wm + 32 * m + r0 + r;
+          const uint32_t o = out[r] | (((uint32_t)row * (uint32_t)e.n + (uint32_t)(wn + lane)) << shift);
+          float v[1] = {z[r]};
+          if (out[r] == 0) mend(k.i0 + row, col, v);
+          if (SCALED && row < rows) v[0] *= e.a_scale[k.i0 + row] * scale;
+          if (!PLAIN) {
+            v[0] += bias;
+            if (e.pre) store(rp, o, v[0]);
+            v[0] = activate<decltype(act)::kind>(v[0]);
+            if (e.residual) v[0] += res[r];
+          }
+          store(ro, o, v[0]);
         }
       }
       __builtin_amdgcn_wave_barrier();
@@ -373,27 +386,48 @@ struct MendNothing {
   __device__ __forceinline__ void operator()(int64_t, int64_t, float (&)[N]) const {}
 };
 
-// The partial products added in the order of the splits, then the epilogue: eight columns a thread.
-template <bool PLAIN, typename Mend>
+// The partial products added in the order of the splits, then the epilogue: N columns a thread, eight where rows are
+// whole aligned eights, else one, so that a wave's accesses still lie side by side.
+template <bool PLAIN, int N, typename Mend>
 __device__ __forceinline__ void join(const ProductArgs& g, const Mend& mend) {
-  const int64_t across = g.part_row / 8, id = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t row = id / across, col = (id - row * across) * 8;
-  if (row >= g.e.m) return;
-  float v[8] = {};
+  const EpilogueArgs& e = g.e;
+  const int64_t across = N == 8 ? g.part_row / 8 : e.n, id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t row = id / across, col = (id - row * across) * N;
+  if (row >= e.m) return;
+  float v[N] = {};
 #pragma unroll 4
   for (int s = 0; s < g.splits; ++s) {
-    float p[8];
-    load8(g.part, ((int64_t)s * g.e.m + row) * g.part_row + col, FWN_F32, p);
+    const int64_t at = ((int64_t)s * e.m + row) * g.part_row + col;
+    if constexpr (N == 8) {
+      float p[8];
+      load8(g.part, at, FWN_F32, p);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] += p[k];
+      for (int k = 0; k < 8; ++k) v[k] += p[k];
+    } else {
+      v[0] += g.part[at];
+    }
   }
-  Columns c;
-  c.load(g.e, col);
   mend(row, col, v);
-  with_activation<PLAIN>(g.e.activation, [&](auto act) { finish<decltype(act)::kind>(g.e, row, col, v, c); });
+  with_activation<PLAIN>(e.activation, [&](auto act) {
+    if constexpr (N == 8) {
+      Columns c;
+      c.load(e, col);
+      finish<decltype(act)::kind>(e, row, col, v, c);
+    } else {
+      float z = v[0];
+      if (e.a_scale) z *= e.a_scale[row] * e.b_scale[col];
+      if (e.bias) z += load_one(e.bias, col, e.dtype);
+      if (e.pre) store_one(e.pre, row * e.n + col, e.dtype, z);
+      z = activate<decltype(act)::kind>(z);
+      if (e.residual) z += load_one(e.residual, row * e.r_row + col, e.dtype);
+      store_one(e.out, row * e.n + col, e.dtype, z);
+    }
+  });
 }
 
-inline dim3 join_grid(const ProductArgs& g) { return dim3((unsigned)((g.e.m * (g.part_row / 8) + 255) / 256)); }
+inline dim3 join_grid(const ProductArgs& g) {
+  return dim3((unsigned)((g.e.m * (g.e.vec ? g.part_row / 8 : g.e.n) + 255) / 256));
+}
 
 }  // namespace
 }  // namespace fwn

@@ -23,15 +23,16 @@ struct Operand {
   int64_t step;      // bytes from one stage to the next
   uint32_t off[4];   // of this thread's four fours of values
   uint32_t lds[4];
-  int first_k[4], limit;  // inner: k in the stage; outer: the same, and columns of the four inside the operand
-  bool vec;          // fours of values are 16-byte aligned and whole
+  int first_k[4];    // k of a four in the stage
+  int limit;         // outer: columns of the fours inside the operand
+  bool whole;        // fours do not end inside: of the sum (inner), or of the tile's columns (outer)
   uint32_t at[OUTER ? 4 : 2];  // this lane's reads
 
-  __device__ __forceinline__ void init(const char* p, int64_t stride, int64_t first, int64_t rows, int64_t k, bool aligned,
-                                       int wave_first, int lane) {
+  __device__ __forceinline__ void init(const char* p, int64_t stride, int64_t first, int64_t rows, int64_t k, int wave_first,
+                                       int lane) {
     base = p + (OUTER ? first * 4 : first * stride);
     step = OUTER ? STEP * stride : STEP * 4;
-    vec = aligned;
+    whole = OUTER ? rows % 4 == 0 || first + TILE <= rows : k % 4 == 0;
     const int t = (int)threadIdx.x;
     limit = 4;
 #pragma unroll
@@ -66,20 +67,21 @@ struct Operand {
     }
   }
 
-  // Stage t's values; `left`: k from its first to the sum's end (what lies past it is zeros).
+  // Stage t's values; `left`: k from its first to the sum's end (what lies past it is zeros). Fours need no alignment
+  // but their elements'.
   __device__ __forceinline__ void load(int64_t t, int64_t left, u32x4 (&v)[4]) const {
     const rsrc_t r = make_rsrc(base + t * step, kBuffer);
+    if (whole || (!OUTER && left >= STEP)) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (vec) {
-        v[i] = bload16(r, off[i] | (first_k[i] < left ? 0 : kNowhere));
-      } else {
+      for (int i = 0; i < 4; ++i) v[i] = bload16(r, off[i] | (first_k[i] < left ? 0 : kNowhere));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const bool in = OUTER ? e < limit && first_k[i] < left : first_k[i] + e < left;
           v[i][e] = __builtin_amdgcn_raw_buffer_load_b32(r, (int)((off[i] + 4 * e) | (in ? 0 : kNowhere)), 0, 0);
         }
-      }
     }
   }
 
@@ -127,8 +129,8 @@ __global__ void __launch_bounds__(256, 2) product_f32_kernel(ProductArgs g) {
   const int wm = w / 2 * 64, wn = w % 2 * 64;
   Operand<OA> a;
   Operand<OB> b;
-  a.init(g.a, g.a_stride, k.i0, g.e.m, g.k, g.a_vec, wm, lane);
-  b.init(g.b, g.b_stride, k.j0, g.e.n, g.k, g.b_vec, wn, lane);
+  a.init(g.a, g.a_stride, k.i0, g.e.m, g.k, wm, lane);
+  b.init(g.b, g.b_stride, k.j0, g.e.n, g.k, wn, lane);
   f32x16 acc[2][2];
 #pragma unroll
   for (int m = 0; m < 2; ++m)
@@ -171,9 +173,9 @@ __global__ void __launch_bounds__(256, 2) product_f32_kernel(ProductArgs g) {
   write_tile<TILE, 2, OB, 1, false>(g, k, acc, (strip_ptr)(sa + w * kStripBytes), wm, wn, lane, MendParts<OA, OB>{g});
 }
 
-template <bool OA, bool OB>
+template <bool OA, bool OB, int N>
 __global__ void __launch_bounds__(256) join_f32_kernel(ProductArgs g) {
-  join<OB>(g, MendParts<OA, OB>{g});
+  join<OB, N>(g, MendParts<OA, OB>{g});
 }
 
 template <bool OA, bool OB>
@@ -181,7 +183,10 @@ hipError_t launch(const ProductArgs& g, hipStream_t stream) {
   const int64_t tiles = ((g.e.m + TILE - 1) / TILE) * ((g.e.n + TILE - 1) / TILE);
   hipLaunchKernelGGL((product_f32_kernel<OA, OB>), dim3((unsigned)(tiles * g.splits)), dim3(256), 0, stream, g);
   if (hipError_t e = hipGetLastError(); e != hipSuccess || !g.part) return e;
-  hipLaunchKernelGGL((join_f32_kernel<OA, OB>), join_grid(g), dim3(256), 0, stream, g);
+  if (g.e.vec)
+    hipLaunchKernelGGL((join_f32_kernel<OA, OB, 8>), join_grid(g), dim3(256), 0, stream, g);
+  else
+    hipLaunchKernelGGL((join_f32_kernel<OA, OB, 1>), join_grid(g), dim3(256), 0, stream, g);
   return hipGetLastError();
 }
 

@@ -36,29 +36,31 @@ __global__ void __launch_bounds__(256) layout_kernel(LayoutArgs a) {
   *(u32x4*)dst = u32x4{d[0], d[1], d[2], d[3]};
 }
 
-// 256 columns by `chunk` rows a workgroup, eight columns of every eighth row a thread.
-template <int KIND>
+// 256 columns by `chunk` rows a workgroup, eight columns of every eighth row a thread: side by side where rows are whole
+// aligned eights (VEC), else 32 apart, so that a wave's accesses lie side by side.
+template <int KIND, bool VEC>
 __global__ void __launch_bounds__(256) slope_kernel(SlopeArgs a) {
   __shared__ float red[8][256];
   const int across = (a.outs + 255) / 256, block = (int)blockIdx.x / across;
-  const int lane = (int)threadIdx.x & 31, own = (int)threadIdx.x >> 5;
-  const int col = ((int)blockIdx.x - block * across) * 256 + 8 * lane;
+  const int lane = (int)threadIdx.x & 31, own = (int)threadIdx.x >> 5, c0 = ((int)blockIdx.x - block * across) * 256;
+  const auto column = [&](int k) { return c0 + (VEC ? 8 * lane + k : lane + 32 * k); };
   const int64_t r0 = (int64_t)block * a.chunk, r1 = r0 + a.chunk < a.rows ? r0 + a.chunk : a.rows;
-  const bool vec = a.outs % 8 == 0 && (((uintptr_t)a.g | (uintptr_t)a.pre) & 15) == 0;
+  const int padded = (a.outs + 7) / 8 * 8;
   float sum[8] = {};
-  if (col < a.outs) {
+  if (!VEC || column(0) < a.outs) {
+#pragma unroll 2
     for (int64_t r = r0 + own; r < r1; r += 8) {
-      const int64_t at = r * a.outs + col;
+      const int64_t at = r * a.outs;
       float dz[8], z[8];
-      if (vec) {
-        load8(a.g, at, a.dtype, dz);
-        if (KIND != FWN_ACT_NONE) load8(a.pre, at, a.dtype, z);
+      if constexpr (VEC) {
+        load8(a.g, at + column(0), a.dtype, dz);
+        if (KIND != FWN_ACT_NONE) load8(a.pre, at + column(0), a.dtype, z);
       } else {
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          const bool in = col + k < a.outs;
-          dz[k] = in ? load_one(a.g, at + k, a.dtype) : 0.f;
-          z[k] = in && KIND != FWN_ACT_NONE ? load_one(a.pre, at + k, a.dtype) : 0.f;
+          const bool in = column(k) < a.outs;
+          dz[k] = in ? load_one(a.g, at + column(k), a.dtype) : 0.f;
+          z[k] = in && KIND != FWN_ACT_NONE ? load_one(a.pre, at + column(k), a.dtype) : 0.f;
         }
       }
 #pragma unroll
@@ -66,19 +68,28 @@ __global__ void __launch_bounds__(256) slope_kernel(SlopeArgs a) {
         if constexpr (KIND != FWN_ACT_NONE) dz[k] *= slope<KIND>(z[k]);
         sum[k] += dz[k];
       }
-      if (a.dz) store8(a.dz + r * a.dz_stride, col, a.dtype, dz);
+      if (a.dz) {
+        char* const row = a.dz + r * a.dz_stride;
+        if constexpr (VEC) {
+          store8(row, column(0), a.dtype, dz);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            if (column(k) < padded) store_one(row, column(k), a.dtype, dz[k]);
+        }
+      }
     }
   }
   if (!a.part) return;
 #pragma unroll
-  for (int k = 0; k < 8; ++k) red[own][8 * lane + k] = sum[k];
+  for (int k = 0; k < 8; ++k) red[own][column(k) - c0] = sum[k];
   __syncthreads();
-  const int c = (int)threadIdx.x, to = col - 8 * lane + c;
-  if (to >= a.outs) return;
+  const int c = (int)threadIdx.x;
+  if (c0 + c >= a.outs) return;
   float s = red[0][c];
 #pragma unroll
   for (int k = 1; k < 8; ++k) s += red[k][c];
-  a.part[(int64_t)block * a.outs + to] = s;
+  a.part[(int64_t)block * a.outs + c0 + c] = s;
 }
 
 constexpr int kGroups = 16;  // shares of the partial rows that a workgroup adds in parallel
@@ -111,17 +122,22 @@ hipError_t launch_layout(const LayoutArgs& a, hipStream_t stream) {
   return hipGetLastError();
 }
 
-hipError_t launch_slope(const SlopeArgs& a, hipStream_t stream) {
-  const unsigned across = (unsigned)(a.outs + 255) / 256;
-  const dim3 grid(across * (unsigned)a.blocks), block(256);
+template <bool VEC>
+static hipError_t launch_slope_as(const SlopeArgs& a, hipStream_t stream) {
+  const dim3 grid((unsigned)((a.outs + 255) / 256) * (unsigned)a.blocks), block(256);
   switch (a.activation) {
-    case FWN_ACT_RELU: hipLaunchKernelGGL(slope_kernel<FWN_ACT_RELU>, grid, block, 0, stream, a); break;
-    case FWN_ACT_GELU: hipLaunchKernelGGL(slope_kernel<FWN_ACT_GELU>, grid, block, 0, stream, a); break;
-    case FWN_ACT_GELU_TANH: hipLaunchKernelGGL(slope_kernel<FWN_ACT_GELU_TANH>, grid, block, 0, stream, a); break;
-    case FWN_ACT_SILU: hipLaunchKernelGGL(slope_kernel<FWN_ACT_SILU>, grid, block, 0, stream, a); break;
-    default: hipLaunchKernelGGL(slope_kernel<FWN_ACT_NONE>, grid, block, 0, stream, a);
+    case FWN_ACT_RELU: hipLaunchKernelGGL((slope_kernel<FWN_ACT_RELU, VEC>), grid, block, 0, stream, a); break;
+    case FWN_ACT_GELU: hipLaunchKernelGGL((slope_kernel<FWN_ACT_GELU, VEC>), grid, block, 0, stream, a); break;
+    case FWN_ACT_GELU_TANH: hipLaunchKernelGGL((slope_kernel<FWN_ACT_GELU_TANH, VEC>), grid, block, 0, stream, a); break;
+    case FWN_ACT_SILU: hipLaunchKernelGGL((slope_kernel<FWN_ACT_SILU, VEC>), grid, block, 0, stream, a); break;
+    default: hipLaunchKernelGGL((slope_kernel<FWN_ACT_NONE, VEC>), grid, block, 0, stream, a);
   }
   return hipGetLastError();
+}
+
+hipError_t launch_slope(const SlopeArgs& a, hipStream_t stream) {
+  const bool vec = a.outs % 8 == 0 && (((uintptr_t)a.g | (uintptr_t)a.pre) & 15) == 0;
+  return vec ? launch_slope_as<true>(a, stream) : launch_slope_as<false>(a, stream);
 }
 
 hipError_t launch_column_sums(const float* part, int64_t count, int64_t n, void* out, int dtype, hipStream_t stream) {

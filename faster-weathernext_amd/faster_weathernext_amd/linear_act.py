@@ -31,6 +31,14 @@ def _check(x, weight, bias, residual, dtype, lead):
       raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
 
 
+def _residual(t):
+  """(t's rows, their stride) as the kernels read a residual: at most LINEAR_ACT_MAX elements apart."""
+  if t is None:
+    return None, 0
+  rows, stride = rows_of(t)
+  return (rows, stride) if stride <= nat.LINEAR_ACT_MAX else (rows.contiguous(), rows.shape[-1])
+
+
 def _activation(name):
   if name not in nat.ACTIVATIONS:
     raise ValueError(f"unknown activation {name!r} ({', '.join(str(a) for a in nat.ACTIVATIONS)})")
@@ -48,7 +56,7 @@ def _forward(x, weight, bias, residual, activation, keep):
   lead, (outs, ins) = x.shape[:-1], weight.shape
   xr, xs = rows_of(x)
   wr, ws = rows_of(weight)
-  rr, rs = rows_of(residual) if residual is not None else (None, 0)
+  rr, rs = _residual(residual)
   bias = bias.contiguous() if bias is not None else None
   L = nat.lib()
   out = torch.empty((*lead, outs), dtype=x.dtype, device=x.device)
@@ -171,7 +179,7 @@ def linear_act_q8(x, x_scale, weight, weight_scale, bias=None, *, activation=Non
   outs, ins = weight.shape
   xr, xs = rows_of(x)
   wr, ws = rows_of(weight)
-  rr, rs = rows_of(residual) if residual is not None else (None, 0)
+  rr, rs = _residual(residual)
   bias = bias.contiguous() if bias is not None else None
   x_scale, weight_scale = x_scale.contiguous(), weight_scale.contiguous()
   L = nat.lib()

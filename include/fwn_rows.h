@@ -164,7 +164,8 @@ int fwn_rms_norm_bwd_launch(const fwn_rms_desc* d, const void* s, const void* we
 /* Matrix product with bias, activation and residual in its epilogue:
  *   z = x weight^T + bias,  out = act(z) + residual
  * x is [rows, ins], weight [outs, ins], residual [rows, outs], with contiguous rows x_stride, w_stride and
- * r_stride elements apart (0: one row for all); bias [outs], out and pre [rows, outs] are contiguous.
+ * r_stride elements apart (0: one row for all; r_stride at most FWN_LINEAR_ACT_MAX); bias [outs], out and pre
+ * [rows, outs] are contiguous.
  * Products accumulate in float32; out, and pre (z for the backward, NULL: not stored) are rounded
  * once. bias and residual may be NULL. Every tensor is of `dtype`; float32 products keep float32's precision. */
 #define FWN_ACT_NONE 0
