@@ -132,7 +132,7 @@ struct Cost {
 };
 
 Plan plan(int64_t m, int64_t n, int64_t k, int32_t op) {
-  constexpr Cost bf16[] = {{256, 1.55, 1.55, 6.0}, {128, 0.6, 0.5, 2.2}}, f32[] = {{128, 1.3, 0.95, 2.5}};
+  constexpr Cost bf16[] = {{256, 1.55, 1.55, 6.0}, {128, 0.6, 0.5, 2.2}}, f32[] = {{128, 2.0, 1.1, 3.0}};
   const int64_t of = op == kOpF32 ? kStageF32 : op == kOpE4m3 ? kStageBytes : kStageRows;
   const int64_t stages = std::max<int64_t>(1, parts(k, of));
   Plan best{128, 1, (int32_t)stages};

@@ -6,8 +6,11 @@
 // LDS, so an operand of any strides and alignment is read where it lies, once a tile.
 //
 // A workgroup is 4 waves on a 128 x 128 tile, a wave 64 x 64: per 16 k it reads 12 KB of LDS for 24 MFMAs. One
-// stage of 32 k is 48 KB of parts, so that three workgroups share a CU: while one splits and writes its next stage,
-// loaded a stage ahead into registers, the others multiply.
+// stage of 32 k is 48 KB of parts, so that two or three workgroups share a CU: while one splits and writes its next
+// stage, loaded a stage ahead into registers, the others multiply. A stage takes 2.0 us alone on a CU and 1.1 among
+// others. 8 waves with two stages in LDS, a wave splitting the next between its products, were quicker where
+// tiles are few (2,562 x 515 -> 1027: 34 us against 42), but slower where they fill the chip (10,242 x 768 -> 3072:
+// 348 against 290), for the two waves of a SIMD then split at the same time.
 #include "linear_act_device.h"
 
 namespace fwn {
@@ -117,7 +120,7 @@ struct Operand {
 };
 
 template <bool OA, bool OB>
-__global__ void __launch_bounds__(256, 2) product_f32_kernel(ProductArgs g) {
+__global__ void __launch_bounds__(256, OA || OB ? 2 : 3) product_f32_kernel(ProductArgs g) {
   __shared__ __align__(256) char lds[2 * OPERAND];
   static_assert(sizeof(lds) >= 4 * kStripBytes, "the waves' strips");
   lds_char* const sa = (lds_char*)lds;
