@@ -24,7 +24,7 @@ ARCH = "gfx950"
 
 DEVICE_SOURCES = ["attn_bf16.hip", "attn_x3.hip", "attn_x3_dkv.hip", "attn_f32.hip", "attn_combine.hip",
                   "attn_noalloc.hip", "rows.hip", "linear.hip", "linear_act.hip",
-                  "linear_act_f32.hip", "linear_act_passes.hip", "rms.hip"]
+                  "linear_act_f32.hip", "linear_act_passes.hip", "linear_act_rows.hip", "rms.hip"]
 HOST_SOURCES = ["attn_api.cpp", "mask_host.cpp", "node_order.cpp", "rows_api.cpp", "linear_api.cpp",
                 "linear_act_api.cpp", "rms_api.cpp"]
 

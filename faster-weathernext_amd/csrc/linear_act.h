@@ -51,6 +51,9 @@ enum class Operands { kInnerInner, kInnerOuter, kOuterOuter };  // how a and b l
 // One product, by tiles of 256 x 256 or 128 x 128 (float32: the latter). Of e4m3 operands kInnerInner alone.
 hipError_t launch_product(Operands how, int32_t op, int tile, const ProductArgs& a, hipStream_t stream);
 hipError_t launch_product_f32(Operands how, const ProductArgs& a, hipStream_t stream);
+// One product of inner operands with at most kFewRows rows of a, unsplit.
+hipError_t launch_product_rows(int32_t op, const ProductArgs& a, hipStream_t stream);
+constexpr int64_t kFewRows = 32;
 
 // A matrix copied to rows padded with zeros to 16 bytes.
 struct LayoutArgs {

@@ -162,11 +162,13 @@ struct Product {
   Operands how;
   int32_t op;
   Plan p;
+  bool few;  // rows: no tiles
 
   // `sums`: the column sums of a are wanted.
   void shape(Operands h, int64_t m, int64_t n, int64_t k, int32_t o, bool sums, Workspace& ws) {
     how = h, op = o;
-    p = plan(m, n, k, op);
+    few = how == Operands::kInnerInner && m <= kFewRows;
+    p = few ? Plan{0, 1, 0} : plan(m, n, k, op);
     g.k = k;
     g.splits = p.splits;
     g.chunk = p.chunk;
@@ -183,7 +185,7 @@ struct Product {
     const EpilogueArgs& e = g.e;
     g.e.vec = e.n % 8 == 0 && (!e.residual || e.r_row % 8 == 0) &&
               (((uintptr_t)e.out | (uintptr_t)e.pre | (uintptr_t)e.residual) & 15) == 0;
-    return launch_product(how, op, p.tile, g, stream);
+    return few ? launch_product_rows(op, g, stream) : launch_product(how, op, p.tile, g, stream);
   }
 };
 
