@@ -13,22 +13,27 @@ import ctypes
 import torch
 
 from . import _native as nat
-from .rms import _Q8, _needs, _no_grad, launch, rows_of
+from .rms import _Q8, _needs, _no_grad, dense, launch, rows_of
 from .rows import _DTYPES, _addr, as_torch
 
 
 def _check(x, weight, bias, residual, dtype, lead):
   if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
     raise ValueError(f"weight must be [outs, ins] and x [..., ins], got {tuple(weight.shape)} and {tuple(x.shape)}")
-  if not all(1 <= s <= nat.LINEAR_ACT_MAX for s in weight.shape):
+  outs, ins = weight.shape
+  if not (1 <= outs <= nat.LINEAR_ACT_MAX and 1 <= ins <= nat.LINEAR_ACT_MAX):
     raise ValueError(f"weight's sizes must be 1 to {nat.LINEAR_ACT_MAX}, got {tuple(weight.shape)}")
-  for t, name, shape in ((bias, "bias", weight.shape[:1]), (residual, "residual", (*lead, weight.shape[0]))):
-    if t is None:
-      continue
-    if not isinstance(t, torch.Tensor) or t.device != x.device or t.shape != shape:
-      raise ValueError(f"{name} must be a tensor of shape {tuple(shape)} on the device of x")
-    if t.dtype != dtype:
-      raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+  if bias is not None:
+    _check_like(bias, "bias", (outs,), dtype, x)
+  if residual is not None:
+    _check_like(residual, "residual", (*lead, outs), dtype, x)
+
+
+def _check_like(t, name, shape, dtype, x):
+  if not isinstance(t, torch.Tensor) or t.get_device() != x.get_device() or t.shape != shape:
+    raise ValueError(f"{name} must be a tensor of shape {tuple(shape)} on the device of x")
+  if t.dtype != dtype:
+    raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
 
 
 def _residual(t):
@@ -45,10 +50,10 @@ def _activation(name):
   return nat.ACTIVATIONS[name]
 
 
-def _workspace(query, d, device, *tensors):
-  size = ctypes.c_uint64(0)
-  nat.check(query(d, *(_addr(t) for t in tensors), ctypes.byref(size)))
-  return (torch.empty(size.value, dtype=torch.uint8, device=device) if size.value else None), size.value
+def _workspace(query, d, like, *addresses):
+  size = ctypes.c_uint64()
+  nat.check(query(d, *addresses, ctypes.byref(size)))
+  return (torch.empty(size.value, dtype=torch.uint8, device=like.device) if size.value else None), size.value
 
 
 def _forward(x, weight, bias, residual, activation, keep):
@@ -57,14 +62,14 @@ def _forward(x, weight, bias, residual, activation, keep):
   xr, xs = rows_of(x)
   wr, ws = rows_of(weight)
   rr, rs = _residual(residual)
-  bias = bias.contiguous() if bias is not None else None
+  bias = dense(bias)
   L = nat.lib()
-  out = torch.empty((*lead, outs), dtype=x.dtype, device=x.device)
+  out = x.new_empty((*lead, outs))
   pre = torch.empty_like(out) if keep else None
   d = nat.LinearDesc(x.numel() // ins, xs, ws, rs, ins, outs, _DTYPES[x.dtype], activation)
-  work, size = _workspace(L.fwn_linear_act_workspace_size, d, x.device, xr, wr)
-  launch(x, L.fwn_linear_act_launch, d, _addr(xr), _addr(wr), _addr(bias), _addr(rr), _addr(out), _addr(pre), _addr(work),
-         size)
+  xa, wa = _addr(xr), _addr(wr)
+  work, size = _workspace(L.fwn_linear_act_workspace_size, d, x, xa, wa)
+  launch(x, L.fwn_linear_act_launch, d, xa, wa, _addr(bias), _addr(rr), _addr(out), _addr(pre), _addr(work), size)
   return out, pre
 
 
@@ -126,9 +131,9 @@ class _LinearAct(torch.autograd.Function):
     L = nat.lib()
     gx, gw, gb = (torch.empty(shape, dtype=g.dtype, device=g.device) if need else None
                   for shape, need in zip((x_shape, w_shape, (outs,)), needs))
-    work, size = _workspace(L.fwn_linear_act_bwd_workspace_size, d, g.device, xr, wr, g, gx, gw, gb)
-    launch(g, L.fwn_linear_act_bwd_launch, d, _addr(xr), _addr(wr), _addr(pre), _addr(g), _addr(gx), _addr(gw), _addr(gb),
-           _addr(work), size)
+    xa, wa, ga, gxa, gwa, gba = (_addr(t) for t in (xr, wr, g, gx, gw, gb))
+    work, size = _workspace(L.fwn_linear_act_bwd_workspace_size, d, g, xa, wa, ga, gxa, gwa, gba)
+    launch(g, L.fwn_linear_act_bwd_launch, d, xa, wa, _addr(pre), ga, gxa, gwa, gba, _addr(work), size)
     return gx, gw, gb, g_res, None
 
 
@@ -142,7 +147,7 @@ def linear_act(x, weight, bias=None, *, activation=None, residual=None):
     raise ValueError("x must be a CUDA tensor")
   if x.dtype not in _DTYPES:
     raise TypeError(f"x must be float32 or bfloat16, got {x.dtype}")
-  if not isinstance(weight, torch.Tensor) or weight.device != x.device:
+  if not isinstance(weight, torch.Tensor) or weight.get_device() != x.get_device():
     raise ValueError("weight must be a tensor on the device of x")
   if weight.dtype != x.dtype:
     raise TypeError(f"weight must be {x.dtype}, got {weight.dtype}")
@@ -161,7 +166,7 @@ def linear_act_q8(x, x_scale, weight, weight_scale, bias=None, *, activation=Non
   residual in `dtype`, which bias and residual have. Forward only."""
   if not isinstance(x, torch.Tensor) or not x.is_cuda:
     raise ValueError("x must be a CUDA tensor")
-  if not isinstance(weight, torch.Tensor) or weight.device != x.device:
+  if not isinstance(weight, torch.Tensor) or weight.get_device() != x.get_device():
     raise ValueError("weight must be a tensor on the device of x")
   if x.dtype != _Q8 or weight.dtype != _Q8:
     raise TypeError(f"x and weight must be {_Q8}, got {x.dtype} and {weight.dtype}")
@@ -170,22 +175,20 @@ def linear_act_q8(x, x_scale, weight, weight_scale, bias=None, *, activation=Non
   act = _activation(activation)
   lead = x.shape[:-1]
   _check(x, weight, bias, residual, dtype, lead)
-  for t, name, shape in ((x_scale, "x_scale", lead), (weight_scale, "weight_scale", weight.shape[:1])):
-    if not isinstance(t, torch.Tensor) or t.device != x.device or t.shape != shape:
-      raise ValueError(f"{name} must be a tensor of shape {tuple(shape)} on the device of x")
-    if t.dtype != torch.float32:
-      raise TypeError(f"{name} must be float32, got {t.dtype}")
+  _check_like(x_scale, "x_scale", lead, torch.float32, x)
+  _check_like(weight_scale, "weight_scale", weight.shape[:1], torch.float32, x)
   _no_grad("linear_act_q8", x_scale, weight_scale, bias, residual)
   outs, ins = weight.shape
   xr, xs = rows_of(x)
   wr, ws = rows_of(weight)
   rr, rs = _residual(residual)
-  bias = bias.contiguous() if bias is not None else None
-  x_scale, weight_scale = x_scale.contiguous(), weight_scale.contiguous()
+  bias = dense(bias)
+  x_scale, weight_scale = dense(x_scale), dense(weight_scale)
   L = nat.lib()
   out = torch.empty((*lead, outs), dtype=dtype, device=x.device)
   d = nat.LinearDesc(x.numel() // ins, xs, ws, rs, ins, outs, _DTYPES[dtype], act)
-  work, size = _workspace(L.fwn_linear_act_q8_workspace_size, d, x.device, xr, wr)
-  launch(x, L.fwn_linear_act_q8_launch, d, _addr(xr), _addr(x_scale), _addr(wr), _addr(weight_scale), _addr(bias), _addr(rr),
-         _addr(out), _addr(work), size)
+  xa, wa = _addr(xr), _addr(wr)
+  work, size = _workspace(L.fwn_linear_act_q8_workspace_size, d, x, xa, wa)
+  launch(x, L.fwn_linear_act_q8_launch, d, xa, _addr(x_scale), wa, _addr(weight_scale), _addr(bias), _addr(rr), _addr(out),
+         _addr(work), size)
   return out

@@ -33,14 +33,20 @@ def launch(t, fn, *args):
     nat.check(fn(*args, torch._C._cuda_getCurrentRawStream(device)))
 
 
+def dense(t):
+  return t if t is None or t.is_contiguous() else t.contiguous()
+
+
 def new_like(t):
   """A contiguous tensor of t's shape, dtype and device."""
   return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
 def rows_of(t):
-  """(t as [rows, channels] without a copy where its strides allow it, the rows' stride)."""
+  """(t, or its rows [rows, channels] without a copy where its strides allow it; the rows' stride)."""
   c = t.shape[-1]
+  if t.is_contiguous():
+    return t, c
   if t.numel() == 0:
     return t.reshape(-1, c) if c else t.reshape(0, 0), c
   if t.dim() == 2 and t.stride(1) == 1:
@@ -60,7 +66,7 @@ def _check(x, name, like=None):
   if not isinstance(x, torch.Tensor) or not x.is_cuda:
     raise ValueError(f"{name} must be a CUDA tensor")
   if like is not None:
-    if x.shape != like.shape or x.dtype != like.dtype or x.device != like.device:
+    if x.shape != like.shape or x.dtype != like.dtype or x.get_device() != like.get_device():
       raise ValueError(f"{name} must be a tensor of x's shape, dtype and device")
     return
   if x.dim() < 1 or not 1 <= x.shape[-1] <= nat.RMS_MAX_CHANNELS:
@@ -73,30 +79,30 @@ def _check(x, name, like=None):
 def _check_weight(weight, x):
   if weight is None:
     return
-  if not isinstance(weight, torch.Tensor) or weight.device != x.device or weight.shape != x.shape[-1:]:
+  if not isinstance(weight, torch.Tensor) or weight.get_device() != x.get_device() or weight.shape != x.shape[-1:]:
     raise ValueError(f"weight must be a tensor of shape {tuple(x.shape[-1:])} on the device of x")
   if weight.dtype not in (x.dtype, torch.float32):
     raise TypeError(f"weight must be {x.dtype} or float32, got {weight.dtype}")
 
 
 def _desc(x, weight, eps, x_stride, y_stride=0):
-  return nat.RmsDesc(x.numel() // x.shape[-1], x_stride, y_stride, x.shape[-1], _DTYPES[x.dtype],
-                     _DTYPES[x.dtype if weight is None else weight.dtype], float(eps))
+  c, dtype = x.shape[-1], _DTYPES[x.dtype]
+  return nat.RmsDesc(x.numel() // c, x_stride, y_stride, c, dtype, dtype if weight is None else _DTYPES[weight.dtype], eps)
 
 
 def _forward(x, y, weight, eps, q8):
   """(sum or None, out) or, with q8, (sum or None, q, scale): one HIP pass (no autograd)."""
   xr, xs = rows_of(x)
   yr, ys = rows_of(y) if y is not None else (None, 0)
-  weight = weight.contiguous() if weight is not None else None
+  weight = dense(weight)
   d = _desc(x, weight, eps, xs, ys)
   s = None if y is None else new_like(x)
   if not q8:
     out = new_like(x)
     launch(x, nat.lib().fwn_rms_norm_launch, d, _addr(xr), _addr(yr), _addr(weight), _addr(s), _addr(out))
     return s, out
-  q = torch.empty(x.shape, dtype=_Q8, device=x.device)
-  scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+  q = x.new_empty(x.shape, dtype=_Q8)
+  scale = x.new_empty(x.shape[:-1], dtype=torch.float32)
   launch(x, nat.lib().fwn_rms_norm_q8_launch, d, _addr(xr), _addr(yr), _addr(weight), _addr(s), _addr(q), _addr(scale))
   return s, q, scale
 
@@ -139,7 +145,7 @@ class _RmsNorm(torch.autograd.Function):
 
   @staticmethod
   def forward(ctx, x, y, weight, eps):
-    weight = weight.contiguous() if weight is not None else None
+    weight = dense(weight)
     if y is None:
       s = x.contiguous()
       _, out = _forward(s, None, weight, eps, False)
@@ -171,7 +177,11 @@ def _no_grad(name, *tensors):
 
 
 def _needs(*tensors):
-  return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+  if torch.is_grad_enabled():
+    for t in tensors:
+      if t is not None and t.requires_grad:
+        return True
+  return False
 
 
 def rms_norm(x, weight=None, *, eps=1e-6):
@@ -222,7 +232,7 @@ def quantize_rows(x):
   _no_grad("quantize_rows", x)
   xr, xs = rows_of(x)
   d = _desc(x, None, 0.0, xs)
-  q = torch.empty(x.shape, dtype=_Q8, device=x.device)
-  scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+  q = x.new_empty(x.shape, dtype=_Q8)
+  scale = x.new_empty(x.shape[:-1], dtype=torch.float32)
   launch(x, nat.lib().fwn_quantize_rows_launch, d, _addr(xr), _addr(q), _addr(scale))
   return q, scale
