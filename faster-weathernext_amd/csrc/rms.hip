@@ -7,7 +7,8 @@
 //
 // Streaming passes bound by HBM: a row is held in registers from its only load to its outputs, so each
 // byte moves once, and the backward recomputes r from s rather than reading it. TPR threads share a row,
-// each with VPT vectors of E elements (16 bytes; E = 1 for rows that are not whole aligned vectors).
+// each with VPT vectors of E elements (16 bytes). Vectors need no alignment but their elements' (the compiler makes
+// one 16-byte access of them all the same); where a row ends inside a vector (TAIL) that one goes by elements.
 #include "rms_kernels.h"
 
 #include "fwn_attn.h"
@@ -17,6 +18,19 @@ namespace {
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+// The same at any address of a row.
+typedef uint32_t f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t bf16x8_any __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t u8x4_any __attribute__((ext_vector_type(1), aligned(1)));
+typedef uint32_t u8x8_any __attribute__((ext_vector_type(2), aligned(1)));
+template <typename T>
+struct Any {
+  typedef bf16x8_any type;
+};
+template <>
+struct Any<float> {
+  typedef f32x4_any type;
+};
 
 constexpr int64_t kMostBlocks = 1 << 20;           // of a forward launch; more rows are looped over
 constexpr uint64_t kStreamBytes = 256ull << 20;  // bytes written from which stores are non-temporal (rows.hip)
@@ -25,59 +39,69 @@ __device__ __forceinline__ float as_float(uint32_t u) { return __builtin_bit_cas
 __device__ __forceinline__ uint32_t as_bits(float f) { return __builtin_bit_cast(uint32_t, f); }
 __device__ __forceinline__ uint32_t bf16_bits(float f) { return __builtin_bit_cast(uint16_t, (__bf16)f); }
 
-// E elements of T (float, or uint16_t: bfloat16 bits) at p as floats.
-template <typename T, int E, bool NT>
-__device__ __forceinline__ void load(const T* p, float (&f)[E]) {
-  if constexpr (E == 1) {
-    const T v = NT ? __builtin_nontemporal_load(p) : *p;
-    if constexpr (sizeof(T) == 4) {
-      f[0] = v;
-    } else {
-      f[0] = as_float((uint32_t)v << 16);
-    }
+template <typename T>
+__device__ __forceinline__ float load_one(const T* p) {
+  if constexpr (sizeof(T) == 4) {
+    return *p;
   } else {
-    const u32x4 v = NT ? __builtin_nontemporal_load((const u32x4*)p) : *(const u32x4*)p;
+    return as_float((uint32_t)*p << 16);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void store_one(T* p, float v) {
+  if constexpr (sizeof(T) == 4) {
+    *p = v;
+  } else {
+    *p = (T)bf16_bits(v);
+  }
+}
+
+// The E elements of T (float, or uint16_t: bfloat16 bits) at p as floats; with TAIL those of the first `left`, and
+// zeros.
+template <typename T, int E, bool NT, bool TAIL>
+__device__ __forceinline__ void load(const T* p, int left, float (&f)[E]) {
+  if (TAIL && left < E) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const uint32_t u = v[k];
-      if constexpr (sizeof(T) == 4) {
-        f[k] = as_float(u);
-      } else {
-        f[2 * k] = as_float(u << 16);
-        f[2 * k + 1] = as_float(u & 0xffff0000u);
-      }
+    for (int e = 0; e < E; ++e) f[e] = e < left ? load_one(p + e) : 0.f;
+    return;
+  }
+  typedef typename Any<T>::type vec;
+  const u32x4 v = NT ? __builtin_nontemporal_load((const vec*)p) : *(const vec*)p;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const uint32_t u = v[k];
+    if constexpr (sizeof(T) == 4) {
+      f[k] = as_float(u);
+    } else {
+      f[2 * k] = as_float(u << 16);
+      f[2 * k + 1] = as_float(u & 0xffff0000u);
     }
   }
 }
 
-template <typename T, int E, bool NT>
-__device__ __forceinline__ void store(T* p, const float (&f)[E]) {
-  if constexpr (E == 1) {
-    T v;
-    if constexpr (sizeof(T) == 4) {
-      v = f[0];
-    } else {
-      v = (T)bf16_bits(f[0]);
-    }
-    if constexpr (NT)
-      __builtin_nontemporal_store(v, p);
-    else
-      *p = v;
-  } else {
-    u32x4 v;
+template <typename T, int E, bool NT, bool TAIL>
+__device__ __forceinline__ void store(T* p, int left, const float (&f)[E]) {
+  if (TAIL && left < E) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      if constexpr (sizeof(T) == 4) {
-        v[k] = as_bits(f[k]);
-      } else {
-        v[k] = bf16_bits(f[2 * k]) | bf16_bits(f[2 * k + 1]) << 16;
-      }
-    }
-    if constexpr (NT)
-      __builtin_nontemporal_store(v, (u32x4*)p);
-    else
-      *(u32x4*)p = v;
+    for (int e = 0; e < E; ++e)
+      if (e < left) store_one(p + e, f[e]);
+    return;
   }
+  typedef typename Any<T>::type vec;
+  vec v;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    if constexpr (sizeof(T) == 4) {
+      v[k] = as_bits(f[k]);
+    } else {
+      v[k] = bf16_bits(f[2 * k]) | bf16_bits(f[2 * k + 1]) << 16;
+    }
+  }
+  if constexpr (NT)
+    __builtin_nontemporal_store(v, (vec*)p);
+  else
+    *(vec*)p = v;
 }
 
 // The values as their dtype holds them.
@@ -90,16 +114,17 @@ __device__ __forceinline__ void round_to(float (&f)[E]) {
 }
 
 // E weights from channel c, of T or of float.
-template <typename T, int E>
-__device__ __forceinline__ void load_weight(const void* w, bool f32, int64_t c, float (&f)[E]) {
+template <typename T, int E, bool TAIL>
+__device__ __forceinline__ void load_weight(const void* w, bool f32, int64_t c, int left, float (&f)[E]) {
   if (sizeof(T) == 4 || !f32) {
-    load<T, E, false>((const T*)w + c, f);
-  } else if constexpr (E == 1) {
-    f[0] = ((const float*)w)[c];
+    load<T, E, false, TAIL>((const T*)w + c, left, f);
+  } else if (TAIL && left < E) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) f[e] = e < left ? ((const float*)w)[c + e] : 0.f;
   } else {
 #pragma unroll
     for (int h = 0; h < E; h += 4) {
-      const u32x4 v = *(const u32x4*)((const float*)w + c + h);
+      const u32x4 v = *(const f32x4_any*)((const float*)w + c + h);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const uint32_t u = v[k];
@@ -149,30 +174,32 @@ __device__ __forceinline__ uint32_t row_max(uint32_t v, float* red) {
 
 // E codes of f * inv at p. |f * inv| is at most 448 (1 + 2^-22), which rounds to 448: no clamp, which
 // would turn NaN into a number.
-template <int E>
-__device__ __forceinline__ void store_q8(uint8_t* p, const float (&f)[E], float inv) {
-  if constexpr (E == 1) {
-    *p = (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(f[0] * inv, 0.f, 0, false);
-  } else {
-    uint32_t d[E / 4];
+template <int E, bool TAIL>
+__device__ __forceinline__ void store_q8(uint8_t* p, int left, const float (&f)[E], float inv) {
+  if (TAIL && left < E) {
 #pragma unroll
-    for (int k = 0; k < E / 4; ++k) {
-      const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(f[4 * k] * inv, f[4 * k + 1] * inv, 0, false);
-      d[k] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(f[4 * k + 2] * inv, f[4 * k + 3] * inv, lo, true);
-    }
-    if constexpr (E == 8)
-      *(u32x2*)p = u32x2{d[0], d[1]};
-    else
-      *(uint32_t*)p = d[0];
+    for (int e = 0; e < E; ++e)
+      if (e < left) p[e] = (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(f[e] * inv, 0.f, 0, false);
+    return;
   }
+  uint32_t d[E / 4];
+#pragma unroll
+  for (int k = 0; k < E / 4; ++k) {
+    const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(f[4 * k] * inv, f[4 * k + 1] * inv, 0, false);
+    d[k] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(f[4 * k + 2] * inv, f[4 * k + 3] * inv, lo, true);
+  }
+  if constexpr (E == 8)
+    *(u8x8_any*)p = u8x8_any{d[0], d[1]};
+  else
+    *(u8x4_any*)p = u8x4_any{d[0]};
 }
 
 template <int TPR>
 constexpr int kThreads = TPR < 256 ? 256 : TPR;
 
-template <typename T, int E, int TPR, int VPT, bool Q8, bool NT>
+template <typename T, int TPR, int VPT, bool Q8, bool NT, bool TAIL>
 __global__ void __launch_bounds__(kThreads<TPR>) rms_kernel(RmsArgs a) {
-  constexpr int RPW = kThreads<TPR> / TPR;  // rows of a workgroup
+  constexpr int E = 16 / sizeof(T), RPW = kThreads<TPR> / TPR;  // rows of a workgroup
   __shared__ float red[16];
   const int t = (int)threadIdx.x % TPR;
   const float inv_c = 1.f / (float)a.channels;
@@ -186,7 +213,7 @@ __global__ void __launch_bounds__(kThreads<TPR>) rms_kernel(RmsArgs a) {
       const int c = (t + TPR * k) * E;
 #pragma unroll
       for (int e = 0; e < E; ++e) f[k][e] = 0.f;
-      if (ok && c < a.channels) load<T, E, true>(x + c, f[k]);
+      if (ok && c < a.channels) load<T, E, true, TAIL>(x + c, a.channels - c, f[k]);
     }
     if (a.y) {
       const T* y = (const T*)a.y + row * a.y_stride;
@@ -194,7 +221,7 @@ __global__ void __launch_bounds__(kThreads<TPR>) rms_kernel(RmsArgs a) {
 #pragma unroll
       for (int k = 0; k < VPT; ++k) {
         const int c = (t + TPR * k) * E;
-        if (ok && c < a.channels) load<T, E, true>(y + c, g[k]);
+        if (ok && c < a.channels) load<T, E, true, TAIL>(y + c, a.channels - c, g[k]);
       }
 #pragma unroll
       for (int k = 0; k < VPT; ++k) {
@@ -203,7 +230,7 @@ __global__ void __launch_bounds__(kThreads<TPR>) rms_kernel(RmsArgs a) {
 #pragma unroll
         for (int e = 0; e < E; ++e) f[k][e] += g[k][e];
         round_to<T>(f[k]);
-        store<T, E, NT>((T*)a.sum + row * a.channels + c, f[k]);
+        store<T, E, NT, TAIL>((T*)a.sum + row * a.channels + c, a.channels - c, f[k]);
       }
     }
     float r = 1.f;
@@ -211,7 +238,7 @@ __global__ void __launch_bounds__(kThreads<TPR>) rms_kernel(RmsArgs a) {
 #pragma unroll
       for (int k = 0; k < VPT; ++k) {
         const int c = (t + TPR * k) * E;
-        if (a.weight && c < a.channels) load_weight<T, E>(a.weight, a.weight_f32, c, w[k]);
+        if (a.weight && c < a.channels) load_weight<T, E, TAIL>(a.weight, a.weight_f32, c, a.channels - c, w[k]);
       }
       float sq = 0.f;
 #pragma unroll
@@ -243,7 +270,7 @@ __global__ void __launch_bounds__(kThreads<TPR>) rms_kernel(RmsArgs a) {
 #pragma unroll
       for (int k = 0; k < VPT; ++k) {
         const int c = (t + TPR * k) * E;
-        if (c < a.channels) store_q8<E>(a.q + row * a.channels + c, f[k], inv);
+        if (c < a.channels) store_q8<E, TAIL>(a.q + row * a.channels + c, a.channels - c, f[k], inv);
       }
       if (t == 0) a.scale[row] = scale;
     } else {
@@ -251,7 +278,7 @@ __global__ void __launch_bounds__(kThreads<TPR>) rms_kernel(RmsArgs a) {
 #pragma unroll
       for (int k = 0; k < VPT; ++k) {
         const int c = (t + TPR * k) * E;
-        if (c < a.channels) store<T, E, NT>((T*)a.out + row * a.channels + c, f[k]);
+        if (c < a.channels) store<T, E, NT, TAIL>((T*)a.out + row * a.channels + c, a.channels - c, f[k]);
       }
     }
   }
@@ -259,9 +286,9 @@ __global__ void __launch_bounds__(kThreads<TPR>) rms_kernel(RmsArgs a) {
 
 // gw's sums stay in each thread's registers over all rows of its workgroup, are added over the rows that
 // the workgroup holds at once and go out as one partial row a workgroup, in a fixed order.
-template <typename T, int E, int TPR, int VPT, bool NT>
+template <typename T, int TPR, int VPT, bool NT, bool TAIL>
 __global__ void __launch_bounds__(kThreads<TPR>) rms_bwd_kernel(RmsBwdArgs a) {
-  constexpr int RPW = kThreads<TPR> / TPR;
+  constexpr int E = 16 / sizeof(T), RPW = kThreads<TPR> / TPR;
   __shared__ float red[16];
   __shared__ float sums[RPW > 1 ? TPR * VPT * E : 1];
   const int t = (int)threadIdx.x % TPR, own = (int)threadIdx.x / TPR;
@@ -272,7 +299,7 @@ __global__ void __launch_bounds__(kThreads<TPR>) rms_bwd_kernel(RmsBwdArgs a) {
     const int c = (t + TPR * k) * E;
 #pragma unroll
     for (int e = 0; e < E; ++e) gw[k][e] = 0.f, w[k][e] = 1.f;
-    if (a.weight && c < a.channels) load_weight<T, E>(a.weight, a.weight_f32, c, w[k]);
+    if (a.weight && c < a.channels) load_weight<T, E, TAIL>(a.weight, a.weight_f32, c, a.channels - c, w[k]);
   }
   for (int64_t row0 = (int64_t)blockIdx.x * RPW; row0 < a.rows; row0 += (int64_t)gridDim.x * RPW) {
     const int64_t row = row0 + own;
@@ -285,9 +312,9 @@ __global__ void __launch_bounds__(kThreads<TPR>) rms_bwd_kernel(RmsBwdArgs a) {
 #pragma unroll
       for (int e = 0; e < E; ++e) f[k][e] = g[k][e] = gs[k][e] = 0.f;
       if (!ok || c >= a.channels) continue;
-      load<T, E, true>((const T*)a.s + at + c, f[k]);
-      load<T, E, true>((const T*)a.g_out + at + c, g[k]);
-      if (a.g_sum) load<T, E, true>((const T*)a.g_sum + at + c, gs[k]);
+      load<T, E, true, TAIL>((const T*)a.s + at + c, a.channels - c, f[k]);
+      load<T, E, true, TAIL>((const T*)a.g_out + at + c, a.channels - c, g[k]);
+      if (a.g_sum) load<T, E, true, TAIL>((const T*)a.g_sum + at + c, a.channels - c, gs[k]);
     }
     float sq = 0.f, hs = 0.f;
 #pragma unroll
@@ -310,7 +337,7 @@ __global__ void __launch_bounds__(kThreads<TPR>) rms_bwd_kernel(RmsBwdArgs a) {
         o[e] = fmaf(r, g[k][e] * w[k][e] - f[k][e] * c2, gs[k][e]);
         gw[k][e] = fmaf(g[k][e], f[k][e] * r, gw[k][e]);
       }
-      store<T, E, NT>((T*)a.gx + at + c, o);
+      store<T, E, NT, TAIL>((T*)a.gx + at + c, a.channels - c, o);
     }
   }
   if (!a.part) return;
@@ -375,16 +402,13 @@ hipError_t choose(int n, F&& f) {
   if (n <= 512) return f.template operator()<256, 2>();
   if (n <= 1024) return f.template operator()<256, 4>();
   if (n <= 2048) return f.template operator()<1024, 2>();
-  if constexpr (E <= 4) {
+  if constexpr (E == 4) {
     if (n <= 4096) return f.template operator()<1024, 4>();
-  }
-  if constexpr (E == 1) {
-    if (n <= 16384) return f.template operator()<1024, 16>();
   }
   return hipErrorInvalidValue;
 }
 
-template <typename T, int E>
+template <typename T, bool NT, bool TAIL>
 struct Forward {
   const RmsArgs& a;
   hipStream_t stream;
@@ -393,48 +417,41 @@ struct Forward {
     constexpr int RPW = kThreads<TPR> / TPR;
     const int64_t blocks = (a.rows + RPW - 1) / RPW;
     const dim3 grid((unsigned)(blocks < kMostBlocks ? blocks : kMostBlocks)), block(kThreads<TPR>);
-    if (a.q && a.stream)
-      hipLaunchKernelGGL((rms_kernel<T, E, TPR, VPT, true, true>), grid, block, 0, stream, a);
-    else if (a.q)
-      hipLaunchKernelGGL((rms_kernel<T, E, TPR, VPT, true, false>), grid, block, 0, stream, a);
-    else if (a.stream)
-      hipLaunchKernelGGL((rms_kernel<T, E, TPR, VPT, false, true>), grid, block, 0, stream, a);
+    if (a.q)
+      hipLaunchKernelGGL((rms_kernel<T, TPR, VPT, true, NT, TAIL>), grid, block, 0, stream, a);
     else
-      hipLaunchKernelGGL((rms_kernel<T, E, TPR, VPT, false, false>), grid, block, 0, stream, a);
+      hipLaunchKernelGGL((rms_kernel<T, TPR, VPT, false, NT, TAIL>), grid, block, 0, stream, a);
     return hipGetLastError();
   }
 };
 
-template <typename T, int E>
+template <typename T, bool NT, bool TAIL>
 struct Backward {
   const RmsBwdArgs& a;
   hipStream_t stream;
   template <int TPR, int VPT>
   hipError_t operator()() const {
-    const dim3 grid((unsigned)a.blocks), block(kThreads<TPR>);
-    if (a.stream)
-      hipLaunchKernelGGL((rms_bwd_kernel<T, E, TPR, VPT, true>), grid, block, 0, stream, a);
-    else
-      hipLaunchKernelGGL((rms_bwd_kernel<T, E, TPR, VPT, false>), grid, block, 0, stream, a);
+    hipLaunchKernelGGL((rms_bwd_kernel<T, TPR, VPT, NT, TAIL>), dim3((unsigned)a.blocks), dim3(kThreads<TPR>), 0, stream, a);
     return hipGetLastError();
   }
 };
 
-bool aligned(const void* p, uintptr_t to = 16) { return ((uintptr_t)p & (to - 1)) == 0; }
+template <template <typename, bool, bool> class Pass, typename T, typename Args>
+hipError_t launch_as(const Args& a, hipStream_t stream) {
+  constexpr int E = 16 / sizeof(T);
+  const int n = (a.channels + E - 1) / E;
+  if (a.channels % E)
+    return a.stream ? choose<E>(n, Pass<T, true, true>{a, stream}) : choose<E>(n, Pass<T, false, true>{a, stream});
+  return a.stream ? choose<E>(n, Pass<T, true, false>{a, stream}) : choose<E>(n, Pass<T, false, false>{a, stream});
+}
 
 }  // namespace
 
 hipError_t launch_rms(int dtype, const RmsArgs& args, hipStream_t stream) {
   RmsArgs a = args;
-  const int size = dtype == FWN_F32 ? 4 : 2, e = 16 / size;
-  const uint64_t bytes = (uint64_t)a.rows * a.channels * size;
+  const uint64_t bytes = (uint64_t)a.rows * a.channels * (dtype == FWN_F32 ? 4 : 2);
   a.stream = (a.y ? bytes : 0) + (a.q ? (uint64_t)a.rows * a.channels : bytes) >= kStreamBytes;
-  const bool vec = a.channels % e == 0 && a.x_stride % e == 0 && a.y_stride % e == 0 && aligned(a.x) && aligned(a.y) &&
-                   aligned(a.weight) && aligned(a.sum) && aligned(a.out) && aligned(a.q, e);
-  const int n = vec ? a.channels / e : a.channels;
-  if (dtype == FWN_F32)
-    return vec ? choose<4>(n, Forward<float, 4>{a, stream}) : choose<1>(n, Forward<float, 1>{a, stream});
-  return vec ? choose<8>(n, Forward<uint16_t, 8>{a, stream}) : choose<1>(n, Forward<uint16_t, 1>{a, stream});
+  return dtype == FWN_F32 ? launch_as<Forward, float>(a, stream) : launch_as<Forward, uint16_t>(a, stream);
 }
 
 // Four rows at least to each of a workgroup's places and about four workgroups a CU.
@@ -446,16 +463,8 @@ int32_t rms_bwd_blocks(int64_t rows, int32_t channels) {
 
 hipError_t launch_rms_bwd(int dtype, const RmsBwdArgs& args, hipStream_t stream) {
   RmsBwdArgs a = args;
-  const int size = dtype == FWN_F32 ? 4 : 2, e = 16 / size;
-  a.stream = (uint64_t)a.rows * a.channels * size >= kStreamBytes;
-  const bool vec = a.channels % e == 0 && aligned(a.s) && aligned(a.weight) && aligned(a.g_out) && aligned(a.g_sum) &&
-                   aligned(a.gx);
-  const int n = vec ? a.channels / e : a.channels;
-  hipError_t rc;
-  if (dtype == FWN_F32)
-    rc = vec ? choose<4>(n, Backward<float, 4>{a, stream}) : choose<1>(n, Backward<float, 1>{a, stream});
-  else
-    rc = vec ? choose<8>(n, Backward<uint16_t, 8>{a, stream}) : choose<1>(n, Backward<uint16_t, 1>{a, stream});
+  a.stream = (uint64_t)a.rows * a.channels * (dtype == FWN_F32 ? 4 : 2) >= kStreamBytes;
+  const hipError_t rc = dtype == FWN_F32 ? launch_as<Backward, float>(a, stream) : launch_as<Backward, uint16_t>(a, stream);
   if (rc != hipSuccess || !a.part) return rc;
   hipLaunchKernelGGL(rms_sums_kernel, dim3((unsigned)(a.channels + 63) / 64), dim3(64 * kGroups), 0, stream, a,
                      dtype == FWN_BF16 && !a.weight_f32);
