@@ -94,15 +94,17 @@ def _backward_torch(x, weight, bias, g, activation, needs):
   differentiate the pre-activation too: it is formed anew) or of batched gradients."""
   dz = g.float()
   if activation:
-    z = torch.mm(x.float(), weight.float().t())
+    z = torch.matmul(x.float(), weight.float().t())
     dz = dz * _slope(z if bias is None else z + bias.float(), activation)
-  return (torch.mm(dz, weight.float()).to(g.dtype) if needs[0] else None,
-          torch.mm(dz.t(), x.float()).to(g.dtype) if needs[1] else None, dz.sum(0).to(g.dtype) if needs[2] else None)
+  rows = lambda t: t.reshape(-1, t.shape[-1])
+  return (torch.matmul(dz, weight.float()).to(g.dtype) if needs[0] else None,
+          torch.mm(rows(dz).t(), rows(x).float()).to(g.dtype) if needs[1] else None,
+          rows(dz).sum(0).to(g.dtype) if needs[2] else None)
 
 
 class _LinearAct(torch.autograd.Function):
-  """x [rows, ins]. Without an activation x is kept for the weight's gradient alone and the weight for x's;
-  with one the pre-activation is kept beside them."""
+  """Without an activation x is kept for the weight's gradient alone and the weight for x's; with one the
+  pre-activation is kept beside them."""
 
   @staticmethod
   def forward(ctx, x, weight, bias, residual, activation):
@@ -116,22 +118,22 @@ class _LinearAct(torch.autograd.Function):
   @staticmethod
   def backward(ctx, g):
     x, weight, bias, pre = ctx.saved_tensors
-    (x_shape, w_shape), act = ctx.sizes, ctx.activation
-    needs = need_x, need_w, need_b = ctx.needs_input_grad[:3]
-    g_res = g if ctx.needs_input_grad[3] else None
-    if not any(needs):
+    (x_shape, (outs, ins)), act = ctx.sizes, ctx.activation
+    needs = need_x, need_w, need_b, need_r, _ = ctx.needs_input_grad
+    g_res = g if need_r else None
+    if not (need_x or need_w or need_b):
       return None, None, None, g_res, None
     if as_torch(g):
       return (*_backward_torch(x, weight, bias, g, act, needs), g_res, None)
-    g = g.contiguous()
-    outs, ins = w_shape
+    g = dense(g)
     xr, xs = rows_of(x) if need_w else (None, 0)
     wr, ws = rows_of(weight) if need_x else (None, 0)
-    d = nat.LinearDesc(x_shape[0], xs, ws, 0, ins, outs, _DTYPES[g.dtype], act)
+    d = nat.LinearDesc(g.numel() // outs, xs, ws, 0, ins, outs, _DTYPES[g.dtype], act)
     L = nat.lib()
-    gx, gw, gb = (torch.empty(shape, dtype=g.dtype, device=g.device) if need else None
-                  for shape, need in zip((x_shape, w_shape, (outs,)), needs))
-    xa, wa, ga, gxa, gwa, gba = (_addr(t) for t in (xr, wr, g, gx, gw, gb))
+    gx = g.new_empty(x_shape) if need_x else None
+    gw = g.new_empty((outs, ins)) if need_w else None
+    gb = g.new_empty(outs) if need_b else None
+    xa, wa, ga, gxa, gwa, gba = _addr(xr), _addr(wr), _addr(g), _addr(gx), _addr(gw), _addr(gb)
     work, size = _workspace(L.fwn_linear_act_bwd_workspace_size, d, g, xa, wa, ga, gxa, gwa, gba)
     launch(g, L.fwn_linear_act_bwd_launch, d, xa, wa, _addr(pre), ga, gxa, gwa, gba, _addr(work), size)
     return gx, gw, gb, g_res, None
@@ -155,8 +157,7 @@ def linear_act(x, weight, bias=None, *, activation=None, residual=None):
   _check(x, weight, bias, residual, x.dtype, x.shape[:-1])
   if not _needs(x, weight, bias, residual):
     return _forward(x, weight, bias, residual, act, False)[0]
-  rows = lambda t: None if t is None else t.reshape(-1, t.shape[-1])
-  return _LinearAct.apply(rows(x), weight, bias, rows(residual), act).view(*x.shape[:-1], weight.shape[0])
+  return _LinearAct.apply(x, weight, bias, residual, act)
 
 
 def linear_act_q8(x, x_scale, weight, weight_scale, bias=None, *, activation=None, residual=None, dtype=torch.bfloat16):
