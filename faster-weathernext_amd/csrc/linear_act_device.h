@@ -194,11 +194,14 @@ __device__ __forceinline__ Work work_of(const EpilogueArgs& e) {
 
 typedef __attribute__((address_space(3))) float* strip_ptr;
 constexpr int kStrip = 72;                      // floats from one row of a strip to the next: its halves' rows fall in other banks
-constexpr int kStripBytes = 32 * kStrip * 4;  // of LDS, for each wave
+constexpr int kStripBf16 = 80;                  // the same of 64 rows of bf16
+constexpr int kStripBytes = 64 * kStripBf16 * 2;  // of LDS, for each wave
+static_assert(kStripBytes >= 32 * kStrip * 4, "either strip");
 
 // The epilogue of a wave's 32 MI x 64 part (from row wm and column wn) of a BM-row tile: 32 rows at a time through
 // the wave's strip of LDS to rows of eight columns a lane, or of one column a lane where rows are not whole aligned
-// eights. PLAIN: no epilogue but the rounding (gradients). F32: 1 the outputs are float32, 0 bf16, -1 either.
+// eights. bf16 outputs that nothing but their column's bias is added to are finished where the MFMAs leave them
+// and go through LDS as bf16, 64 rows at a time: half the LDS traffic, and longer runs of it. PLAIN: no epilogue but the rounding (gradients). F32: 1 the outputs are float32, 0 bf16, -1 either.
 // mend(row, col, v) may put right outputs before the epilogue.
 template <int BM, int MI, bool PLAIN, int F32, bool SCALED, typename Mend>
 __device__ __forceinline__ void write_tile(const ProductArgs& g, const Work& k, const f32x16 (&acc)[MI][2], strip_ptr strip,
@@ -213,6 +216,59 @@ __device__ __forceinline__ void write_tile(const ProductArgs& g, const Work& k, 
   };
   const EpilogueArgs& e = g.e;
   const int rows = (int)(e.m - k.i0 < BM ? e.m - k.i0 : BM);  // of the tile
+  if constexpr (F32 != 1) {
+    if (!g.part && e.vec && e.dtype == FWN_BF16 && (PLAIN || (!e.pre && !e.residual))) {
+      static_assert(MI % 2 == 0, "64 rows at a time");
+      auto* const half_strip = (__attribute__((address_space(3))) uint16_t*)strip;
+      float bias[2], scale[2];
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const int64_t col = k.j0 + wn + 32 * n + j;
+        bias[n] = !PLAIN && e.bias && col < e.n ? load_one(e.bias, col, FWN_BF16) : 0.f;
+        scale[n] = SCALED && col < e.n ? e.b_scale[col] : 0.f;
+      }
+      const rsrc_t ro = make_rsrc((char*)e.out + (k.i0 * e.n + k.j0) * 2, kBuffer);
+      const rsrc_t rs = make_rsrc(e.a_scale + (SCALED ? k.i0 : 0), kBuffer);
+      const int sub = lane >> 3, at_col = wn + 8 * (lane & 7);
+      const uint32_t nowhere = k.j0 + at_col < e.n ? 0 : kNowhere;
+      with_activation<PLAIN>(e.activation, [&](auto act) {
+#pragma unroll
+        for (int m0 = 0; m0 < MI; m0 += 2) {
+#pragma unroll
+          for (int m = m0; m < m0 + 2; ++m) {
+            float a_scale[16];
+            if constexpr (SCALED) {
+#pragma unroll
+              for (int r = 0; r < 16; ++r) {
+                const int row = wm + 32 * m + 8 * (r >> 2) + 4 * half + (r & 3);
+                a_scale[r] = as_float(
+                    __builtin_amdgcn_raw_buffer_load_b32(rs, (int)((uint32_t)row * 4 | (row < rows ? 0 : kNowhere)), 0, 0));
+              }
+            }
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+              for (int r = 0; r < 16; ++r) {
+                float v = acc[m][n][r];
+                if constexpr (SCALED) v *= a_scale[r] * scale[n];
+                if constexpr (!PLAIN) v = activate<decltype(act)::kind>(v + bias[n]);
+                half_strip[(32 * (m - m0) + 8 * (r >> 2) + 4 * half + (r & 3)) * kStripBf16 + 32 * n + j] = (uint16_t)bf16_bits(v);
+              }
+          }
+          __builtin_amdgcn_wave_barrier();
+#pragma unroll
+          for (int p = 0; p < 8; ++p) {
+            const int row = wm + 32 * m0 + 8 * p + sub;
+            const u32x4 v = *(const __attribute__((address_space(3))) u32x4*)(half_strip + (8 * p + sub) * kStripBf16 + 8 * (lane & 7));
+            __builtin_amdgcn_raw_buffer_store_b128(
+                v, ro, (int)(((uint32_t)row * (uint32_t)e.n + (uint32_t)at_col) * 2 | (row < rows ? 0 : kNowhere) | nowhere), 0, 0);
+          }
+          __builtin_amdgcn_wave_barrier();
+        }
+      });
+      return;
+    }
+  }
   if (g.part || e.vec) {
     // Offsets in the tile.
     const bool f32 = g.part || F32 == 1 || (F32 == -1 && e.dtype == FWN_F32);
