@@ -38,6 +38,7 @@ struct ProductArgs {
   float* part;                 // [splits, m, part_row] where splits > 1
   int64_t part_row;            // n padded to 8
   float* sums;                 // column sums of an outer a: [splits, m], or null
+  void* sums_out;              // the sums in the dtype where splits is 1, or null
   EpilogueArgs e;
 };
 
@@ -71,7 +72,8 @@ struct SlopeArgs {
   const void* pre;  // [rows, outs], unread without an activation
   char* dz;         // or null
   int64_t dz_stride;  // bytes, room for whole eights of columns
-  float* part;      // [blocks, outs] partial sums, or null: no sums
+  float* part;      // [blocks, outs] partial sums, or null
+  void* gb;         // the sums in the dtype where blocks is 1, or null
   int64_t rows, chunk;  // rows of a workgroup
   int32_t outs, dtype, activation, blocks;
 };

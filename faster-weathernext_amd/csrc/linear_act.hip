@@ -171,7 +171,7 @@ __global__ void __launch_bounds__((threads_of(BM)), 2) product_kernel(ProductArg
                                                                     0x7f7f7f7f, 0, 0x7f7f7f7f);
   };
   // Column sums of a, in the workgroups of the first column tile: wave w takes 32 columns.
-  const bool sums = OA && g.sums != nullptr && k.j0 == 0;
+  const bool sums = OA && (g.sums || g.sums_out) && k.j0 == 0;
   float sum = 0.f;
   Reads<OA, 1> rs;
   rs.init(0, 32 * w, lane);
@@ -233,7 +233,13 @@ __global__ void __launch_bounds__((threads_of(BM)), 2) product_kernel(ProductArg
   if constexpr (OA) {
     if (sums) {
       sum += __shfl_xor(sum, 32);
-      if (lane < 32 && k.i0 + 32 * w + lane < g.e.m) g.sums[(int64_t)k.split * g.e.m + k.i0 + 32 * w + lane] = sum;
+      const int64_t row = k.i0 + 32 * w + lane;
+      if (lane < 32 && row < g.e.m) {
+        if (g.sums_out)
+          store_one(g.sums_out, row, g.e.dtype, sum);
+        else
+          g.sums[(int64_t)k.split * g.e.m + row] = sum;
+      }
     }
   }
   constexpr int PER = WAVES / 2;  // waves whose strips share a stage's array

@@ -132,7 +132,7 @@ struct Cost {
 };
 
 Plan plan(int64_t m, int64_t n, int64_t k, int32_t op) {
-  constexpr Cost bf16[] = {{256, 1.55, 1.55, 6.0}, {128, 0.6, 0.5, 2.2}}, f32[] = {{128, 2.0, 1.1, 3.0}};
+  constexpr Cost bf16[] = {{256, 1.55, 1.55, 5.0}, {128, 0.6, 0.5, 2.0}}, f32[] = {{128, 2.0, 1.1, 3.0}};
   const int64_t of = op == kOpF32 ? kStageF32 : op == kOpE4m3 ? kStageBytes : kStageRows;
   const int64_t stages = std::max<int64_t>(1, parts(k, of));
   Plan best{128, 1, (int32_t)stages};
@@ -176,7 +176,7 @@ struct Product {
     g.e.n = n;
     g.part_row = up(n, 8);
     g.part = p.splits > 1 ? (float*)ws.take((uint64_t)p.splits * m * g.part_row * sizeof(float)) : nullptr;
-    g.sums = sums ? (float*)ws.take((uint64_t)p.splits * m * sizeof(float)) : nullptr;
+    g.sums = sums && p.splits > 1 ? (float*)ws.take((uint64_t)p.splits * m * sizeof(float)) : nullptr;
   }
 
   hipError_t launch(const Matrix& a, const Matrix& b, hipStream_t stream) {
@@ -238,8 +238,10 @@ int forward(const fwn_linear_desc* d, int32_t op, const void* x, const float* x_
   return status(f.z.launch(f.x, f.w, s), what);
 }
 
-// Workgroups by rows of the dz pass: about four workgroups a CU, 32 rows at least.
+// Rows of a workgroup in the dz pass: about four workgroups a CU, 32 rows at least; up to 128 rows one workgroup sums
+// a column, which saves the launch that joins the sums.
 int64_t slope_chunk(int64_t rows, int64_t outs) {
+  if (rows <= 128) return std::max<int64_t>(1, rows);
   const int64_t blocks = std::max<int64_t>(1, std::min(4 * kCus / parts(outs, 256), parts(rows, 32)));
   return std::max<int64_t>(1, parts(rows, blocks));
 }
@@ -263,7 +265,7 @@ struct Backward {
     sums_in_product = need_b && need_w && !formed && op == kOpBf16;
     slope.chunk = slope_chunk(d->rows, d->outs);
     slope.blocks = (int32_t)std::max<int64_t>(1, parts(d->rows, slope.chunk));
-    if (need_b && !sums_in_product) slope.part = (float*)ws.take((uint64_t)slope.blocks * d->outs * sizeof(float));
+    if (need_b && !sums_in_product && slope.blocks > 1) slope.part = (float*)ws.take((uint64_t)slope.blocks * d->outs * sizeof(float));
     if (need_x) {
       w.place(wp, d->outs, d->ins, d->w_stride, op, ws);
       to_x.shape(Operands::kInnerOuter, d->rows, d->ins, d->outs, op, false, ws);
@@ -359,8 +361,9 @@ int fwn_linear_act_bwd_launch(const fwn_linear_desc* d, const void* x, const voi
     a.outs = d->outs;
     a.dtype = d->dtype;
     a.activation = d->activation;
+    a.gb = gb && !b.sums_in_product && a.blocks == 1 ? gb : nullptr;
     if (int rc = status(launch_slope(a, s), what)) return rc;
-    if (gb)
+    if (gb && !b.sums_in_product && a.blocks > 1)
       if (int rc = status(launch_column_sums(a.part, a.blocks, d->outs, gb, d->dtype, s), what)) return rc;
   }
   if (gx && d->rows > 0) {
@@ -373,8 +376,9 @@ int fwn_linear_act_bwd_launch(const fwn_linear_desc* d, const void* x, const voi
     if (int rc = status(b.x.lay_out(s), what)) return rc;
     b.to_w.g.e.out = gw;
     b.to_w.g.e.dtype = d->dtype;
+    b.to_w.g.sums_out = b.sums_in_product && b.to_w.p.splits == 1 ? gb : nullptr;
     if (int rc = status(b.to_w.launch(b.dz, b.x, s), what)) return rc;
-    if (b.sums_in_product)
+    if (b.sums_in_product && b.to_w.p.splits > 1)
       if (int rc = status(launch_column_sums(b.to_w.g.sums, b.to_w.p.splits, d->outs, gb, d->dtype, s), what)) return rc;
   }
   return FWN_OK;

@@ -80,7 +80,7 @@ __global__ void __launch_bounds__(256) slope_kernel(SlopeArgs a) {
       }
     }
   }
-  if (!a.part) return;
+  if (!a.part && !a.gb) return;
 #pragma unroll
   for (int k = 0; k < 8; ++k) red[own][column(k) - c0] = sum[k];
   __syncthreads();
@@ -89,7 +89,10 @@ __global__ void __launch_bounds__(256) slope_kernel(SlopeArgs a) {
   float s = red[0][c];
 #pragma unroll
   for (int k = 1; k < 8; ++k) s += red[k][c];
-  a.part[(int64_t)block * a.outs + c0 + c] = s;
+  if (a.gb)
+    store_one(a.gb, c0 + c, a.dtype, s);
+  else
+    a.part[(int64_t)block * a.outs + c0 + c] = s;
 }
 
 constexpr int kSumCols = 16, kGroups = 64;  // columns of a workgroup, and shares of the rows that it adds in parallel
