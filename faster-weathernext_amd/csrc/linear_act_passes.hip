@@ -5,35 +5,22 @@
 namespace fwn {
 namespace {
 
+constexpr int64_t kMostBlocks = 1 << 20;  // of the layout's launch; more are looped over
+
 // Rows padded with zeros to 16 bytes, 16 bytes a thread.
+template <typename T>
 __global__ void __launch_bounds__(256) layout_kernel(LayoutArgs a) {
-  const int per = a.op == kOpE4m3 ? 16 : a.op == kOpBf16 ? 8 : 4;  // columns a thread
-  const int64_t across = (a.cols + per - 1) / per, id = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t row = id / across, col = (id - row * across) * per;
-  if (row >= a.rows) return;
-  char* dst = a.dst + row * a.dst_stride + (id - row * across) * 16;
-  if (a.op == kOpE4m3) {
-    const uint8_t* p = (const uint8_t*)a.src + row * a.stride + col;
+  constexpr int PER = 16 / sizeof(T);  // columns a thread
+  const int64_t across = (a.cols + PER - 1) / PER, total = a.rows * across;
+  for (int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x; id < total; id += (int64_t)gridDim.x * 256) {
+    const int64_t row = id / across, at = id - row * across, col = at * PER;
+    const T* p = (const T*)a.src + row * a.stride + col;
     uint32_t d[4] = {};
 #pragma unroll
-    for (int k = 0; k < 16; ++k)
-      if (col + k < a.cols) d[k / 4] |= (uint32_t)p[k] << 8 * (k % 4);
-    *(u32x4*)dst = u32x4{d[0], d[1], d[2], d[3]};
-    return;
+    for (int k = 0; k < PER; ++k)
+      if (col + k < a.cols) d[k * (int)sizeof(T) / 4] |= (uint32_t)p[k] << 8 * (k * (int)sizeof(T) % 4);
+    *(u32x4*)(a.dst + row * a.dst_stride + at * 16) = u32x4{d[0], d[1], d[2], d[3]};
   }
-  uint32_t d[4] = {};
-  if (a.op == kOpBf16) {
-    const uint16_t* p = (const uint16_t*)a.src + row * a.stride + col;
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (col + k < a.cols) d[k / 2] |= (uint32_t)p[k] << 16 * (k % 2);
-  } else {
-    const uint32_t* p = (const uint32_t*)a.src + row * a.stride + col;
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (col + k < a.cols) d[k] = p[k];
-  }
-  *(u32x4*)dst = u32x4{d[0], d[1], d[2], d[3]};
 }
 
 // 256 columns by `chunk` rows a workgroup, eight columns of every eighth row a thread: side by side where rows are whole
@@ -127,10 +114,16 @@ __global__ void __launch_bounds__(kSumCols * kGroups) column_sums_kernel(const f
 }  // namespace
 
 hipError_t launch_layout(const LayoutArgs& a, hipStream_t stream) {
-  const int per = a.op == kOpE4m3 ? 16 : a.op == kOpBf16 ? 8 : 4;
-  const int64_t threads = a.rows * ((a.cols + per - 1) / per);
+  const int64_t per = a.op == kOpE4m3 ? 16 : a.op == kOpBf16 ? 8 : 4, threads = a.rows * ((a.cols + per - 1) / per);
   if (threads == 0) return hipSuccess;
-  hipLaunchKernelGGL(layout_kernel, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, stream, a);
+  const int64_t blocks = (threads + 255) / 256;
+  const dim3 grid((unsigned)(blocks < kMostBlocks ? blocks : kMostBlocks)), block(256);
+  if (a.op == kOpE4m3)
+    hipLaunchKernelGGL(layout_kernel<uint8_t>, grid, block, 0, stream, a);
+  else if (a.op == kOpBf16)
+    hipLaunchKernelGGL(layout_kernel<uint16_t>, grid, block, 0, stream, a);
+  else
+    hipLaunchKernelGGL(layout_kernel<uint32_t>, grid, block, 0, stream, a);
   return hipGetLastError();
 }
 

@@ -15,6 +15,7 @@ if their channels are contiguous. The weight is [channels] in x's dtype or float
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native as nat
 from .rows import _DTYPES, _addr, as_torch
@@ -172,11 +173,18 @@ class _RmsNorm(torch.autograd.Function):
 
 
 def _no_grad(name, *tensors):
-  if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors):
+  """Refuses tensors that autograd, backward or forward, would have to differentiate."""
+  tensors = [t for t in tensors if isinstance(t, torch.Tensor)]
+  if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+    raise RuntimeError(f"{name} has no derivative")
+  if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
     raise RuntimeError(f"{name} has no derivative")
 
 
 def _needs(*tensors):
+  """Whether autograd has to see the call (forward mode too: the Function refuses its tangents)."""
+  if forward_ad._current_level >= 0:
+    return True
   if torch.is_grad_enabled():
     for t in tensors:
       if t is not None and t.requires_grad:

@@ -510,3 +510,42 @@ def test_slopes_are_the_activations_derivatives():
   z = z[z != 0]
   for name, code in nat.ACTIVATIONS.items():
     torch.testing.assert_close(_slope(z, code), _act64(z, name)[1], rtol=1e-6, atol=1e-7)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_far_apart_rows(dtype):
+  """Rows more than 2^20 elements apart, of every operand."""
+  far = (1 << 20) + 72
+  def spread(rows, cols, seed):
+    buf = torch.full((rows * far,), float("nan"), device=DEV, dtype=dtype)
+    return buf.as_strided((rows, cols), (far, 1)).copy_(_whole((rows, cols), dtype, seed))
+  for rows in (3, 40):
+    x, w, r = spread(rows, 200, 1), spread(24, 200, 2), spread(rows, 24, 3)
+    lx, lw = x.detach().requires_grad_(), w.detach().requires_grad_()
+    out = fwn.linear_act(lx, lw, residual=r)
+    assert torch.equal(out, (x.double() @ w.double().t() + r.double()).to(dtype))
+    g = _whole((rows, 24), dtype, 4)
+    gx, gw = torch.autograd.grad(out, (lx, lw), g)
+    assert torch.equal(gx, (g.double() @ w.double()).to(dtype)) and torch.equal(gw, (g.double().t() @ x.double()).to(dtype))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_offsets_past_32_bits(dtype):
+  """x and its gradient past 2^32 bytes: rows near the end, to the bit."""
+  size = 2 if dtype == torch.bfloat16 else 4
+  ins = 16384
+  rows = (1 << 32) // (ins * size) + 1000
+  gen = torch.Generator(device=DEV).manual_seed(1)
+  x = torch.randint(-2, 3, (rows, ins), generator=gen, device=DEV, dtype=torch.int8).to(dtype)
+  w = _whole((40, ins), dtype, 2)
+  g = torch.randint(-2, 3, (rows, 40), generator=gen, device=DEV, dtype=torch.int8).to(dtype)
+  at = [0, 255, rows // 2, rows - 3, rows - 2, rows - 1]
+  lx, lw = x.requires_grad_(), w.clone().requires_grad_()
+  out = fwn.linear_act(lx, lw)
+  assert torch.equal(out[at], (x.detach()[at].double() @ w.double().t()).to(dtype))
+  gx, gw = torch.autograd.grad(out, (lx, lw), g)
+  assert torch.equal(gx[at], (g[at].double() @ w.double()).to(dtype))
+  cols = [0, 100, ins - 1]
+  assert torch.equal(gw[:, cols], (g.double().t() @ x.detach()[:, cols].double()).to(dtype))

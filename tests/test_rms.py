@@ -348,3 +348,45 @@ def test_needs_a_gpu_tensor():
   for call in (fwn.rms_norm, fwn.rms_norm_q8, fwn.quantize_rows):
     with pytest.raises(ValueError, match="CUDA"):
       call(torch.zeros(2, 64))
+
+
+@gpu
+def test_offsets_past_32_bits():
+  """Rows whose bytes lie past 2^32 from the first, in the forward, the 8-bit output and the backward."""
+  rows, c = 140000, 16384  # 4.6 GB
+  gen = torch.Generator(device=DEV).manual_seed(1)
+  x = torch.randint(-4, 5, (rows, c), generator=gen, device=DEV, dtype=torch.int8).to(torch.bfloat16)
+  w = _normal((c,), torch.bfloat16, 2)
+  at = [0, 1, rows // 2, rows - 2, rows - 1]
+  out = fwn.rms_norm(x, w)
+  want = _norm64(x[at], w, 1e-6)
+  _within(out[at], want, want.abs() * (2.0 ** -8 + NEAR) + 1e-37)
+  q, scale = fwn.rms_norm_q8(x, w)
+  _check_q8(q[at], scale[at], want)
+  leaf = x.requires_grad_()
+  gx, = torch.autograd.grad(fwn.rms_norm(leaf, w), leaf, out)
+  wx, _, bx, _ = _grads64(x.detach()[at], w, 1e-6, out[at], None)
+  _within(gx[at], wx, wx.abs() * 2.0 ** -8 + bx)
+
+
+@gpu
+def test_the_same_tensor_twice():
+  x, g = _normal((9, 72), torch.float32, 1), _normal((9, 72), torch.float32, 2)
+  leaf = x.clone().requires_grad_()
+  s, out = fwn.add_rms_norm(leaf, leaf)
+  gx, = torch.autograd.grad(out, leaf, g)
+  want, _, bx, _ = _grads64(s.detach(), None, 1e-6, g, None)
+  _within(gx, 2 * want, 2.0 ** -23 * want.abs() + 2 * bx)
+
+
+@gpu
+def test_forward_mode_is_refused():
+  import torch.autograd.forward_ad as fwad
+  x = _normal((4, 64), torch.float32, 1)
+  with fwad.dual_level():
+    dual = fwad.make_dual(x, torch.ones_like(x))
+    for call in (fwn.rms_norm, fwn.rms_norm_q8, fwn.quantize_rows, lambda t: fwn.add_rms_norm(t, x),
+                 lambda t: fwn.linear_act(t, x)):
+      with pytest.raises(RuntimeError):
+        call(dual)
+    assert torch.equal(fwn.rms_norm(x), fwn.rms_norm(x))
