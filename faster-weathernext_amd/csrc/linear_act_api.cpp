@@ -120,7 +120,10 @@ struct Matrix {
 
 // The tiles and ranges of the sum of one product, by an estimate of its time in us: a CU takes its share of the
 // workgroups one after the other, or two at a time where that fills it, each its stages and its ends (the
-// first loads and the epilogue); split sums add the partial products' trip through memory.
+// first loads and the epilogue); split sums add the partial products' trip through memory. Both tiles, one range, us
+// with 256 and with 128 (rows x inputs -> outputs, bf16): 40,962 x 768 -> 3,072 231 and 247, 40,962 x 3,072 -> 768 180
+// and 208, 65,536 x 256 -> 1,024 64 and 71; 10,242 x 3,072 -> 768 72 and 50, 40,962 x 128 -> 512 20 and 18. Ranges: the
+// weight's gradient over 40,962 rows of 768 -> 3,072 takes 840 and 492 with one and 187 with the ones taken here.
 struct Plan {
   int tile;
   int32_t splits, chunk;
@@ -132,7 +135,7 @@ struct Cost {
 };
 
 Plan plan(int64_t m, int64_t n, int64_t k, int32_t op) {
-  constexpr Cost bf16[] = {{256, 1.55, 1.55, 5.0}, {128, 0.6, 0.5, 2.0}}, f32[] = {{128, 2.0, 1.1, 3.0}};
+  constexpr Cost bf16[] = {{256, 1.55, 1.55, 9.0}, {128, 0.6, 0.5, 1.8}}, f32[] = {{128, 2.0, 1.1, 3.0}};
   const int64_t of = op == kOpF32 ? kStageF32 : op == kOpE4m3 ? kStageBytes : kStageRows;
   const int64_t stages = std::max<int64_t>(1, parts(k, of));
   Plan best{128, 1, (int32_t)stages};
