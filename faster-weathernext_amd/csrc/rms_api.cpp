@@ -138,10 +138,12 @@ int fwn_rms_norm_bwd_launch(const fwn_rms_desc* d, const void* s, const void* we
   if (misaligned(s, size) || misaligned(g_out, size) || misaligned(g_sum, size) || misaligned(gx, size) ||
       misaligned(weight, size_of(d->weight_dtype)) || misaligned(gw, size_of(d->weight_dtype)))
     return fail(FWN_ERR_INVALID_ARG, "%s: a tensor is not aligned to its elements", what);
-  const Span out = rows_of(d, gx, d->channels, size);
-  for (const void* p : {s, g_out, g_sum})
-    if (overlap(out, rows_of(d, p, d->channels, size)))
-      return fail(FWN_ERR_INVALID_ARG, "%s: gx must not overlap an input", what);
+  const uint64_t channels = (uint64_t)d->channels * size_of(d->weight_dtype);
+  const Span out = rows_of(d, gx, d->channels, size), sums{gw, channels};
+  for (const Span& in : {rows_of(d, s, d->channels, size), rows_of(d, g_out, d->channels, size),
+                         rows_of(d, g_sum, d->channels, size), Span{weight, channels}})
+    if (overlap(out, in) || overlap(sums, in)) return fail(FWN_ERR_INVALID_ARG, "%s: an output overlaps an input", what);
+  if (overlap(out, sums)) return fail(FWN_ERR_INVALID_ARG, "%s: outputs overlap", what);
   if (gw && (!workspace || misaligned(workspace, 16) || workspace_bytes < part_bytes(d)))
     return fail(FWN_ERR_INVALID_ARG, "%s: a 16-byte aligned workspace of %llu bytes is needed", what,
                 (unsigned long long)part_bytes(d));

@@ -155,7 +155,7 @@ int fwn_quantize_rows_launch(const fwn_rms_desc* d, const void* x, uint8_t* q, f
  *   gw = sum over the rows of g_out s r, in weight_dtype
  * g_sum (NULL: zeros) is the gradient of sum. gx is the gradient of x and of y. gw may be NULL; with it the
  * launch needs fwn_rms_norm_bwd_workspace_size bytes of workspace (16-byte aligned), whose sums run in a
- * fixed order. gx must not overlap an input. */
+ * fixed order. gx and gw must not overlap an input or each other. */
 int fwn_rms_norm_bwd_workspace_size(const fwn_rms_desc* d, uint64_t* bytes);
 int fwn_rms_norm_bwd_launch(const fwn_rms_desc* d, const void* s, const void* weight, const void* g_out,
                             const void* g_sum, void* gx, void* gw, void* workspace, uint64_t workspace_bytes,
@@ -167,7 +167,8 @@ int fwn_rms_norm_bwd_launch(const fwn_rms_desc* d, const void* s, const void* we
  * r_stride elements apart (0: one row for all; r_stride at most FWN_LINEAR_ACT_MAX); bias [outs], out and pre
  * [rows, outs] are contiguous.
  * Products accumulate in float32; out, and pre (z for the backward, NULL: not stored) are rounded
- * once. bias and residual may be NULL. Every tensor is of `dtype`; float32 products keep float32's precision. */
+ * once. bias and residual may be NULL. Every tensor is of `dtype`; float32 products keep float32's precision. No output
+ * of the launches here may overlap an input or another output. */
 #define FWN_ACT_NONE 0
 #define FWN_ACT_RELU 1
 #define FWN_ACT_GELU 2      /* z (1 + erf(z / sqrt 2)) / 2 */

@@ -390,3 +390,10 @@ def test_forward_mode_is_refused():
       with pytest.raises(RuntimeError):
         call(dual)
     assert torch.equal(fwn.rms_norm(x), fwn.rms_norm(x))
+
+
+def test_backward_outputs_overlap_nothing():
+  L, d = nat.lib(), _desc()
+  for gx, gw, weight in ((3 * F, 3 * F + 256, 5 * F), (3 * F, 4 * F, 3 * F), (3 * F, 5 * F, 5 * F), (3 * F, F, 5 * F),
+                         (3 * F, 2 * F, 5 * F)):
+    assert L.fwn_rms_norm_bwd_launch(d, F, weight, 2 * F, None, gx, gw, 16 * F, 1 << 20, None) == nat.ERR_INVALID_ARG
