@@ -425,11 +425,14 @@ struct MendParts {
     for (int e = 0; e < N; ++e) bad |= v[e] != v[e];
     if (!bad) return;
     float s[N] = {};
-    for (int64_t k = 0; k < g.k; ++k) {
+    for (int64_t k = 0; k < g.k && bad; ++k) {  // until every one is NaN for good
       const float x = value<OA>(g.a, g.a_stride, row, k);
+      bad = false;
 #pragma unroll
-      for (int e = 0; e < N; ++e)
+      for (int e = 0; e < N; ++e) {
         if (col + e < g.e.n) s[e] = fmaf(x, value<OB>(g.b, g.b_stride, col + e, k), s[e]);
+        bad |= v[e] != v[e] && s[e] == s[e];
+      }
     }
 #pragma unroll
     for (int e = 0; e < N; ++e)
