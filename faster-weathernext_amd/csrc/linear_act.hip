@@ -155,7 +155,7 @@ __global__ void __launch_bounds__((threads_of(BM)), 2) product_kernel(ProductArg
 #pragma unroll
     for (int m = 0; m < MI; ++m)
 #pragma unroll
-      for (int n = 0; n < NI; ++n) acc[m][n] = mfma_bf16(fa[set][m], fb[set][n], acc[m][n]);
+      for (int n = 0; n < NI; ++n) acc[m][n] = mfma_bf16(fb[set][n], fa[set][m], acc[m][n]);
   };
   // The same for half a stage of e4m3: 64 k, the bytes of two quarters, scales 2^0.
   const auto multiply8 = [&](int set) {
@@ -166,8 +166,8 @@ __global__ void __launch_bounds__((threads_of(BM)), 2) product_kernel(ProductArg
     for (int m = 0; m < MI; ++m)
 #pragma unroll
       for (int n = 0; n < NI; ++n)
-        acc[m][n] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(join(fa[set][m], fa[set + 1][m]),
-                                                                    join(fb[set][n], fb[set + 1][n]), acc[m][n], 0, 0, 0,
+        acc[m][n] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(join(fb[set][n], fb[set + 1][n]),
+                                                                    join(fa[set][m], fa[set + 1][m]), acc[m][n], 0, 0, 0,
                                                                     0x7f7f7f7f, 0, 0x7f7f7f7f);
   };
   // Column sums of a, in the workgroups of the first column tile: wave w takes 32 columns.

@@ -193,16 +193,21 @@ __device__ __forceinline__ Work work_of(const EpilogueArgs& e) {
 }
 
 typedef __attribute__((address_space(3))) float* strip_ptr;
-constexpr int kStrip = 72;                      // floats from one row of a strip to the next: its halves' rows fall in other banks
-constexpr int kStripBf16 = 80;                  // the same of 64 rows of bf16
-constexpr int kStripBytes = 64 * kStripBf16 * 2;  // of LDS, for each wave
-static_assert(kStripBytes >= 32 * kStrip * 4, "either strip");
+// Fours at any address of an element.
+typedef uint32_t bf16x4_any __attribute__((ext_vector_type(2), aligned(2)));
+typedef uint32_t f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
+constexpr int kStrip = 72;                      // floats from one row of a strip to the next: eight rows' fours fall in other banks
+constexpr int kStripBytes = 32 * kStrip * 4;    // of LDS, for each wave
+static_assert(kStripBytes >= 64 * 128, "a strip of 64 rows of bf16, chunk c of row r at c ^ (r / 2 % 8)");
 
-// The epilogue of a wave's 32 MI x 64 part (from row wm and column wn) of a BM-row tile: 32 rows at a time through
-// the wave's strip of LDS to rows of eight columns a lane, or of one column a lane where rows are not whole aligned
-// eights. bf16 outputs that nothing but their column's bias is added to are finished where the MFMAs leave them
-// and go through LDS as bf16, 64 rows at a time: half the LDS traffic, and longer runs of it. PLAIN: no epilogue but the rounding (gradients). F32: 1 the outputs are float32, 0 bf16, -1 either.
-// mend(row, col, v) may put right outputs before the epilogue.
+// The epilogue of a wave's 32 MI x 64 part (from row wm and column wn) of a BM-row tile. The products are formed with
+// the weight's side as the MFMA's rows, so that a lane's registers are fours of columns of one row (acc[m][n][4 q + i]:
+// row 32 m + lane % 32, column 32 n + 8 q + 4 (lane / 32) + i), which go to LDS whole (gx of 10,242 x 768 with 3,072
+// outputs 62 us with single columns, 57 so): 32 rows at a time through the wave's strip to rows of eight columns a
+// lane, or of one column a lane where rows are not whole aligned eights. bf16 outputs that nothing but their column's
+// bias is added to are finished where the MFMAs leave them and go through LDS as bf16, 64 rows at a time. PLAIN: no
+// epilogue but the rounding (gradients). F32: 1 the outputs are float32, 0 bf16, -1 either. mend(row, col, v) may put
+// right outputs before the epilogue.
 template <int BM, int MI, bool PLAIN, int F32, bool SCALED, typename Mend>
 __device__ __forceinline__ void write_tile(const ProductArgs& g, const Work& k, const f32x16 (&acc)[MI][2], strip_ptr strip,
                                            int wm, int wn, int lane, const Mend& mend) {
@@ -211,7 +216,9 @@ __device__ __forceinline__ void write_tile(const ProductArgs& g, const Work& k, 
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) strip[(8 * (r >> 2) + 4 * half + (r & 3)) * kStrip + 32 * n + j] = acc[m][n][r];
+      for (int q = 0; q < 4; ++q)
+        *(__attribute__((address_space(3))) f32x4*)(strip + j * kStrip + 32 * n + 8 * q + 4 * half) =
+            f32x4{acc[m][n][4 * q], acc[m][n][4 * q + 1], acc[m][n][4 * q + 2], acc[m][n][4 * q + 3]};
     __builtin_amdgcn_wave_barrier();
   };
   const EpilogueArgs& e = g.e;
@@ -219,16 +226,25 @@ __device__ __forceinline__ void write_tile(const ProductArgs& g, const Work& k, 
   if constexpr (F32 != 1) {
     if (!g.part && e.vec && e.dtype == FWN_BF16 && (PLAIN || (!e.pre && !e.residual))) {
       static_assert(MI % 2 == 0, "64 rows at a time");
-      auto* const half_strip = (__attribute__((address_space(3))) uint16_t*)strip;
-      float bias[2], scale[2];
+      typedef __attribute__((address_space(3))) char* bytes_ptr;
+      bytes_ptr const half_strip = (bytes_ptr)strip;
+      // This lane's columns are fours: 32 n + 8 q + 4 half.
+      float bias[2][4][4], scale[2][4][4];
+      if constexpr (!PLAIN) {
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        const int64_t col = k.j0 + wn + 32 * n + j;
-        bias[n] = !PLAIN && e.bias && col < e.n ? load_one(e.bias, col, FWN_BF16) : 0.f;
-        scale[n] = SCALED && col < e.n ? e.b_scale[col] : 0.f;
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int64_t col = k.j0 + wn + 32 * n + 8 * q + 4 * half;
+            const u32x2 u = e.bias && col < e.n ? *(const bf16x4_any*)((const uint16_t*)e.bias + col) : u32x2{0, 0};
+            const u32x4 v = SCALED && col < e.n ? *(const f32x4_any*)(e.b_scale + col) : u32x4{0, 0, 0, 0};
+            const uint32_t lo = u[0], hi = u[1], v0 = v[0], v1 = v[1], v2 = v[2], v3 = v[3];
+            bias[n][q][0] = as_float(lo << 16), bias[n][q][1] = as_float(lo & 0xffff0000u);
+            bias[n][q][2] = as_float(hi << 16), bias[n][q][3] = as_float(hi & 0xffff0000u);
+            scale[n][q][0] = as_float(v0), scale[n][q][1] = as_float(v1), scale[n][q][2] = as_float(v2), scale[n][q][3] = as_float(v3);
+          }
       }
       const rsrc_t ro = make_rsrc((char*)e.out + (k.i0 * e.n + k.j0) * 2, kBuffer);
-      const rsrc_t rs = make_rsrc(e.a_scale + (SCALED ? k.i0 : 0), kBuffer);
       const int sub = lane >> 3, at_col = wn + 8 * (lane & 7);
       const uint32_t nowhere = k.j0 + at_col < e.n ? 0 : kNowhere;
       with_activation<PLAIN>(e.activation, [&](auto act) {
@@ -236,30 +252,30 @@ __device__ __forceinline__ void write_tile(const ProductArgs& g, const Work& k, 
         for (int m0 = 0; m0 < MI; m0 += 2) {
 #pragma unroll
           for (int m = m0; m < m0 + 2; ++m) {
-            float a_scale[16];
-            if constexpr (SCALED) {
-#pragma unroll
-              for (int r = 0; r < 16; ++r) {
-                const int row = wm + 32 * m + 8 * (r >> 2) + 4 * half + (r & 3);
-                a_scale[r] = as_float(
-                    __builtin_amdgcn_raw_buffer_load_b32(rs, (int)((uint32_t)row * 4 | (row < rows ? 0 : kNowhere)), 0, 0));
-              }
-            }
+            const int at_row = wm + 32 * m + j, strip_row = 32 * (m - m0) + j;
+            const float a_scale = SCALED && at_row < rows ? e.a_scale[k.i0 + at_row] : 0.f;
 #pragma unroll
             for (int n = 0; n < 2; ++n)
 #pragma unroll
-              for (int r = 0; r < 16; ++r) {
-                float v = acc[m][n][r];
-                if constexpr (SCALED) v *= a_scale[r] * scale[n];
-                if constexpr (!PLAIN) v = activate<decltype(act)::kind>(v + bias[n]);
-                half_strip[(32 * (m - m0) + 8 * (r >> 2) + 4 * half + (r & 3)) * kStripBf16 + 32 * n + j] = (uint16_t)bf16_bits(v);
+              for (int q = 0; q < 4; ++q) {
+                float v[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  v[i] = acc[m][n][4 * q + i];
+                  if constexpr (SCALED) v[i] *= a_scale * scale[n][q][i];
+                  if constexpr (!PLAIN) v[i] = activate<decltype(act)::kind>(v[i] + bias[n][q][i]);
+                }
+                *(__attribute__((address_space(3))) u32x2*)(half_strip + strip_row * 128 +
+                                                            (((4 * n + q) ^ (strip_row / 2 % 8)) << 4) + 8 * half) =
+                    u32x2{bf16_bits(v[0]) | bf16_bits(v[1]) << 16, bf16_bits(v[2]) | bf16_bits(v[3]) << 16};
               }
           }
           __builtin_amdgcn_wave_barrier();
 #pragma unroll
           for (int p = 0; p < 8; ++p) {
-            const int row = wm + 32 * m0 + 8 * p + sub;
-            const u32x4 v = *(const __attribute__((address_space(3))) u32x4*)(half_strip + (8 * p + sub) * kStripBf16 + 8 * (lane & 7));
+            const int strip_row = 8 * p + sub, row = wm + 32 * m0 + strip_row;
+            const u32x4 v = *(const __attribute__((address_space(3))) u32x4*)(half_strip + strip_row * 128 +
+                                                                              (((lane & 7) ^ (strip_row / 2 % 8)) << 4));
             __builtin_amdgcn_raw_buffer_store_b128(
                 v, ro, (int)(((uint32_t)row * (uint32_t)e.n + (uint32_t)at_col) * 2 | (row < rows ? 0 : kNowhere) | nowhere), 0, 0);
           }

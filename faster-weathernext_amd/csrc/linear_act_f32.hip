@@ -169,7 +169,7 @@ __global__ void __launch_bounds__(256, OA || OB ? 2 : 3) product_f32_kernel(Prod
 #pragma unroll
         for (int m = 0; m < 2; ++m)
 #pragma unroll
-          for (int n = 0; n < 2; ++n) acc[m][n] = mfma_bf16(fa[pa[i]][m], fb[pb[i]][n], acc[m][n]);
+          for (int n = 0; n < 2; ++n) acc[m][n] = mfma_bf16(fb[pb[i]][n], fa[pa[i]][m], acc[m][n]);
     }
   }
   __syncthreads();
