@@ -49,9 +49,10 @@ constexpr int kStageF32 = 32;     // k of a stage of float32 operands
 
 enum class Operands { kInnerInner, kInnerOuter, kOuterOuter };  // how a and b lie
 
-// One product, by tiles of 256 x 256 or 128 x 128 (float32: the latter). Of e4m3 operands kInnerInner alone.
+// One product, by tiles of 256 x 256 or 128 x 128 (float32: 128 x 128, or 64 x 128 of an inner a). Of e4m3 operands
+// kInnerInner alone.
 hipError_t launch_product(Operands how, int32_t op, int tile, const ProductArgs& a, hipStream_t stream);
-hipError_t launch_product_f32(Operands how, const ProductArgs& a, hipStream_t stream);
+hipError_t launch_product_f32(Operands how, int tile, const ProductArgs& a, hipStream_t stream);
 // One product of inner operands with at most kFewRows rows of a, unsplit.
 hipError_t launch_product_rows(int32_t op, const ProductArgs& a, hipStream_t stream);
 constexpr int64_t kFewRows = 32;

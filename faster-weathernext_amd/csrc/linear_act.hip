@@ -273,7 +273,7 @@ hipError_t launch_operands(int tile, const ProductArgs& g, hipStream_t stream) {
 }  // namespace
 
 hipError_t launch_product(Operands how, int32_t op, int tile, const ProductArgs& a, hipStream_t stream) {
-  if (op == kOpF32) return launch_product_f32(how, a, stream);
+  if (op == kOpF32) return launch_product_f32(how, tile, a, stream);
   if (op == kOpE4m3) return launch_operands<false, false, true>(tile, a, stream);
   if (how == Operands::kInnerInner) return launch_operands<false, false, false>(tile, a, stream);
   if (how == Operands::kInnerOuter) return launch_operands<false, true, false>(tile, a, stream);

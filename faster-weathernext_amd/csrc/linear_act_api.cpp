@@ -130,19 +130,19 @@ struct Plan {
 };
 
 struct Cost {
-  int tile;
+  int tile;  // rows, and columns (128 at least)
   double alone, full, ends;  // a stage of the one workgroup on a CU, of one among those that fill it, a workgroup's ends
 };
 
-Plan plan(int64_t m, int64_t n, int64_t k, int32_t op) {
-  constexpr Cost bf16[] = {{256, 1.55, 1.55, 9.0}, {128, 0.6, 0.5, 1.8}}, f32[] = {{128, 2.0, 1.1, 3.0}};
+Plan plan(Operands how, int64_t m, int64_t n, int64_t k, int32_t op) {
+  constexpr Cost bf16[] = {{256, 1.55, 1.55, 9.0}, {128, 0.6, 0.5, 1.8}}, f32[] = {{128, 2.0, 1.1, 3.0}, {64, 1.1, 0.66, 2.0}};
   const int64_t of = op == kOpF32 ? kStageF32 : op == kOpE4m3 ? kStageBytes : kStageRows;
   const int64_t stages = std::max<int64_t>(1, parts(k, of));
   Plan best{128, 1, (int32_t)stages};
   double least = -1;
-  for (int t = 0; t < (op == kOpF32 ? 1 : 2); ++t) {
+  for (int t = 0; t < (op == kOpF32 && how == Operands::kOuterOuter ? 1 : 2); ++t) {
     const Cost& c = op == kOpF32 ? f32[t] : bf16[t];
-    const int64_t tiles = parts(m, c.tile) * parts(n, c.tile);
+    const int64_t tiles = parts(m, c.tile) * parts(n, std::max(c.tile, 128));
     for (int64_t want = 1; want <= 64; ++want) {
       const int64_t chunk = parts(stages, want), splits = parts(stages, chunk);
       if (splits != want) continue;
@@ -171,7 +171,7 @@ struct Product {
   void shape(Operands h, int64_t m, int64_t n, int64_t k, int32_t o, bool sums, Workspace& ws) {
     how = h, op = o;
     few = how == Operands::kInnerInner && m <= kFewRows;
-    p = few ? Plan{0, 1, 0} : plan(m, n, k, op);
+    p = few ? Plan{0, 1, 0} : plan(how, m, n, k, op);
     g.k = k;
     g.splits = p.splits;
     g.chunk = p.chunk;

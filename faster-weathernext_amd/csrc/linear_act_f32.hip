@@ -8,25 +8,28 @@
 // A workgroup is 4 waves on a 128 x 128 tile, a wave 64 x 64: per 16 k it reads 12 KB of LDS for 24 MFMAs. One
 // stage of 32 k is 48 KB of parts, so that two or three workgroups share a CU: while one splits and writes its next
 // stage, loaded a stage ahead into registers, the others multiply. A stage takes 2.0 us alone on a CU and 1.1 among
-// others. 8 waves with two stages in LDS, a wave splitting the next between its products, were quicker where
-// tiles are few (2,562 x 515 -> 1027: 34 us against 42), but slower where they fill the chip (10,242 x 768 -> 3072:
-// 348 against 290), for the two waves of a SIMD then split at the same time.
+// others (4,096 x 4,096 -> 4,096: 210 TFLOP/s). Where such tiles are too few, an inner a is taken in tiles of 64 x 128, of 1.1 us a
+// stage alone and 0.66 among others, us with 128 rows and with 64: 1,000 x 512 -> 512 22 and 17, 2,562 x 515 -> 1,027 43
+// and 36, 130 x 1,024 -> 1,024 16 and 13; 10,242 x 768 -> 3,072 260 and 286. Two stages in LDS (a stage split between the products
+// of the one before) were slower where tiles fill the chip: 337.
 #include "linear_act_device.h"
 
 namespace fwn {
 namespace {
 
-constexpr int TILE = 128, STEP = 32, PLANE = TILE * STEP * 2, OPERAND = 3 * PLANE;
+constexpr int TILE = 128, STEP = 32;
 
-// One operand's stages: 128 rows of 32 k ("inner") or 32 rows of k of 128 columns ("outer"), 16 values a thread.
-// In LDS a part is 128 rows of 64 bytes or 32 of 256, 16-byte chunks swizzled as for the bf16 kernels.
-template <bool OUTER>
+// One operand's stages: ROWS rows of 32 k ("inner") or 32 rows of k of 128 columns ("outer"), 4 FOURS values a thread.
+// In LDS a part is ROWS rows of 64 bytes or 32 of 256, 16-byte chunks swizzled as for the bf16 kernels.
+template <bool OUTER, int ROWS>
 struct Operand {
+  static constexpr int FOURS = ROWS / 32, PLANE = ROWS * STEP * 2, BYTES = 3 * PLANE;
+  static_assert(!OUTER || ROWS == 128, "outer operands have 128 columns");
   const char* base;
   int64_t step;      // bytes from one stage to the next
-  uint32_t off[4];   // of this thread's four fours of values
-  uint32_t lds[4];
-  int first_k[4];    // k of a four in the stage
+  uint32_t off[FOURS];   // of this thread's fours of values
+  uint32_t lds[FOURS];
+  int first_k[FOURS];    // k of a four in the stage
   int limit;         // outer: columns of the fours inside the operand
   bool whole;        // fours do not end inside: of the sum (inner), or of the tile's columns (outer)
   uint32_t at[OUTER ? 4 : 2];  // this lane's reads
@@ -35,11 +38,11 @@ struct Operand {
                                        int lane) {
     base = p + (OUTER ? first * 4 : first * stride);
     step = OUTER ? STEP * stride : STEP * 4;
-    whole = OUTER ? rows % 4 == 0 || first + TILE <= rows : k % 4 == 0;
+    whole = OUTER ? rows % 4 == 0 || first + ROWS <= rows : k % 4 == 0;
     const int t = (int)threadIdx.x;
     limit = 4;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < FOURS; ++i) {
       if constexpr (OUTER) {
         const int row = t / 32 + 8 * i, col = t % 32 * 4;
         off[i] = first + col < rows ? (uint32_t)row * (uint32_t)stride + (uint32_t)col * 4 : kNowhere;
@@ -72,14 +75,14 @@ struct Operand {
 
   // Stage t's values; `left`: k from its first to the sum's end (what lies past it is zeros). Fours need no alignment
   // but their elements'.
-  __device__ __forceinline__ void load(int64_t t, int64_t left, u32x4 (&v)[4]) const {
+  __device__ __forceinline__ void load(int64_t t, int64_t left, u32x4 (&v)[FOURS]) const {
     const rsrc_t r = make_rsrc(base + t * step, kBuffer);
     if (whole || (!OUTER && left >= STEP)) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = bload16(r, off[i] | (first_k[i] < left ? 0 : kNowhere));
+      for (int i = 0; i < FOURS; ++i) v[i] = bload16(r, off[i] | (first_k[i] < left ? 0 : kNowhere));
     } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < FOURS; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const bool in = OUTER ? e < limit && first_k[i] < left : first_k[i] + e < left;
@@ -89,9 +92,9 @@ struct Operand {
   }
 
   // Their parts to LDS. An infinity or NaN gives NaN in the middle part, and so in every output that it feeds.
-  __device__ __forceinline__ void split(lds_char* to, const u32x4 (&v)[4]) const {
+  __device__ __forceinline__ void split(lds_char* to, const u32x4 (&v)[FOURS]) const {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < FOURS; ++i) {
       uint32_t part[3][4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -119,27 +122,31 @@ struct Operand {
   }
 };
 
-template <bool OA, bool OB>
+// A tile of BM x 128: a wave has BM / 2 x 64 of it.
+template <bool OA, bool OB, int BM>
 __global__ void __launch_bounds__(256, OA || OB ? 2 : 3) product_f32_kernel(ProductArgs g) {
-  __shared__ __align__(256) char lds[2 * OPERAND];
+  typedef Operand<OA, BM> A;
+  typedef Operand<OB, TILE> B;
+  constexpr int MI = BM / 64;
+  __shared__ __align__(256) char lds[A::BYTES + B::BYTES];
   static_assert(sizeof(lds) >= 4 * kStripBytes, "the waves' strips");
   lds_char* const sa = (lds_char*)lds;
-  lds_char* const sb = sa + OPERAND;
+  lds_char* const sb = sa + A::BYTES;
   const int lane = (int)threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const Work k = work_of<TILE, TILE>(g.e);
+  const Work k = work_of<BM, TILE>(g.e);
   const int64_t stages = (g.k + STEP - 1) / STEP, t0 = (int64_t)k.split * g.chunk;
   const int64_t t1 = t0 + g.chunk < stages ? t0 + g.chunk : stages;
-  const int wm = w / 2 * 64, wn = w % 2 * 64;
-  Operand<OA> a;
-  Operand<OB> b;
+  const int wm = w / 2 * (BM / 2), wn = w % 2 * 64;
+  A a;
+  B b;
   a.init(g.a, g.a_stride, k.i0, g.e.m, g.k, wm, lane);
   b.init(g.b, g.b_stride, k.j0, g.e.n, g.k, wn, lane);
-  f32x16 acc[2][2];
+  f32x16 acc[MI][2];
 #pragma unroll
-  for (int m = 0; m < 2; ++m)
+  for (int m = 0; m < MI; ++m)
 #pragma unroll
     for (int n = 0; n < 2; ++n) acc[m][n] = zero16();
-  u32x4 va[4], vb[4];
+  u32x4 va[A::FOURS], vb[B::FOURS];
   if (t0 < t1) {
     a.load(t0, g.k - t0 * STEP, va);
     b.load(t0, g.k - t0 * STEP, vb);
@@ -155,25 +162,25 @@ __global__ void __launch_bounds__(256, OA || OB ? 2 : 3) product_f32_kernel(Prod
     lds_barrier();
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      u32x4 fa[3][2], fb[3][2];
+      u32x4 fa[3][MI], fb[3][2];
 #pragma unroll
-      for (int p = 2; p >= 0; --p)
+      for (int p = 2; p >= 0; --p) {
 #pragma unroll
-        for (int m = 0; m < 2; ++m) {
-          fa[p][m] = a.read(sa + p * PLANE, m, c);
-          fb[p][m] = b.read(sb + p * PLANE, m, c);
-        }
+        for (int m = 0; m < MI; ++m) fa[p][m] = a.read(sa + p * A::PLANE, m, c);
+#pragma unroll
+        for (int n = 0; n < 2; ++n) fb[p][n] = b.read(sb + p * B::PLANE, n, c);
+      }
       constexpr int pa[6] = {2, 0, 1, 1, 0, 0}, pb[6] = {0, 2, 1, 0, 1, 0};
 #pragma unroll
       for (int i = 0; i < 6; ++i)
 #pragma unroll
-        for (int m = 0; m < 2; ++m)
+        for (int m = 0; m < MI; ++m)
 #pragma unroll
           for (int n = 0; n < 2; ++n) acc[m][n] = mfma_bf16(fb[pb[i]][n], fa[pa[i]][m], acc[m][n]);
     }
   }
   __syncthreads();
-  write_tile<TILE, 2, OB, 1, false>(g, k, acc, (strip_ptr)(sa + w * kStripBytes), wm, wn, lane, MendParts<OA, OB>{g});
+  write_tile<BM, MI, OB, 1, false>(g, k, acc, (strip_ptr)(sa + w * kStripBytes), wm, wn, lane, MendParts<OA, OB>{g});
 }
 
 template <bool OA, bool OB, int N>
@@ -181,10 +188,10 @@ __global__ void __launch_bounds__(256) join_f32_kernel(ProductArgs g) {
   join<OB, N>(g, MendParts<OA, OB>{g});
 }
 
-template <bool OA, bool OB>
+template <bool OA, bool OB, int BM = TILE>
 hipError_t launch(const ProductArgs& g, hipStream_t stream) {
-  const int64_t tiles = ((g.e.m + TILE - 1) / TILE) * ((g.e.n + TILE - 1) / TILE);
-  hipLaunchKernelGGL((product_f32_kernel<OA, OB>), dim3((unsigned)(tiles * g.splits)), dim3(256), 0, stream, g);
+  const int64_t tiles = ((g.e.m + BM - 1) / BM) * ((g.e.n + TILE - 1) / TILE);
+  hipLaunchKernelGGL((product_f32_kernel<OA, OB, BM>), dim3((unsigned)(tiles * g.splits)), dim3(256), 0, stream, g);
   if (hipError_t e = hipGetLastError(); e != hipSuccess || !g.part) return e;
   if (g.e.vec)
     hipLaunchKernelGGL((join_f32_kernel<OA, OB, 8>), join_grid(g), dim3(256), 0, stream, g);
@@ -195,9 +202,9 @@ hipError_t launch(const ProductArgs& g, hipStream_t stream) {
 
 }  // namespace
 
-hipError_t launch_product_f32(Operands how, const ProductArgs& g, hipStream_t stream) {
-  if (how == Operands::kInnerInner) return launch<false, false>(g, stream);
-  if (how == Operands::kInnerOuter) return launch<false, true>(g, stream);
+hipError_t launch_product_f32(Operands how, int tile, const ProductArgs& g, hipStream_t stream) {
+  if (how == Operands::kInnerInner) return tile == 64 ? launch<false, false, 64>(g, stream) : launch<false, false>(g, stream);
+  if (how == Operands::kInnerOuter) return tile == 64 ? launch<false, true, 64>(g, stream) : launch<false, true>(g, stream);
   return launch<true, true>(g, stream);
 }
 
