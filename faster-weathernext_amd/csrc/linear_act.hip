@@ -227,6 +227,8 @@ __global__ void __launch_bounds__((threads_of(BM)), 2) product_kernel(ProductArg
     step(s0, s1);
     step(s1, s0);
   }
+  Bf16Terms<MI, OB, E4M3> terms;
+  if (bf16_rows<OB>(g)) terms.load(g.e, k, (int)(g.e.m - k.i0 < BM ? g.e.m - k.i0 : BM), wm, wn, lane);
   wait_vmem();  // no copy outlives the stages
   __syncthreads();
 
@@ -244,7 +246,7 @@ __global__ void __launch_bounds__((threads_of(BM)), 2) product_kernel(ProductArg
   }
   constexpr int PER = WAVES / 2;  // waves whose strips share a stage's array
   write_tile<BM, MI, OB, E4M3 ? -1 : 0, E4M3>(g, k, acc, (strip_ptr)((w < PER ? s0 : s1) + (w % PER) * kStripBytes), wm, wn,
-                                              lane, MendNothing());
+                                              lane, terms, MendNothing());
 }
 
 template <bool PLAIN, int N>

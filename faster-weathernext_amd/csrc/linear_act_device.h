@@ -200,6 +200,42 @@ constexpr int kStrip = 72;                      // floats from one row of a stri
 constexpr int kStripBytes = 32 * kStrip * 4;    // of LDS, for each wave
 static_assert(kStripBytes >= 64 * 128, "a strip of 64 rows of bf16, chunk c of row r at c ^ (r / 2 % 8)");
 
+// Whether a product's outputs are bf16 that nothing but their column's bias is added to, in rows of whole aligned eights.
+template <bool PLAIN>
+__device__ __forceinline__ bool bf16_rows(const ProductArgs& g) {
+  return !g.part && g.e.vec && g.e.dtype == FWN_BF16 && (PLAIN || (!g.e.pre && !g.e.residual));
+}
+
+// What the epilogue of those needs of memory for a wave's part, in the layout of its registers: asked for before the last
+// barrier, and before the stores, which a later load would wait for.
+template <int MI, bool PLAIN, bool SCALED>
+struct Bf16Terms {
+  u32x2 bias[2][4];
+  u32x4 scale[2][4];
+  float a_scale[MI];
+
+  __device__ __forceinline__ void load(const EpilogueArgs& e, const Work& k, int rows, int wm, int wn, int lane) {
+    const int j = lane & 31, half = lane >> 5;
+    if constexpr (!PLAIN) {
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int64_t col = k.j0 + wn + 32 * n + 8 * q + 4 * half;
+          bias[n][q] = e.bias && col < e.n ? *(const bf16x4_any*)((const uint16_t*)e.bias + col) : u32x2{0, 0};
+          if constexpr (SCALED) scale[n][q] = col < e.n ? *(const f32x4_any*)(e.b_scale + col) : u32x4{0, 0, 0, 0};
+        }
+    }
+    if constexpr (SCALED) {
+#pragma unroll
+      for (int m = 0; m < MI; ++m) {
+        const int row = wm + 32 * m + j;
+        a_scale[m] = row < rows ? e.a_scale[k.i0 + row] : 0.f;
+      }
+    }
+  }
+};
+
 // The epilogue of a wave's 32 MI x 64 part (from row wm and column wn) of a BM-row tile. The products are formed with
 // the weight's side as the MFMA's rows, so that a lane's registers are fours of columns of one row (acc[m][n][4 q + i]:
 // row 32 m + lane % 32, column 32 n + 8 q + 4 (lane / 32) + i), which go to LDS whole (gx of 10,242 x 768 with 3,072
@@ -210,7 +246,7 @@ static_assert(kStripBytes >= 64 * 128, "a strip of 64 rows of bf16, chunk c of r
 // right outputs before the epilogue.
 template <int BM, int MI, bool PLAIN, int F32, bool SCALED, typename Mend>
 __device__ __forceinline__ void write_tile(const ProductArgs& g, const Work& k, const f32x16 (&acc)[MI][2], strip_ptr strip,
-                                           int wm, int wn, int lane, const Mend& mend) {
+                                           int wm, int wn, int lane, const Bf16Terms<MI, PLAIN, SCALED>& terms, const Mend& mend) {
   const int j = lane & 31, half = lane >> 5;
   const auto to_strip = [&](int m) {
 #pragma unroll
@@ -224,26 +260,10 @@ __device__ __forceinline__ void write_tile(const ProductArgs& g, const Work& k, 
   const EpilogueArgs& e = g.e;
   const int rows = (int)(e.m - k.i0 < BM ? e.m - k.i0 : BM);  // of the tile
   if constexpr (F32 != 1) {
-    if (!g.part && e.vec && e.dtype == FWN_BF16 && (PLAIN || (!e.pre && !e.residual))) {
+    if (bf16_rows<PLAIN>(g)) {
       static_assert(MI % 2 == 0, "64 rows at a time");
       typedef __attribute__((address_space(3))) char* bytes_ptr;
       bytes_ptr const half_strip = (bytes_ptr)strip;
-      // This lane's columns are fours: 32 n + 8 q + 4 half.
-      float bias[2][4][4], scale[2][4][4];
-      if constexpr (!PLAIN) {
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const int64_t col = k.j0 + wn + 32 * n + 8 * q + 4 * half;
-            const u32x2 u = e.bias && col < e.n ? *(const bf16x4_any*)((const uint16_t*)e.bias + col) : u32x2{0, 0};
-            const u32x4 v = SCALED && col < e.n ? *(const f32x4_any*)(e.b_scale + col) : u32x4{0, 0, 0, 0};
-            const uint32_t lo = u[0], hi = u[1], v0 = v[0], v1 = v[1], v2 = v[2], v3 = v[3];
-            bias[n][q][0] = as_float(lo << 16), bias[n][q][1] = as_float(lo & 0xffff0000u);
-            bias[n][q][2] = as_float(hi << 16), bias[n][q][3] = as_float(hi & 0xffff0000u);
-            scale[n][q][0] = as_float(v0), scale[n][q][1] = as_float(v1), scale[n][q][2] = as_float(v2), scale[n][q][3] = as_float(v3);
-          }
-      }
       const rsrc_t ro = make_rsrc((char*)e.out + (k.i0 * e.n + k.j0) * 2, kBuffer);
       const int sub = lane >> 3, at_col = wn + 8 * (lane & 7);
       const uint32_t nowhere = k.j0 + at_col < e.n ? 0 : kNowhere;
@@ -252,8 +272,7 @@ __device__ __forceinline__ void write_tile(const ProductArgs& g, const Work& k, 
         for (int m0 = 0; m0 < MI; m0 += 2) {
 #pragma unroll
           for (int m = m0; m < m0 + 2; ++m) {
-            const int at_row = wm + 32 * m + j, strip_row = 32 * (m - m0) + j;
-            const float a_scale = SCALED && at_row < rows ? e.a_scale[k.i0 + at_row] : 0.f;
+            const int strip_row = 32 * (m - m0) + j;
 #pragma unroll
             for (int n = 0; n < 2; ++n)
 #pragma unroll
@@ -262,8 +281,14 @@ __device__ __forceinline__ void write_tile(const ProductArgs& g, const Work& k, 
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                   v[i] = acc[m][n][4 * q + i];
-                  if constexpr (SCALED) v[i] *= a_scale * scale[n][q][i];
-                  if constexpr (!PLAIN) v[i] = activate<decltype(act)::kind>(v[i] + bias[n][q][i]);
+                  if constexpr (SCALED) {
+                    const uint32_t u = terms.scale[n][q][i];
+                    v[i] *= terms.a_scale[m] * as_float(u);
+                  }
+                  if constexpr (!PLAIN) {
+                    const uint32_t u = terms.bias[n][q][i / 2];
+                    v[i] = activate<decltype(act)::kind>(v[i] + as_float(i % 2 ? u & 0xffff0000u : u << 16));
+                  }
                 }
                 *(__attribute__((address_space(3))) u32x2*)(half_strip + strip_row * 128 +
                                                             (((4 * n + q) ^ (strip_row / 2 % 8)) << 4) + 8 * half) =

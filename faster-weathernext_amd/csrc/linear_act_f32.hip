@@ -180,7 +180,8 @@ __global__ void __launch_bounds__(256, OA || OB ? 2 : 3) product_f32_kernel(Prod
     }
   }
   __syncthreads();
-  write_tile<BM, MI, OB, 1, false>(g, k, acc, (strip_ptr)(sa + w * kStripBytes), wm, wn, lane, MendParts<OA, OB>{g});
+  write_tile<BM, MI, OB, 1, false>(g, k, acc, (strip_ptr)(sa + w * kStripBytes), wm, wn, lane, {},
+                                    MendParts<OA, OB>{g});
 }
 
 template <bool OA, bool OB, int N>
