@@ -549,3 +549,40 @@ def test_offsets_past_32_bits(dtype):
   assert torch.equal(gx[at], (g[at].double() @ w.double()).to(dtype))
   cols = [0, 100, ins - 1]
   assert torch.equal(gw[:, cols], (g.double().t() @ x.detach()[:, cols].double()).to(dtype))
+
+
+@gpu
+def test_the_same_tensor_twice():
+  """One tensor as x, weight and residual: small whole numbers, so that every sum is exact in float32."""
+  for n in (24, 130):
+    x = _leaf(_whole((n, n), torch.float32, 1))
+    g = _whole((n, n), torch.float32, 2)
+    out = fwn.linear_act(x, x, residual=x)
+    gx, = torch.autograd.grad(out, x, g)
+    d, e = x.detach().double(), g.double()
+    assert torch.equal(out.double(), d @ d.t() + d)
+    assert torch.equal(gx.double(), e @ d + e.t() @ d + e)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_two_streams_at_once(dtype):
+  """Calls on two streams that may overlap, with split sums and operands laid out: the results of one after the other."""
+  sizes = [(70, 2048, 64), (600, 100, 130), (24, 1030, 200), (300, 640, 512)]
+  calls = []
+  for k, (rows, ins, outs) in enumerate(sizes):
+    x, w, b = _leaf(_whole((rows, ins), dtype, k)), _leaf(_whole((outs, ins), dtype, k + 10)), _leaf(_whole((outs,), dtype, k + 20))
+    g = _whole((rows, outs), dtype, k + 30)
+    calls.append(lambda x=x, w=w, b=b, g=g: [*torch.autograd.grad(fwn.linear_act(x, w, b, activation="silu"), (x, w, b), g),
+                                             fwn.linear_act(x.detach(), w.detach(), b.detach())])
+  want = [call() for call in calls]
+  torch.cuda.synchronize()
+  streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], {}
+  for repeat in range(3):
+    for k, call in enumerate(calls):
+      with torch.cuda.stream(streams[(k + repeat) % 2]):
+        got[repeat, k] = call()
+  torch.cuda.synchronize()
+  for (repeat, k), outs in got.items():
+    for p, q in zip(outs, want[k]):
+      assert torch.equal(p, q), (repeat, sizes[k])
