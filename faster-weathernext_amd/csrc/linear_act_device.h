@@ -325,12 +325,26 @@ __device__ __forceinline__ void write_tile(const ProductArgs& g, const Work& k, 
     const uint32_t nowhere = col < e.n ? 0 : kNowhere;
     Columns c;
     if (!PLAIN && !g.part) c.load(e, col);
-    const auto load = [&](rsrc_t r, uint32_t o, float(&f)[8]) {
-      const u32x4 lo = bload16(r, o), hi = f32 ? bload16(r, o + 16) : lo;
+    // The residual of 32 rows is asked for before the stores of the 32 before them, which a later load would wait for (where
+    // registers allow it).
+    constexpr bool AHEAD = F32 != -1;
+    const bool wide = F32 == 1 || (F32 == -1 && e.dtype == FWN_F32);
+    u32x4 next[AHEAD ? 2 : 1][4][2];
+    const auto ask = [&](int m) {
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        const int row = wm + 32 * m + 8 * p + sub;
+        const uint32_t o = (row < rows ? 0 : kNowhere) | nowhere | (((uint32_t)row * (uint32_t)e.r_row + (uint32_t)at_col) << shift);
+        next[AHEAD ? m & 1 : 0][p][0] = bload16(rr, o);
+        if (wide) next[AHEAD ? m & 1 : 0][p][1] = bload16(rr, o + 16);
+      }
+    };
+    const auto asked = [&](int m, int p, float(&f)[8]) {
+      const u32x4 lo = next[AHEAD ? m & 1 : 0][p][0], hi = next[AHEAD ? m & 1 : 0][p][1];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const uint32_t x = lo[i], y = hi[i];
-        if (f32) {
+        if (wide) {
           f[i] = as_float(x);
           f[4 + i] = as_float(y);
         } else {
@@ -347,17 +361,18 @@ __device__ __forceinline__ void write_tile(const ProductArgs& g, const Work& k, 
         __builtin_amdgcn_raw_buffer_store_b128(pack8(f), r, (int)o, 0, 0);
       }
     };
+    if (AHEAD && residual) ask(0);
     with_activation<PLAIN>(g.part ? FWN_ACT_NONE : e.activation, [&](auto act) {
 #pragma unroll
       for (int m = 0; m < MI; ++m) {
         to_strip(m);
+        if (residual && m + AHEAD < MI) ask(m + AHEAD);
 #pragma unroll
         for (int p = 0; p < 4; ++p) {
           const int row = wm + 32 * m + 8 * p + sub;
           const uint32_t out = (row < rows ? 0 : kNowhere) | nowhere;
           const uint32_t o = out | (((uint32_t)row * (uint32_t)width + (uint32_t)at_col) << shift);
-          float v[8], r[8];
-          if (residual) load(rr, out | (((uint32_t)row * (uint32_t)e.r_row + (uint32_t)at_col) << shift), r);
+          float v[8];
           const auto* q = (const __attribute__((address_space(3))) f32x4*)(strip + (8 * p + sub) * kStrip + 8 * (lane & 7));
           const f32x4 lo = q[0], hi = q[1];
 #pragma unroll
@@ -380,6 +395,8 @@ __device__ __forceinline__ void write_tile(const ProductArgs& g, const Work& k, 
 #pragma unroll
               for (int i = 0; i < 8; ++i) v[i] = activate<decltype(act)::kind>(v[i]);
               if (residual) {
+                float r[8];
+                asked(m, p, r);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) v[i] += r[i];
               }
