@@ -6,9 +6,10 @@
 // are contiguous in k ("inner": x, w and dz in the first two) is read from LDS row by row, one whose rows are k
 // ("outer": w in gx, dz and x in gw) by transpose reads, and both arrive as the same MFMA operands.
 //
-// Bound by the matrix units, and for short sums by what is not overlapped with them: 8,192 x 8,192 x 8,192 runs at 1,110 to 1,260 TFLOP/s in bf16 and 2,100 in e4m3; 40,962 x 768 -> 3,072 takes 204 us (950), 229 with bias and
-// GELU, 167 in e4m3 with both, of which the main loop has 160 and 92. One workgroup a CU (its two stages are 128 KB of
-// LDS, its sums half of the registers): 8 waves of 128 x 64 outputs, each operand byte in LDS read 2 and 4 times.
+// Bound by the matrix units, and for short sums by what is not overlapped with them: 8,192 x 8,192 x 8,192 runs at 1,110 to
+// 1,260 TFLOP/s in bf16 and 2,100 in e4m3; 40,962 x 768 -> 3,072 takes 204 us (950), 229 with bias and GELU, 167 in e4m3
+// with both, of which the main loop has 160 and 92. One workgroup a CU (its two stages are 128 KB of LDS, its sums half
+// of the registers): 8 waves of 128 x 64 outputs, so that a byte of a in LDS is read four times and one of b twice.
 #include "linear_act_device.h"
 
 namespace fwn {
