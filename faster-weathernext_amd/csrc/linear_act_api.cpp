@@ -134,7 +134,8 @@ struct Cost {
   double alone, full, ends;  // a stage of the one workgroup on a CU, of one among those that fill it, a workgroup's ends
 };
 
-Plan plan(Operands how, int64_t m, int64_t n, int64_t k, int32_t op) {
+// `widened`: e4m3 operands multiplied as bf16, twice the products of a stage of bf16.
+Plan plan(Operands how, int64_t m, int64_t n, int64_t k, int32_t op, bool widened) {
   constexpr Cost bf16[] = {{256, 1.55, 1.55, 9.0}, {128, 0.6, 0.5, 1.8}}, f32[] = {{128, 2.0, 1.1, 3.0}, {64, 1.1, 0.66, 2.0}};
   const int64_t of = op == kOpF32 ? kStageF32 : op == kOpE4m3 ? kStageBytes : kStageRows;
   const int64_t stages = std::max<int64_t>(1, parts(k, of));
@@ -149,7 +150,7 @@ Plan plan(Operands how, int64_t m, int64_t n, int64_t k, int32_t op) {
       if (want > 1 && (chunk < 2 || tiles * want > 4 * kCus)) break;
       const int64_t load = parts(tiles * splits, kCus);
       const double join = splits > 1 ? 4.0 + (double)(splits + 1) * m * n * 4 / 4e6 : 0;
-      const double time = load * (chunk * (load == 1 ? c.alone : c.full) + c.ends) + join;
+      const double time = load * (chunk * (load == 1 ? c.alone : c.full) * (widened ? 2 : 1) + c.ends) + join;
       if (least < 0 || time < least) {
         least = time;
         best = {c.tile, (int32_t)splits, (int32_t)chunk};
@@ -167,11 +168,11 @@ struct Product {
   Plan p;
   bool few;  // rows: no tiles
 
-  // `sums`: the column sums of a are wanted.
-  void shape(Operands h, int64_t m, int64_t n, int64_t k, int32_t o, bool sums, Workspace& ws) {
+  // `sums`: the column sums of a are wanted. `dtype`: of the outputs.
+  void shape(Operands h, int64_t m, int64_t n, int64_t k, int32_t o, int32_t dtype, bool sums, Workspace& ws) {
     how = h, op = o;
     few = how == Operands::kInnerInner && m <= kFewRows;
-    p = few ? Plan{0, 1, 0} : plan(how, m, n, k, op);
+    p = few ? Plan{0, 1, 0} : plan(how, m, n, k, op, op == kOpE4m3 && dtype == FWN_F32);
     g.k = k;
     g.splits = p.splits;
     g.chunk = p.chunk;
@@ -202,7 +203,7 @@ struct Forward {
     Workspace ws{(char*)workspace};
     x.place(xp, d->rows, d->ins, d->x_stride, op, ws);
     w.place(wp, d->outs, d->ins, d->w_stride, op, ws);
-    z.shape(Operands::kInnerInner, d->rows, d->outs, d->ins, op, false, ws);
+    z.shape(Operands::kInnerInner, d->rows, d->outs, d->ins, op, d->dtype, false, ws);
     bytes = ws.used;
   }
 };
@@ -271,11 +272,11 @@ struct Backward {
     if (need_b && !sums_in_product && slope.blocks > 1) slope.part = (float*)ws.take((uint64_t)slope.blocks * d->outs * sizeof(float));
     if (need_x) {
       w.place(wp, d->outs, d->ins, d->w_stride, op, ws);
-      to_x.shape(Operands::kInnerOuter, d->rows, d->ins, d->outs, op, false, ws);
+      to_x.shape(Operands::kInnerOuter, d->rows, d->ins, d->outs, op, d->dtype, false, ws);
     }
     if (need_w) {
       x.place(xp, d->rows, d->ins, d->x_stride, op, ws);
-      to_w.shape(Operands::kOuterOuter, d->outs, d->ins, d->rows, op, sums_in_product, ws);
+      to_w.shape(Operands::kOuterOuter, d->outs, d->ins, d->rows, op, d->dtype, sums_in_product, ws);
     }
     bytes = ws.used;
   }

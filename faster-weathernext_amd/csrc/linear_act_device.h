@@ -2,6 +2,8 @@
 // tile and the order of the tiles (gfx950).
 #pragma once
 
+#include <type_traits>
+
 #include "attn_bf16_tiles.h"
 #include "linear_act.h"
 
@@ -9,6 +11,7 @@ namespace fwn {
 namespace {
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 
 __device__ __forceinline__ float as_float(uint32_t u) { return __builtin_bit_cast(float, u); }
 __device__ __forceinline__ uint32_t as_bits(float f) { return __builtin_bit_cast(uint32_t, f); }
@@ -63,6 +66,14 @@ __device__ __forceinline__ void store8(void* p, int64_t i, int dtype, const floa
   } else {
     *(u32x4*)((uint16_t*)p + i) = pack8(f);
   }
+}
+
+// Eight e4m3 codes as the bf16 values that they are exactly.
+__device__ __forceinline__ u32x4 widen(uint32_t lo, uint32_t hi) {
+  const auto two = [](uint32_t codes, auto high) {
+    return __builtin_bit_cast(uint32_t, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, 1.f, decltype(high)::value));
+  };
+  return u32x4{two(lo, std::false_type()), two(lo, std::true_type()), two(hi, std::false_type()), two(hi, std::true_type())};
 }
 
 // e^x and 1 / x on the transcendental unit, within two units in the last place.
@@ -242,9 +253,9 @@ struct Bf16Terms {
 // outputs 62 us with single columns, 57 so): 32 rows at a time through the wave's strip to rows of eight columns a
 // lane, or of one column a lane where rows are not whole aligned eights. bf16 outputs that nothing but their column's
 // bias is added to are finished where the MFMAs leave them and go through LDS as bf16, 64 rows at a time. PLAIN: no
-// epilogue but the rounding (gradients). F32: 1 the outputs are float32, 0 bf16, -1 either. mend(row, col, v) may put
-// right outputs before the epilogue.
-template <int BM, int MI, bool PLAIN, int F32, bool SCALED, typename Mend>
+// epilogue but the rounding (gradients). F32: the outputs are float32, else bf16. mend(row, col, v) may put right outputs
+// before the epilogue.
+template <int BM, int MI, bool PLAIN, bool F32, bool SCALED, typename Mend>
 __device__ __forceinline__ void write_tile(const ProductArgs& g, const Work& k, const f32x16 (&acc)[MI][2], strip_ptr strip,
                                            int wm, int wn, int lane, const Bf16Terms<MI, PLAIN, SCALED>& terms, const Mend& mend) {
   const int j = lane & 31, half = lane >> 5;
@@ -259,7 +270,7 @@ __device__ __forceinline__ void write_tile(const ProductArgs& g, const Work& k, 
   };
   const EpilogueArgs& e = g.e;
   const int rows = (int)(e.m - k.i0 < BM ? e.m - k.i0 : BM);  // of the tile
-  if constexpr (F32 != 1) {
+  if constexpr (!F32) {
     if (bf16_rows<PLAIN>(g)) {
       static_assert(MI % 2 == 0, "64 rows at a time");
       typedef __attribute__((address_space(3))) char* bytes_ptr;
@@ -312,7 +323,7 @@ __device__ __forceinline__ void write_tile(const ProductArgs& g, const Work& k, 
   }
   if (g.part || e.vec) {
     // Offsets in the tile.
-    const bool f32 = g.part || F32 == 1 || (F32 == -1 && e.dtype == FWN_F32);
+    const bool f32 = g.part || F32;
     const int64_t width = g.part ? g.part_row : e.n;
     const uint32_t shift = f32 ? 2 : 1;
     char* const to = g.part ? (char*)(g.part + (int64_t)k.split * e.m * g.part_row) : (char*)e.out;
@@ -327,8 +338,7 @@ __device__ __forceinline__ void write_tile(const ProductArgs& g, const Work& k, 
     if (!PLAIN && !g.part) c.load(e, col);
     // The residual of 32 rows is asked for before the stores of the 32 before them, which a later load would wait for (where
     // registers allow it).
-    constexpr bool AHEAD = F32 != -1;
-    const bool wide = F32 == 1 || (F32 == -1 && e.dtype == FWN_F32);
+    constexpr bool AHEAD = F32 || !SCALED;
     u32x4 next[AHEAD ? 2 : 1][4][2];
     const auto ask = [&](int m) {
 #pragma unroll
@@ -336,7 +346,7 @@ __device__ __forceinline__ void write_tile(const ProductArgs& g, const Work& k, 
         const int row = wm + 32 * m + 8 * p + sub;
         const uint32_t o = (row < rows ? 0 : kNowhere) | nowhere | (((uint32_t)row * (uint32_t)e.r_row + (uint32_t)at_col) << shift);
         next[AHEAD ? m & 1 : 0][p][0] = bload16(rr, o);
-        if (wide) next[AHEAD ? m & 1 : 0][p][1] = bload16(rr, o + 16);
+        if (F32) next[AHEAD ? m & 1 : 0][p][1] = bload16(rr, o + 16);
       }
     };
     const auto asked = [&](int m, int p, float(&f)[8]) {
@@ -344,7 +354,7 @@ __device__ __forceinline__ void write_tile(const ProductArgs& g, const Work& k, 
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const uint32_t x = lo[i], y = hi[i];
-        if (wide) {
+        if (F32) {
           f[i] = as_float(x);
           f[4 + i] = as_float(y);
         } else {
@@ -413,13 +423,12 @@ __device__ __forceinline__ void write_tile(const ProductArgs& g, const Work& k, 
   const bool in = col < e.n;
   const float bias = !PLAIN && e.bias && in ? load_one(e.bias, col, e.dtype) : 0.f;
   const float scale = SCALED && in ? e.b_scale[col] : 1.f;
-  const bool f32 = F32 == 1 || (F32 == -1 && e.dtype == FWN_F32);
-  const uint32_t shift = f32 ? 2 : 1;
+  const uint32_t shift = F32 ? 2 : 1;
   const rsrc_t ro = make_rsrc((char*)e.out + ((k.i0 * e.n + k.j0) << shift), kBuffer);
   const rsrc_t rp = make_rsrc((char*)e.pre + ((k.i0 * e.n + k.j0) << shift), kBuffer);
   const rsrc_t rr = make_rsrc((const char*)e.residual + ((k.i0 * e.r_row + k.j0) << shift), kBuffer);
   const auto store = [&](rsrc_t r, uint32_t o, float v) {
-    if (f32)
+    if (F32)
       __builtin_amdgcn_raw_buffer_store_b32(as_bits(v), r, (int)o, 0, 0);
     else
       __builtin_amdgcn_raw_buffer_store_b16((uint16_t)bf16_bits(v), r, (int)o, 0, 0);
@@ -439,7 +448,7 @@ __device__ __forceinline__ void write_tile(const ProductArgs& g, const Work& k, 
           res[r] = 0.f;
           if (!PLAIN && e.residual) {
             const uint32_t o = out[r] | (((uint32_t)row * (uint32_t)e.r_row + (uint32_t)(wn + lane)) << shift);
-            res[r] = f32 ? as_float(__builtin_amdgcn_raw_buffer_load_b32(rr, (int)o, 0, 0))
+            res[r] = F32 ? as_float(__builtin_amdgcn_raw_buffer_load_b32(rr, (int)o, 0, 0))
                          : as_float((uint32_t)__builtin_amdgcn_raw_buffer_load_b16(rr, (int)o, 0, 0) << 16);
           }
           z[r] = strip[(r0 + r) * kStrip + lane];

@@ -5,7 +5,8 @@
 // workgroup has 16 or 32 outputs, its waves share the sum, 128 bytes of each of the weight's rows at a time. A
 // wave loads its operands straight into registers in the MFMA's layout (16 rows of 64 bytes an instruction; the
 // order of k in a line does not matter as long as both operands have the same) and keeps several lines on
-// their way; the waves' sums meet in LDS. float32 operands use float32 MFMAs: their rate is not what bounds this.
+// their way; the waves' sums meet in LDS. float32 operands use float32 MFMAs, e4m3 ones are widened to bf16, which adds
+// in float32 (linear_act.hip): the matrix units' rate is not what bounds this.
 #include "linear_act_device.h"
 
 namespace fwn {
@@ -41,16 +42,16 @@ struct Rows {
 // c += a b over the k of one line: both pieces of both operands.
 template <int OP>
 __device__ __forceinline__ f32x4 multiply(const u32x4 (&a)[2], const u32x4 (&b)[2], f32x4 c) {
-  if constexpr (OP == kOpE4m3) {
-    const auto join = [](const u32x4(&x)[2]) {
-      return i32x8{(int)x[0][0], (int)x[0][1], (int)x[0][2], (int)x[0][3], (int)x[1][0], (int)x[1][1], (int)x[1][2], (int)x[1][3]};
-    };
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(join(a), join(b), c, 0, 0, 0, 0x7f7f7f7f, 0, 0x7f7f7f7f);
-  }
+  const auto bf16 = [&](const u32x4& x, const u32x4& y) {
+    c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, y), c, 0, 0, 0);
+  };
 #pragma unroll
   for (int p = 0; p < 2; ++p) {
-    if constexpr (OP == kOpBf16) {
-      c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a[p]), __builtin_bit_cast(bf16x8, b[p]), c, 0, 0, 0);
+    if constexpr (OP == kOpE4m3) {
+#pragma unroll
+      for (int h = 0; h < 4; h += 2) bf16(widen(a[p][h], a[p][h + 1]), widen(b[p][h], b[p][h + 1]));
+    } else if constexpr (OP == kOpBf16) {
+      bf16(a[p], b[p]);
     } else {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {

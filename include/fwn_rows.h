@@ -203,7 +203,9 @@ int fwn_linear_act_bwd_launch(const fwn_linear_desc* d, const void* x, const voi
 
 /* The forward of 8-bit operands: x and weight hold OCP e4m3 codes, z = (x weight^T) x_scale[row]
  * w_scale[column] + bias with float32 scales (fwn_rms_norm_q8_launch, fwn_quantize_rows_launch). The
- * descriptor's dtype is that of bias, residual and out. */
+ * descriptor's dtype is that of bias, residual and out. With FWN_F32, and of up to 32 rows, products are added in
+ * float32. With FWN_BF16 the e4m3 matrix units add them, eight at a time as multiples of 2^-13 of the largest one's
+ * power of two: off by less than 2^-10 of the sum of their magnitudes (random sums: 1.4e-5 of the rows' norms). */
 int fwn_linear_act_q8_workspace_size(const fwn_linear_desc* d, const uint8_t* x, const uint8_t* weight, uint64_t* bytes);
 int fwn_linear_act_q8_launch(const fwn_linear_desc* d, const uint8_t* x, const float* x_scale, const uint8_t* weight,
                              const float* w_scale, const void* bias, const void* residual, void* out,

@@ -1,0 +1,86 @@
+"""Sums and scales of ``linear_act_q8`` against float64.
+
+float32 outputs, and outputs of up to 32 rows in either type, are float32 sums of exact products: a sum of k
+products is off by at most (8 sqrt(k) + 16) 2^-24 |a| |b| (norms of the two rows; 2 / 3 sqrt(k) 2^-24 of
+them for the roundings of partial sums, twelve times that, and 16 for the epilogue). bf16 outputs of more rows
+come from the e4m3 matrix instructions, which add eight products as multiples of 2^-13 of the largest one's
+power of two, cut off: at most seven of the eight lose up to 2^-13 of the largest, together less than 2^-10
+of the sum of the products' magnitudes."""
+import pytest
+import torch
+
+import faster_weathernext_amd as fwn
+
+DEV = "cuda"
+gpu = pytest.mark.gpu
+E4M3 = torch.float8_e4m3fn
+
+
+def _gen(seed):
+  return torch.Generator().manual_seed(seed)
+
+
+def _normal(shape, seed, std=1.0):
+  return (torch.randn(shape, generator=_gen(seed)) * std).to(DEV)
+
+
+def _codes(shape, seed):
+  return _normal(shape, seed, 100).clamp(-448, 448).to(E4M3)
+
+
+def _sums(x, w):
+  return x.float().double() @ w.float().double().t()
+
+
+def _bound(x, w):
+  return (8 * x.shape[1] ** 0.5 + 16) * 2.0 ** -24 * x.float().double().norm(dim=1)[:, None] * w.float().double().norm(dim=1)
+
+
+@gpu
+@pytest.mark.parametrize("rows,ins,outs", [(1, 768, 1000), (24, 1040, 136), (24, 5120, 65), (33, 128, 128), (300, 515, 257),
+                                           (300, 5120, 72), (2000, 256, 512), (40, 16384, 64)])
+def test_float32_sums(rows, ins, outs):
+  x, w, one = _codes((rows, ins), 1), _codes((outs, ins), 2), lambda n: torch.ones(n, device=DEV)
+  want, bound = _sums(x, w), _bound(x, w)
+  got = fwn.linear_act_q8(x, one(rows), w, one(outs), dtype=torch.float32)
+  assert ((got.double() - want).abs() - bound).max() <= 0
+  low = fwn.linear_act_q8(x, one(rows), w, one(outs))
+  if rows > 32:
+    bound = 2.0 ** -10 * _sums(x.float().abs(), w.float().abs())
+  assert ((low.double() - want).abs() - 2.0 ** -8 * want.abs() - 1.01 * bound).max() <= 0
+
+
+@gpu
+@pytest.mark.parametrize("rows", [1, 24, 33, 300])
+def test_large_products_that_cancel(rows):
+  """448^2 - 448^2 + 1, and a product 2^-18 alone beside zeros: float32 sums have them exactly."""
+  x = torch.zeros(rows, 256, device=DEV)
+  w = torch.zeros(64, 256, device=DEV)
+  x[:, 0], x[:, 1], x[:, 2] = 448, 448, 1
+  w[:, 0], w[:, 1], w[:, 2] = 448, -448, 1
+  w[5] = 0
+  x[:, 3], w[5, 3] = 2.0 ** -9, 2.0 ** -9
+  want = torch.ones(rows, 64, device=DEV)
+  want[:, 5] = 2.0 ** -18
+  one = lambda n: torch.ones(n, device=DEV)
+  for dtype in (torch.float32,) if rows > 32 else (torch.float32, torch.bfloat16):
+    assert torch.equal(fwn.linear_act_q8(x.to(E4M3), one(rows), w.to(E4M3), one(64), dtype=dtype), want.to(dtype))
+
+
+@gpu
+@pytest.mark.parametrize("rows", [3, 300])
+def test_float32_epilogue(rows):
+  """Bias, activation and residual behind float32 sums, with rows that are not whole eights."""
+  for ins, outs in ((272, 64), (100, 65), (4096, 72)):
+    x, w = _codes((rows, ins), 1), _codes((outs, ins), 2)
+    xs, ws = (0.5 + _normal((n,), k).abs() for n, k in ((rows, 3), (outs, 4)))
+    xs, ws = xs / 1e4, ws / ins ** 0.5
+    b, r = _normal((outs,), 5), _normal((rows, outs), 6)
+    z = _sums(x, w) * xs.double()[:, None] * ws.double() + b.double()
+    e = _bound(x, w) * xs.double()[:, None] * ws.double() + 2.0 ** -22 * (z.abs() + b.double().abs())
+    for name, act in ((None, lambda t: t), ("relu", torch.relu), ("silu", torch.nn.functional.silu)):
+      want = act(z) + r.double()
+      got = fwn.linear_act_q8(x, xs, w, ws, b, activation=name, residual=r, dtype=torch.float32)
+      # Slopes stay below 1.1; the activation's own arithmetic within 2^-20 of z.
+      slack = 1.1 * e + 2.0 ** -20 * z.abs() + 2.0 ** -23 * (want.abs() + r.double().abs())
+      assert ((got.double() - want).abs() - slack).max() <= 0, (ins, outs, name)
