@@ -10,8 +10,9 @@ namespace fwn {
 
 enum : int32_t { kOpF32 = 0, kOpBf16 = 1, kOpE4m3 = 2 };  // element types of a product's operands
 
-// What happens to a product z[i, j]: z a_scale[i] b_scale[j] + bias[j], kept in pre, activated, the residual
-// added, stored in out. dtype is that of everything but the scales.
+// What happens to a product z[i, j]: z a_scale[i] b_scale[j] + bias[j] (in that order: the scales' own product may lie
+// out of float32's range), kept in pre, activated, the residual added, stored in out. dtype is that of everything but the
+// scales.
 struct EpilogueArgs {
   const float* a_scale;  // [m] and [n], or both null
   const float* b_scale;

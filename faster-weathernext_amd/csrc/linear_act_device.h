@@ -159,7 +159,7 @@ __device__ __forceinline__ void finish(const EpilogueArgs& e, int64_t row, int64
   if (e.a_scale) {
     const float s = e.a_scale[row];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] *= s * c.scale[k];
+    for (int k = 0; k < 8; ++k) v[k] = v[k] * s * c.scale[k];
   }
 #pragma unroll
   for (int k = 0; k < 8; ++k) v[k] += c.bias[k];
@@ -294,7 +294,7 @@ __device__ __forceinline__ void write_tile(const ProductArgs& g, const Work& k, 
                   v[i] = acc[m][n][4 * q + i];
                   if constexpr (SCALED) {
                     const uint32_t u = terms.scale[n][q][i];
-                    v[i] *= terms.a_scale[m] * as_float(u);
+                    v[i] = v[i] * terms.a_scale[m] * as_float(u);
                   }
                   if constexpr (!PLAIN) {
                     const uint32_t u = terms.bias[n][q][i / 2];
@@ -396,7 +396,7 @@ __device__ __forceinline__ void write_tile(const ProductArgs& g, const Work& k, 
             if (SCALED) {
               const float s = row < rows ? e.a_scale[k.i0 + row] : 0.f;
 #pragma unroll
-              for (int i = 0; i < 8; ++i) v[i] *= s * c.scale[i];
+              for (int i = 0; i < 8; ++i) v[i] = v[i] * s * c.scale[i];
             }
             if (!PLAIN) {
 #pragma unroll
@@ -459,7 +459,7 @@ __device__ __forceinline__ void write_tile(const ProductArgs& g, const Work& k, 
           const uint32_t o = out[r] | (((uint32_t)row * (uint32_t)e.n + (uint32_t)(wn + lane)) << shift);
           float v[1] = {z[r]};
           if (out[r] == 0) mend(k.i0 + row, col, v);
-          if (SCALED && row < rows) v[0] *= e.a_scale[k.i0 + row] * scale;
+          if (SCALED && row < rows) v[0] = v[0] * e.a_scale[k.i0 + row] * scale;
           if (!PLAIN) {
             v[0] += bias;
             if (e.pre) store(rp, o, v[0]);
@@ -541,7 +541,7 @@ __device__ __forceinline__ void join(const ProductArgs& g, const Mend& mend) {
       finish<decltype(act)::kind>(e, row, col, v, c);
     } else {
       float z = v[0];
-      if (e.a_scale) z *= e.a_scale[row] * e.b_scale[col];
+      if (e.a_scale) z = z * e.a_scale[row] * e.b_scale[col];
       if (e.bias) z += load_one(e.bias, col, e.dtype);
       if (e.pre) store_one(e.pre, row * e.n + col, e.dtype, z);
       z = activate<decltype(act)::kind>(z);

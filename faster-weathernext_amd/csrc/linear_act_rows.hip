@@ -117,7 +117,7 @@ __global__ void __launch_bounds__(64 * WAVES) rows_kernel(ProductArgs a) {
       float z = red[0][m][i][j];
 #pragma unroll
       for (int v = 1; v < WAVES; ++v) z += red[v][m][i][j];
-      if (OP == kOpE4m3) z *= e.a_scale[row] * e.b_scale[col];
+      if (OP == kOpE4m3) z = z * e.a_scale[row] * e.b_scale[col];
       if (e.bias) z += load_one(e.bias, col, e.dtype);
       if (e.pre) store_one(e.pre, row * e.n + col, e.dtype, z);
       z = activate<decltype(act)::kind>(z);

@@ -84,3 +84,30 @@ def test_float32_epilogue(rows):
       # Slopes stay below 1.1; the activation's own arithmetic within 2^-20 of z.
       slack = 1.1 * e + 2.0 ** -20 * z.abs() + 2.0 ** -23 * (want.abs() + r.double().abs())
       assert ((got.double() - want).abs() - slack).max() <= 0, (ins, outs, name)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,ins,outs", [(24, 64, 64), (24, 64, 65), (300, 64, 64), (300, 64, 65), (300, 8192, 64), (300, 8192, 65)])
+def test_scales_whose_product_has_no_place(rows, ins, outs, dtype):
+  """(x w^T) x_scale w_scale in that order: the scales' own product may lie under float32's range or over it."""
+  x, w = torch.zeros(rows, ins, device=DEV), torch.zeros(outs, ins, device=DEV)
+  x[:, 0], w[:, 0] = 448, 448
+  half = torch.finfo(dtype).eps / 2
+  for z, xs, ws in ((448 ** 2, 1.3 * 2.0 ** -126, 1.7 * 2.0 ** -17), (448 ** 2, 1.1e-30, 1.2e-10), (2.0 ** -18, 1.1e30, 1.3e10),
+                    (2.0 ** -18, 3e25, 3e15)):
+    if z < 1:
+      x[:, 0], w[:, 0] = 2.0 ** -9, 2.0 ** -9
+    else:
+      x[:, 0], w[:, 0] = 448, 448
+    a, b = torch.full((rows,), xs, device=DEV), torch.full((outs,), ws, device=DEV)
+    want = z * a.double()[:, None] * b.double()
+    for r in (None, torch.zeros(rows, outs, device=DEV, dtype=dtype)):
+      got = fwn.linear_act_q8(x.to(E4M3), a, w.to(E4M3), b, residual=r, dtype=dtype).double()
+      # Two products and the output round, by half a step each.
+      assert ((got - want).abs() <= want * (half + 2.0 ** -22)).all(), (z, xs, ws)
+  # A sum of zero stays zero under scales whose product is past float32's range.
+  x.zero_()
+  a, b = torch.full((rows,), 1e25, device=DEV), torch.full((outs,), 1e25, device=DEV)
+  for r in (None, torch.zeros(rows, outs, device=DEV, dtype=dtype)):
+    assert not fwn.linear_act_q8(x.to(E4M3), a, w.to(E4M3), b, residual=r, dtype=dtype).any()
