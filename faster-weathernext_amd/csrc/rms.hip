@@ -2,7 +2,7 @@
 // or in e4m3 with one scale a row, and its backward pass (gfx950).
 //
 //   s = rnd(x + y),  r = 1 / sqrt(mean(s^2) + eps),  v = s r w;  out = rnd(v)
-//   8 bits: scale = max(max|v| / 448, 2^-126), q = e4m3(v / scale), from v before any rounding
+//   8 bits: scale = max(max|v| / 448, 2^-126), q = e4m3(v (1 / scale)), from v before any rounding
 //   gx = g_sum + r (h - s r^2 mean(h s)),  h = g_out w;   gw = sum over the rows of g_out s r
 //
 // Streaming passes bound by HBM: a row is held in registers from its only load to its outputs, so each
@@ -201,8 +201,9 @@ __device__ __forceinline__ uint32_t row_max(uint32_t v, float* red) {
   return v;
 }
 
-// E codes of f * inv at p. |f * inv| is at most 448 (1 + 2^-22), which rounds to 448: no clamp, which
-// would turn NaN into a number.
+// E codes of f * inv at p, inv = 1 / scale rounded: within 2^-23 of the quotient, which decides codes only where it is that near
+// the middle of two (0.05% of bf16 rows' codes, whose quotients often are middles; either is as near there). |f * inv| is at
+// most 448 (1 + 2^-22), which rounds to 448: no clamp, which would turn NaN into a number.
 template <int E, bool TAIL>
 __device__ __forceinline__ void store_q8(uint8_t* p, int left, const float (&f)[E], float inv) {
   if (TAIL && left < E) {

@@ -217,7 +217,8 @@ def add_rms_norm(x, y, weight=None, *, eps=1e-6):
 def rms_norm_q8(x, weight=None, *, eps=1e-6):
   """(q, scale) of rms_norm(x, weight): OCP e4m3 values [..., channels] (torch.float8_e4m3fn) and a float32
   scale [...] a row, from the norm before any rounding: scale = max(max |row| / 448, 2^-126) and
-  q = row / scale. A row with NaN gives NaN. Forward only."""
+  q = row * (1 / scale) in float32, rounded to the nearest code (a quotient within 2^-23 of the middle of
+  two codes may go to either). A row with NaN gives NaN. Forward only."""
   _check(x, "x")
   _check_weight(weight, x)
   _no_grad("rms_norm_q8", x, weight)

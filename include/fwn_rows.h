@@ -142,8 +142,9 @@ int fwn_rms_norm_launch(const fwn_rms_desc* d, const void* x, const void* y, con
                         void* stream);
 
 /* The same with the output in 8 bits: for the unrounded values v of a row, scale[i] = max(max |v| / 448,
- * 2^-126) and q[i, :] the OCP e4m3 codes of v / scale[i], rounded to nearest even. A row with NaN has
- * scale and codes NaN; one whose largest magnitude is infinite has scale infinity and NaN codes there. */
+ * 2^-126) and q[i, :] the OCP e4m3 codes of v * (1 / scale[i]), reciprocal and product each rounded to float32,
+ * to nearest even: the codes nearest to v / scale[i], or, within 2^-23 of the middle of two, either of them. A row
+ * with NaN has scale and codes NaN; one whose largest magnitude is infinite has scale infinity and NaN codes there. */
 int fwn_rms_norm_q8_launch(const fwn_rms_desc* d, const void* x, const void* y, const void* weight, void* sum, uint8_t* q,
                            float* scale, void* stream);
 
