@@ -181,7 +181,7 @@ def linear_act_q8(x, x_scale, weight, weight_scale, bias=None, *, activation=Non
   _check(x, weight, bias, residual, dtype, lead)
   _check_like(x_scale, "x_scale", lead, torch.float32, x)
   _check_like(weight_scale, "weight_scale", weight.shape[:1], torch.float32, x)
-  _no_grad("linear_act_q8", x_scale, weight_scale, bias, residual)
+  _no_grad("linear_act_q8", x, x_scale, weight, weight_scale, bias, residual)
   outs, ins = weight.shape
   xr, xs = rows_of(x)
   wr, ws = rows_of(weight)

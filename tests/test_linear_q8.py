@@ -111,3 +111,17 @@ def test_scales_whose_product_has_no_place(rows, ins, outs, dtype):
   a, b = torch.full((rows,), 1e25, device=DEV), torch.full((outs,), 1e25, device=DEV)
   for r in (None, torch.zeros(rows, outs, device=DEV, dtype=dtype)):
     assert not fwn.linear_act_q8(x.to(E4M3), a, w.to(E4M3), b, residual=r, dtype=dtype).any()
+
+
+@gpu
+def test_codes_that_need_a_gradient_are_refused():
+  """x and weight as codes made under autograd: their gradient would be lost without a word."""
+  x, w, one = _normal((40, 64), 1), _normal((24, 64), 2), lambda n: torch.ones(n, device=DEV)
+  leaf = x.clone().requires_grad_()
+  codes = leaf.to(E4M3)
+  assert codes.requires_grad
+  for a, b in ((codes, w.to(E4M3)), (x.to(E4M3), w.clone().requires_grad_().to(E4M3))):
+    with pytest.raises(RuntimeError, match="no derivative"):
+      fwn.linear_act_q8(a, one(40), b, one(24))
+    with torch.no_grad():
+      assert fwn.linear_act_q8(a, one(40), b, one(24)).shape == (40, 24)
