@@ -114,7 +114,7 @@ def _dense(t, like):
 
 def _backward(s, weight, eps, g_out, g_sum, need_w):
   """(gradient of the rows, gradient of weight or None): fwn_rms_norm_bwd_launch."""
-  g_out, g_sum = _dense(g_out, s), _dense(g_sum, s)
+  s, weight, g_out, g_sum = s.contiguous(), dense(weight), _dense(g_out, s), _dense(g_sum, s)
   d = _desc(s, weight, eps, s.shape[-1])
   L = nat.lib()
   gx = torch.empty_like(s)
@@ -142,17 +142,13 @@ def _backward_torch(s, weight, eps, g_out, g_sum):
 
 
 class _RmsNorm(torch.autograd.Function):
-  """(x + y, its norm), or the norm alone where y is None."""
+  """(x + y, its norm), or the norm alone where y is None. x and weight are kept as they came: of a contiguous copy
+  autograd would not know that it is theirs, and a second derivative would miss what comes through it."""
 
   @staticmethod
   def forward(ctx, x, y, weight, eps):
-    weight = dense(weight)
-    if y is None:
-      s = x.contiguous()
-      _, out = _forward(s, None, weight, eps, False)
-    else:
-      s, out = _forward(x, y, weight, eps, False)
-    ctx.save_for_backward(s, weight)
+    s, out = _forward(x, y, weight, eps, False)
+    ctx.save_for_backward(x if y is None else s, weight)
     ctx.set_materialize_grads(False)
     ctx.eps = eps
     return out if y is None else (s, out)
