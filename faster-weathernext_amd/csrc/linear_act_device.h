@@ -474,8 +474,8 @@ __device__ __forceinline__ void write_tile(const ProductArgs& g, const Work& k, 
   });
 }
 
-// float32 products are formed of three bf16 parts a value, an infinity's beside it zeros or NaN: outputs that came
-// out NaN are formed anew of the whole values. OUTER: the operand's rows are k.
+// float32 products are formed of three bf16 parts a value, NaN beside an infinity: outputs that came out NaN are formed
+// anew of the whole values. OUTER: the operand's rows are k.
 template <bool OA, bool OB>
 struct MendParts {
   const ProductArgs& g;

@@ -1,9 +1,11 @@
 // The linear layers' products of float32 operands (gfx950), at float32's precision on the bf16 matrix units.
 //
-// A value is the exact sum of three bf16 parts: its top 8 significant bits, the next 8 and the last. Of the nine
-// products of parts the six above 2^-24 of the whole are formed and accumulated in float32, small ones first:
-// six bf16 MFMAs do what eight times as many clocks of float32 MFMAs do. The parts are formed on the way from memory to
-// LDS, so an operand of any strides and alignment is read where it lies, once a tile.
+// A value is the exact sum of three bf16 parts: it rounded, what is left rounded, and the rest. The second is at most 2^-8
+// of the value and the third 2^-17, of either sign. Of the nine products of parts the six largest are formed and accumulated in
+// float32, small ones first; the three left out are together within 2^-24 (1 + 2^-9) of the product, as its rounding
+// to float32 would be, and without a direction. (Parts cut off rather than rounded took as long, lost up to 2^-21 of a
+// product and always towards zero.) Six bf16 MFMAs do what eight times as many clocks of float32 MFMAs do. The parts are
+// formed on the way from memory to LDS, so an operand of any strides and alignment is read where it lies, once a tile.
 //
 // A workgroup is 4 waves on a 128 x 128 tile, a wave 64 x 64: per 16 k it reads 12 KB of LDS for 24 MFMAs. One
 // stage of 32 k is 48 KB of parts, so that two or three workgroups share a CU: while one splits and writes its next
@@ -18,6 +20,12 @@ namespace fwn {
 namespace {
 
 constexpr int TILE = 128, STEP = 32;
+
+// Two values as bf16, by one instruction.
+__device__ __forceinline__ uint32_t two_bf16(float a, float b) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2));
+}
 
 // One operand's stages: ROWS rows of 32 k ("inner") or 32 rows of k of 128 columns ("outer"), 4 FOURS values a thread.
 // In LDS a part is ROWS rows of 64 bytes or 32 of 256, 16-byte chunks swizzled as for the bf16 kernels.
@@ -91,23 +99,24 @@ struct Operand {
     }
   }
 
-  // Their parts to LDS. An infinity or NaN gives NaN in the middle part, and so in every output that it feeds.
+  // Their parts to LDS. An infinity or NaN, or a value that rounds to infinity, gives NaN in the middle part, and so in every
+  // output that it feeds.
   __device__ __forceinline__ void split(lds_char* to, const u32x4 (&v)[FOURS]) const {
 #pragma unroll
     for (int i = 0; i < FOURS; ++i) {
-      uint32_t part[3][4];
+      float f[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const uint32_t u = v[i][e];
-        const uint32_t u1 = as_bits(as_float(u) - as_float(u & 0xffff0000u));
-        part[0][e] = u;
-        part[1][e] = u1;
-        part[2][e] = as_bits(as_float(u1) - as_float(u1 & 0xffff0000u));
+        f[e] = as_float(u);
       }
 #pragma unroll
-      for (int p = 0; p < 3; ++p)
-        *(__attribute__((address_space(3))) u32x2*)(to + p * PLANE + lds[i]) =
-            u32x2{__builtin_amdgcn_perm(part[p][1], part[p][0], 0x07060302), __builtin_amdgcn_perm(part[p][3], part[p][2], 0x07060302)};
+      for (int p = 0; p < 3; ++p) {
+        const u32x2 part{two_bf16(f[0], f[1]), two_bf16(f[2], f[3])};
+        *(__attribute__((address_space(3))) u32x2*)(to + p * PLANE + lds[i]) = part;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f[e] -= as_float(e % 2 ? part[e / 2] & 0xffff0000u : part[e / 2] << 16);
+      }
     }
   }
 
