@@ -253,7 +253,7 @@ struct Bf16Terms {
 // outputs 62 us with single columns, 57 so): 32 rows at a time through the wave's strip to rows of eight columns a
 // lane, or of one column a lane where rows are not whole aligned eights. bf16 outputs that nothing but their column's
 // bias is added to are finished where the MFMAs leave them and go through LDS as bf16, 64 rows at a time. PLAIN: no
-// epilogue but the rounding (gradients). F32: the outputs are float32, else bf16. mend(row, col, v) may put right outputs
+// epilogue but the rounding (gradients). F32: the outputs are float32, else bf16. mend(row, col, v) may change outputs
 // before the epilogue.
 template <int BM, int MI, bool PLAIN, bool F32, bool SCALED, typename Mend>
 __device__ __forceinline__ void write_tile(const ProductArgs& g, const Work& k, const f32x16 (&acc)[MI][2], strip_ptr strip,
@@ -474,8 +474,10 @@ __device__ __forceinline__ void write_tile(const ProductArgs& g, const Work& k, 
   });
 }
 
-// float32 products are formed of three bf16 parts a value, NaN beside an infinity: outputs that came out NaN are formed
-// anew of the whole values. OUTER: the operand's rows are k.
+constexpr float kUp = 65536.f;  // of a float32 operand's parts, see linear_act_f32.hip
+
+// float32 products are formed of three bf16 parts of each value times kUp: outputs are divided by kUp^2, and those that
+// came out infinite or NaN formed anew of the whole values. OUTER: the operand's rows are k.
 template <bool OA, bool OB>
 struct MendParts {
   const ProductArgs& g;
@@ -487,9 +489,13 @@ struct MendParts {
 
   template <int N>
   __device__ __forceinline__ void operator()(int64_t row, int64_t col, float (&v)[N]) const {
+    const auto lost = [&](int e) { return !(__builtin_fabsf(v[e]) < __builtin_inff()); };
     bool bad = false;
 #pragma unroll
-    for (int e = 0; e < N; ++e) bad |= v[e] != v[e];
+    for (int e = 0; e < N; ++e) {
+      v[e] *= 1.f / (kUp * kUp);
+      bad |= lost(e);
+    }
     if (!bad) return;
     float s[N] = {};
     for (int64_t k = 0; k < g.k && bad; ++k) {  // until every one is NaN for good
@@ -498,12 +504,12 @@ struct MendParts {
 #pragma unroll
       for (int e = 0; e < N; ++e) {
         if (col + e < g.e.n) s[e] = fmaf(x, value<OB>(g.b, g.b_stride, col + e, k), s[e]);
-        bad |= v[e] != v[e] && s[e] == s[e];
+        bad |= lost(e) && s[e] == s[e];
       }
     }
 #pragma unroll
     for (int e = 0; e < N; ++e)
-      if (v[e] != v[e]) v[e] = s[e];
+      if (lost(e)) v[e] = s[e];
   }
 };
 

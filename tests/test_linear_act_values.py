@@ -13,6 +13,16 @@ def _normal(shape, seed, std=1.0):
   return (torch.randn(shape, generator=torch.Generator().manual_seed(seed)) * std).to(DEV)
 
 
+def _bound(k, a, b):
+  """A float32 sum of k products: (8 sqrt(k) + 16) 2^-24 of the rows' norms, as in test_linear_act."""
+  return (8 * k ** 0.5 + 16) * STEP * a.norm(dim=1)[:, None] * b.norm(dim=1)
+
+
+def _near(got, want, bound):
+  assert torch.isfinite(got).all()
+  assert ((got.double() - want).abs() - bound - STEP * want.abs() - 2.0 ** -149).max() <= 0
+
+
 @gpu
 @pytest.mark.parametrize("rows", [24, 300])
 def test_float32_single_products(rows):
@@ -42,3 +52,54 @@ def test_float32_sums_of_one_sign():
   off = (fwn.linear_act(x, w).double() - want) / want
   assert off.mean().abs() <= 0.15 * STEP, off.mean().item() / STEP
   assert off.abs().max() <= 8 * STEP
+
+
+@gpu
+@pytest.mark.parametrize("rows", [24, 300])
+@pytest.mark.parametrize("scale", [1e-38, 1e-37, 1e-36, 1e-35, 1e-33, 1e-30, 1e30, 1e33, 1e35, 1e36])
+def test_float32_exponents(rows, scale):
+  """Operands near either end of float32's range, subnormal ones among them, in the output and both gradients.
+  A product below the least normal number rounds to 2^-150 by itself: as many of them as the sum has terms."""
+  x, w, g = _normal((rows, 200), 1, scale), _normal((90, 200), 2, 0.01 / scale), _normal((rows, 90), 3)
+  lx, lw = x.clone().requires_grad_(), w.clone().requires_grad_()
+  out = fwn.linear_act(lx, lw)
+  gx, gw = torch.autograd.grad(out, (lx, lw), g)
+  xd, wd, gd = x.double(), w.double(), g.double()
+  _near(out.detach(), xd @ wd.t(), _bound(200, xd, wd))
+  _near(gx, gd @ wd, _bound(90, gd, wd.t()) + 90 * 2.0 ** -150)
+  _near(gw, gd.t() @ xd, _bound(rows, gd.t(), xd.t()) + rows * 2.0 ** -150)
+
+
+@gpu
+@pytest.mark.parametrize("rows", [24, 300])
+def test_float32_small_results(rows):
+  """Tiny times ordinary: results about and below float32's least normal number, in the output and both gradients."""
+  for scale in (1e-36, 1e-38, 1e-40):
+    x, w, g = _normal((rows, 72), 1, scale), _normal((65, 72), 2, 0.1), _normal((rows, 65), 3, scale)
+    lx, lw = x.clone().requires_grad_(), w.clone().requires_grad_()
+    out = fwn.linear_act(lx, lw)
+    xd, wd, gd = x.double(), w.double(), g.double()
+    # A product below the least normal number is held to 2^-150 by its own rounding: 72 (or 65) of them a sum.
+    floor = 100 * 2.0 ** -150
+    _near(out.detach(), xd @ wd.t(), _bound(72, xd, wd) + floor)
+    gx, = torch.autograd.grad(out, lx, g, retain_graph=True)
+    _near(gx, gd @ wd, _bound(65, gd, wd.t()) + floor)
+    gw, = torch.autograd.grad(out, lw, _normal((rows, 65), 4))
+    gd = _normal((rows, 65), 4).double()
+    _near(gw, gd.t() @ xd, _bound(rows, gd.t(), xd.t()) + rows * 2.0 ** -150)
+
+
+@gpu
+@pytest.mark.parametrize("rows", [24, 300])
+def test_float32_large_results(rows):
+  """Sums up to float32's largest, split over ranges too (ins 4,096); past it they are infinite."""
+  for ins in (64, 4096):
+    x, w = _normal((rows, ins), 1, 1e19), _normal((72, ins), 2, 1e19 / ins ** 0.5 / 10)
+    xd, wd = x.double(), w.double()
+    _near(fwn.linear_act(x, w), xd @ wd.t(), _bound(ins, xd, wd))
+  x, w = torch.full((rows, 64), 1e20, device=DEV), torch.full((72, 64), 1e20, device=DEV)
+  w[3] = -1e20
+  w[4] = 0
+  out = fwn.linear_act(x, w)
+  assert (out[:, 3] == -float("inf")).all() and not out[:, 4].any()
+  assert (out[:, 5:] == float("inf")).all() and (out[:, :3] == float("inf")).all()
