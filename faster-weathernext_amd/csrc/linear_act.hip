@@ -278,9 +278,9 @@ __global__ void __launch_bounds__((threads_of(BM)), 2) product_kernel(ProductArg
                                               lane, terms, MendNothing());
 }
 
-template <bool PLAIN, int N>
+template <bool PLAIN, bool F32, int N>
 __global__ void __launch_bounds__(256) join_kernel(ProductArgs g) {
-  join<PLAIN, N>(g, MendNothing());
+  join<PLAIN, F32, N>(g, MendNothing());
 }
 
 template <bool OA, bool OB, Form FORM, int TILE>
@@ -290,9 +290,9 @@ hipError_t launch_tile(const ProductArgs& g, hipStream_t stream) {
                      stream, g);
   if (hipError_t e = hipGetLastError(); e != hipSuccess || !g.part) return e;
   if (g.e.vec)
-    hipLaunchKernelGGL((join_kernel<OB, 8>), join_grid(g), dim3(256), 0, stream, g);
+    hipLaunchKernelGGL((join_kernel<OB, FORM == Form::kWidened, 8>), join_grid(g), dim3(256), 0, stream, g);
   else
-    hipLaunchKernelGGL((join_kernel<OB, 1>), join_grid(g), dim3(256), 0, stream, g);
+    hipLaunchKernelGGL((join_kernel<OB, FORM == Form::kWidened, 1>), join_grid(g), dim3(256), 0, stream, g);
   return hipGetLastError();
 }
 

@@ -76,48 +76,77 @@ __device__ __forceinline__ u32x4 widen(uint32_t lo, uint32_t hi) {
   return u32x4{two(lo, std::false_type()), two(lo, std::true_type()), two(hi, std::false_type()), two(hi, std::true_type())};
 }
 
-// e^x and 1 / x on the transcendental unit, within two units in the last place.
-__device__ __forceinline__ float fast_exp(float x) { return fast_exp2(x * LOG2E); }
-__device__ __forceinline__ float fast_rcp(float x) { return __builtin_amdgcn_rcpf(x); }
+// The activations' functions for outputs of float32 (F32), and of bf16: e^x on the transcendental unit, off by up to
+// (1 + |x|) 2^-23 of itself, its reciprocal there, zero below 2^-126, and erf by Abramowitz and Stegun's 7.1.26, off by
+// up to 1e-6 in float32 (1.5e-7 without its roundings): a thousandth of what a bf16 output of that size rounds.
+// float32 outputs with bf16's functions and with their own, us of 10,242 x 768 -> 3,072: gelu 267 and 277, gelu_tanh 258 and
+// 268, silu 257 and 265.
+template <bool F32>
+constexpr float kLog = F32 ? 1.f : LOG2E;
+template <bool F32>
+__device__ __forceinline__ float power(float x) {  // e^(x / kLog)
+  if constexpr (F32) return expf(x);
+  return fast_exp2(x);
+}
 
-// erf by Abramowitz and Stegun's 7.1.26, off by at most 1.5e-7 (a value times z / 2 here).
+template <bool F32>
 __device__ __forceinline__ float erf_of(float x) {
-  const float y = __builtin_fabsf(x), t = fast_rcp(fmaf(0.3275911f, y, 1.f));
+  if constexpr (F32) return erff(x);
+  const float y = __builtin_fabsf(x), t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, y, 1.f));
   float p = fmaf(1.061405429f, t, -1.453152027f);
   p = fmaf(p, t, 1.421413741f);
   p = fmaf(p, t, -0.284496736f);
   p = fmaf(p, t, 0.254829592f);
-  return __builtin_copysignf(1.f - p * t * fast_exp(-y * y), x);
+  return __builtin_copysignf(1.f - p * t * fast_exp2(-y * y * LOG2E), x);
+}
+
+// p = 1 / (1 + e^(x / kLog)) and q = 1 - p. float32: of e^-|x|, which leaves neither the range nor digits behind.
+struct Logistic {
+  float p, q;
+};
+template <bool F32>
+__device__ __forceinline__ Logistic logistic(float x) {
+  if constexpr (F32) {
+    const float e = expf(-__builtin_fabsf(x)), r = __builtin_amdgcn_rcpf(1.f + e);
+    return x > 0.f ? Logistic{e * r, r} : Logistic{r, e * r};
+  }
+  const float p = __builtin_amdgcn_rcpf(1.f + fast_exp2(x));
+  return {p, 1.f - p};
 }
 
 constexpr float kTanh = 0.7978845608028654f, kCube = 0.044715f;  // gelu_tanh: u = kTanh (z + kCube z^3)
 
+// -2 u kLog of z, z2 = z^2.
+template <bool F32>
+__device__ __forceinline__ float tanh_arg(float z, float z2) {
+  return z * fmaf(z2, -2.f * kTanh * kCube * kLog<F32>, -2.f * kTanh * kLog<F32>);
+}
+
 // act(z). The tanh form is z / (1 + e^(-2u)).
-template <int KIND>
+template <int KIND, bool F32>
 __device__ __forceinline__ float activate(float z) {
   if constexpr (KIND == FWN_ACT_RELU) return z > 0.f || z != z ? z : 0.f;
-  if constexpr (KIND == FWN_ACT_GELU) return 0.5f * z * (1.f + erf_of(z * 0.7071067811865476f));
-  if constexpr (KIND == FWN_ACT_GELU_TANH)
-    return z * fast_rcp(1.f + fast_exp2(z * fmaf(z * z, -2.f * kTanh * kCube * LOG2E, -2.f * kTanh * LOG2E)));
-  if constexpr (KIND == FWN_ACT_SILU) return z * fast_rcp(1.f + fast_exp(-z));
+  if constexpr (KIND == FWN_ACT_GELU) return 0.5f * z * (1.f + erf_of<F32>(z * 0.7071067811865476f));
+  if constexpr (KIND == FWN_ACT_GELU_TANH) return z * logistic<F32>(tanh_arg<F32>(z, z * z)).p;
+  if constexpr (KIND == FWN_ACT_SILU) return z * logistic<F32>(-z * kLog<F32>).p;
   return z;
 }
 
 // act'(z).
-template <int KIND>
+template <int KIND, bool F32>
 __device__ __forceinline__ float slope(float z) {
   if constexpr (KIND == FWN_ACT_RELU) return z > 0.f ? 1.f : 0.f;
   if constexpr (KIND == FWN_ACT_GELU)
-    return 0.5f * (1.f + erf_of(z * 0.7071067811865476f)) + z * fast_exp(-0.5f * z * z) * 0.3989422804014327f;
+    return 0.5f * (1.f + erf_of<F32>(z * 0.7071067811865476f)) + z * power<F32>(-0.5f * z * z * kLog<F32>) * 0.3989422804014327f;
   if constexpr (KIND == FWN_ACT_GELU_TANH) {
-    // p = 1 / (1 + e^(-2u)), p + 2 z p (1 - p) u'; beyond 12 it is 0 or 1, and a large z^2 would meet that 0.
-    const float y = z > 12.f ? 12.f : z < -12.f ? -12.f : z, q = y * y;
-    const float p = fast_rcp(1.f + fast_exp2(y * fmaf(q, -2.f * kTanh * kCube * LOG2E, -2.f * kTanh * LOG2E)));
-    return fmaf(2.f * y * p * (1.f - p), fmaf(q, 3.f * kTanh * kCube, kTanh), p);
+    // p + 2 z p (1 - p) u'; beyond 12 p is 0 or 1, and a large z^2 would meet that 0.
+    const float y = z > 12.f ? 12.f : z < -12.f ? -12.f : z, y2 = y * y;
+    const Logistic l = logistic<F32>(tanh_arg<F32>(y, y2));
+    return fmaf(2.f * y * l.p * l.q, fmaf(y2, 3.f * kTanh * kCube, kTanh), l.p);
   }
   if constexpr (KIND == FWN_ACT_SILU) {
-    const float p = fast_rcp(1.f + fast_exp(-z)), y = p > 0.f ? z : 0.f;
-    return p * fmaf(y, 1.f - p, 1.f);
+    const Logistic l = logistic<F32>(-z * kLog<F32>);
+    return l.p * fmaf(l.p > 0.f ? z : 0.f, l.q, 1.f);
   }
   return 1.f;
 }
@@ -154,7 +183,7 @@ struct Columns {
 };
 
 // The epilogue of z[row, col .. col + 7] in rows of whole aligned eights.
-template <int KIND>
+template <int KIND, bool F32>
 __device__ __forceinline__ void finish(const EpilogueArgs& e, int64_t row, int64_t col, float (&v)[8], const Columns& c) {
   if (e.a_scale) {
     const float s = e.a_scale[row];
@@ -166,7 +195,7 @@ __device__ __forceinline__ void finish(const EpilogueArgs& e, int64_t row, int64
   const int64_t at = row * e.n + col;
   if (e.pre) store8(e.pre, at, e.dtype, v);
 #pragma unroll
-  for (int k = 0; k < 8; ++k) v[k] = activate<KIND>(v[k]);
+  for (int k = 0; k < 8; ++k) v[k] = activate<KIND, F32>(v[k]);
   if (e.residual) {
     float r[8];
     load8(e.residual, row * e.r_row + col, e.dtype, r);
@@ -298,7 +327,7 @@ __device__ __forceinline__ void write_tile(const ProductArgs& g, const Work& k, 
                   }
                   if constexpr (!PLAIN) {
                     const uint32_t u = terms.bias[n][q][i / 2];
-                    v[i] = activate<decltype(act)::kind>(v[i] + as_float(i % 2 ? u & 0xffff0000u : u << 16));
+                    v[i] = activate<decltype(act)::kind, false>(v[i] + as_float(i % 2 ? u & 0xffff0000u : u << 16));
                   }
                 }
                 *(__attribute__((address_space(3))) u32x2*)(half_strip + strip_row * 128 +
@@ -403,7 +432,7 @@ __device__ __forceinline__ void write_tile(const ProductArgs& g, const Work& k, 
               for (int i = 0; i < 8; ++i) v[i] += c.bias[i];
               if (pre) store(rp, o, v);
 #pragma unroll
-              for (int i = 0; i < 8; ++i) v[i] = activate<decltype(act)::kind>(v[i]);
+              for (int i = 0; i < 8; ++i) v[i] = activate<decltype(act)::kind, F32>(v[i]);
               if (residual) {
                 float r[8];
                 asked(m, p, r);
@@ -463,7 +492,7 @@ __device__ __forceinline__ void write_tile(const ProductArgs& g, const Work& k, 
           if (!PLAIN) {
             v[0] += bias;
             if (e.pre) store(rp, o, v[0]);
-            v[0] = activate<decltype(act)::kind>(v[0]);
+            v[0] = activate<decltype(act)::kind, F32>(v[0]);
             if (e.residual) v[0] += res[r];
           }
           store(ro, o, v[0]);
@@ -519,8 +548,8 @@ struct MendNothing {
 };
 
 // The partial products added in the order of the splits, then the epilogue: N columns a thread, eight where rows are
-// whole aligned eights, else one, so that a wave's accesses still lie side by side.
-template <bool PLAIN, int N, typename Mend>
+// whole aligned eights, else one, so that a wave's accesses still lie side by side. F32: the outputs are float32.
+template <bool PLAIN, bool F32, int N, typename Mend>
 __device__ __forceinline__ void join(const ProductArgs& g, const Mend& mend) {
   const EpilogueArgs& e = g.e;
   const int64_t across = N == 8 ? g.part_row / 8 : e.n, id = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -544,13 +573,13 @@ __device__ __forceinline__ void join(const ProductArgs& g, const Mend& mend) {
     if constexpr (N == 8) {
       Columns c;
       c.load(e, col);
-      finish<decltype(act)::kind>(e, row, col, v, c);
+      finish<decltype(act)::kind, F32>(e, row, col, v, c);
     } else {
       float z = v[0];
       if (e.a_scale) z = z * e.a_scale[row] * e.b_scale[col];
       if (e.bias) z += load_one(e.bias, col, e.dtype);
       if (e.pre) store_one(e.pre, row * e.n + col, e.dtype, z);
-      z = activate<decltype(act)::kind>(z);
+      z = activate<decltype(act)::kind, F32>(z);
       if (e.residual) z += load_one(e.residual, row * e.r_row + col, e.dtype);
       store_one(e.out, row * e.n + col, e.dtype, z);
     }

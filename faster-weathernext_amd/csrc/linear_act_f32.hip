@@ -198,7 +198,7 @@ __global__ void __launch_bounds__(256, OA || OB ? 2 : 3) product_f32_kernel(Prod
 
 template <bool OA, bool OB, int N>
 __global__ void __launch_bounds__(256) join_f32_kernel(ProductArgs g) {
-  join<OB, N>(g, MendParts<OA, OB>{g});
+  join<OB, true, N>(g, MendParts<OA, OB>{g});
 }
 
 template <bool OA, bool OB, int BM = TILE>

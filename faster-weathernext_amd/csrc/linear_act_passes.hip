@@ -24,8 +24,8 @@ __global__ void __launch_bounds__(256) layout_kernel(LayoutArgs a) {
 }
 
 // 256 columns by `chunk` rows a workgroup, eight columns of every eighth row a thread: side by side where rows are whole
-// aligned eights (VEC), else 32 apart, so that a wave's accesses lie side by side.
-template <int KIND, bool VEC>
+// aligned eights (VEC), else 32 apart, so that a wave's accesses lie side by side. F32: the dtype is float32.
+template <int KIND, bool VEC, bool F32>
 __global__ void __launch_bounds__(256) slope_kernel(SlopeArgs a) {
   __shared__ float red[8][256];
   const int across = (a.outs + 255) / 256, block = (int)blockIdx.x / across;
@@ -52,7 +52,7 @@ __global__ void __launch_bounds__(256) slope_kernel(SlopeArgs a) {
       }
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        if constexpr (KIND != FWN_ACT_NONE) dz[k] *= slope<KIND>(z[k]);
+        if constexpr (KIND != FWN_ACT_NONE) dz[k] *= slope<KIND, F32>(z[k]);
         sum[k] += dz[k];
       }
       if (a.dz) {
@@ -127,22 +127,23 @@ hipError_t launch_layout(const LayoutArgs& a, hipStream_t stream) {
   return hipGetLastError();
 }
 
-template <bool VEC>
+template <bool VEC, bool F32>
 static hipError_t launch_slope_as(const SlopeArgs& a, hipStream_t stream) {
   const dim3 grid((unsigned)((a.outs + 255) / 256) * (unsigned)a.blocks), block(256);
   switch (a.activation) {
-    case FWN_ACT_RELU: hipLaunchKernelGGL((slope_kernel<FWN_ACT_RELU, VEC>), grid, block, 0, stream, a); break;
-    case FWN_ACT_GELU: hipLaunchKernelGGL((slope_kernel<FWN_ACT_GELU, VEC>), grid, block, 0, stream, a); break;
-    case FWN_ACT_GELU_TANH: hipLaunchKernelGGL((slope_kernel<FWN_ACT_GELU_TANH, VEC>), grid, block, 0, stream, a); break;
-    case FWN_ACT_SILU: hipLaunchKernelGGL((slope_kernel<FWN_ACT_SILU, VEC>), grid, block, 0, stream, a); break;
-    default: hipLaunchKernelGGL((slope_kernel<FWN_ACT_NONE, VEC>), grid, block, 0, stream, a);
+    case FWN_ACT_RELU: hipLaunchKernelGGL((slope_kernel<FWN_ACT_RELU, VEC, F32>), grid, block, 0, stream, a); break;
+    case FWN_ACT_GELU: hipLaunchKernelGGL((slope_kernel<FWN_ACT_GELU, VEC, F32>), grid, block, 0, stream, a); break;
+    case FWN_ACT_GELU_TANH: hipLaunchKernelGGL((slope_kernel<FWN_ACT_GELU_TANH, VEC, F32>), grid, block, 0, stream, a); break;
+    case FWN_ACT_SILU: hipLaunchKernelGGL((slope_kernel<FWN_ACT_SILU, VEC, F32>), grid, block, 0, stream, a); break;
+    default: hipLaunchKernelGGL((slope_kernel<FWN_ACT_NONE, VEC, F32>), grid, block, 0, stream, a);
   }
   return hipGetLastError();
 }
 
 hipError_t launch_slope(const SlopeArgs& a, hipStream_t stream) {
   const bool vec = a.outs % 8 == 0 && (((uintptr_t)a.g | (uintptr_t)a.pre) & 15) == 0;
-  return vec ? launch_slope_as<true>(a, stream) : launch_slope_as<false>(a, stream);
+  if (a.dtype == FWN_F32) return vec ? launch_slope_as<true, true>(a, stream) : launch_slope_as<false, true>(a, stream);
+  return vec ? launch_slope_as<true, false>(a, stream) : launch_slope_as<false, false>(a, stream);
 }
 
 hipError_t launch_column_sums(const float* part, int64_t count, int64_t n, void* out, int dtype, hipStream_t stream) {

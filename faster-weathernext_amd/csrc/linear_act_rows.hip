@@ -120,7 +120,7 @@ __global__ void __launch_bounds__(64 * WAVES) rows_kernel(ProductArgs a) {
       if (OP == kOpE4m3) z = z * e.a_scale[row] * e.b_scale[col];
       if (e.bias) z += load_one(e.bias, col, e.dtype);
       if (e.pre) store_one(e.pre, row * e.n + col, e.dtype, z);
-      z = activate<decltype(act)::kind>(z);
+      z = activate<decltype(act)::kind, OP != kOpBf16>(z);
       if (e.residual) z += load_one(e.residual, row * e.r_row + col, e.dtype);
       store_one(e.out, row * e.n + col, e.dtype, z);
     }

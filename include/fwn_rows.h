@@ -168,8 +168,8 @@ int fwn_rms_norm_bwd_launch(const fwn_rms_desc* d, const void* s, const void* we
  * r_stride elements apart (0: one row for all; r_stride at most FWN_LINEAR_ACT_MAX); bias [outs], out and pre
  * [rows, outs] are contiguous.
  * Products accumulate in float32; out, and pre (z for the backward, NULL: not stored) are rounded
- * once. bias and residual may be NULL. Every tensor is of `dtype`; float32 products keep float32's precision over its whole range. No output
- * of the launches here may overlap an input or another output. */
+ * once. bias and residual may be NULL. Every tensor is of `dtype`; float32 products keep float32's precision over
+ * its whole range. No output of the launches here may overlap an input or another output. */
 #define FWN_ACT_NONE 0
 #define FWN_ACT_RELU 1
 #define FWN_ACT_GELU 2      /* z (1 + erf(z / sqrt 2)) / 2 */

@@ -103,3 +103,62 @@ def test_float32_large_results(rows):
   out = fwn.linear_act(x, w)
   assert (out[:, 3] == -float("inf")).all() and not out[:, 4].any()
   assert (out[:, 5:] == float("inf")).all() and (out[:, :3] == float("inf")).all()
+
+
+def _points():
+  z = torch.cat([torch.linspace(-20, 20, 4001), torch.logspace(-6, 0, 400), -torch.logspace(-6, 0, 400),
+                 torch.logspace(-37, -6, 100), torch.linspace(-110, 110, 441)])
+  return z.float().to(DEV)
+
+
+def _act64(z, name):
+  """act, act' and p with act = z p. gelu_tanh by p = 1 / (1 + e^-2u): z (1 + tanh(u)) / 2 is off by |z| 2^-54
+  in float64 where tanh nears -1, 4e-16 at z = -7.2, where its value is 2e-16."""
+  z = z.double().requires_grad_()
+  phi = {"gelu": torch.special.ndtr, "silu": torch.sigmoid,
+         "gelu_tanh": lambda t: torch.sigmoid(2 * (2 / torch.pi) ** 0.5 * (t + 0.044715 * t ** 3))}[name]
+  a = torch.nn.functional.gelu(z) if name == "gelu" else z * phi(z)
+  return a.detach(), torch.autograd.grad(a.sum(), z)[0], phi(z.detach())
+
+
+@gpu
+@pytest.mark.parametrize("name", ["gelu", "gelu_tanh", "silu"])
+@pytest.mark.parametrize("outs", [1, 8])
+@pytest.mark.parametrize("rows", [32, 5342])
+def test_float32_activations(name, rows, outs):
+  """act and act' of float32 pre-activations that are exact (a weight of one). Half steps that each may take:
+
+  gelu: erf is within two steps of its value below 1 (4 of 2^-24), its sum with 1 rounds below 2 by 2^-24: half of
+  five, 2.5, of z; two products round the value. The slope adds the density's exponent, z^2 / 2 rounded twice.
+  silu and gelu_tanh: z p, p = 1 / (1 + e^-u): e within two steps, the sum a half step, the reciprocal one step
+  and the product a half: 8 of the value, and (1 - p) times the exponent's own roundings (none of silu's -z;
+  four of gelu_tanh's u, which grow with u). Where p is below the least normal number it has steps of 2^-149, a few
+  of them, times what it is multiplied by."""
+  z = _points()
+  if rows == 32:
+    z = z[torch.randperm(z.numel(), generator=torch.Generator().manual_seed(1))[:32].to(DEV)]
+  one, g = torch.ones(outs, 1, device=DEV), torch.zeros(rows, outs, device=DEV)
+  g[:, 0] = 1
+  leaf = z[:, None].contiguous().requires_grad_()
+  out = fwn.linear_act(leaf, one, activation=name)
+  want, slope, p = _act64(z, name)
+  y, u = z.double().abs(), 2 * (2 / torch.pi) ** 0.5 * (z.double() + 0.044715 * z.double() ** 3).abs()
+  if name == "gelu":
+    bound = 2.5 * y + 2 * want.abs()
+  else:
+    bound = want.abs() * (8 + (4 * u * (1 - p) if name == "gelu_tanh" else 0))
+  over = (out[:, 0].double() - want).abs() - bound * STEP - (1 + y) * 2.0 ** -147
+  assert over.max() <= 0, (name, z[over.argmax()].item())
+  gx, = torch.autograd.grad(out, leaf, g)
+  if name == "gelu":
+    density = y * torch.exp(-0.5 * y * y) * (0.5 / torch.pi) ** 0.5
+    bound = 2.5 + density * (8 + 2 * y * y) + 2 * slope.abs()
+  elif name == "silu":
+    # p (1 + z (1 - p)): p's 8 in each place, and the difference 1 - p rounds by 2^-24 of 1.
+    bound = p * (8 * (1 + y * (1 - p)) + y * (1 + 8 * p) + 4 * (1 + y))
+  else:
+    c = 2 * y * p * (1 - p) * (2 / torch.pi) ** 0.5 * (1 + 3 * 0.044715 * y * y)
+    e = 8 + 4 * u * (1 - p)
+    bound = p * e + c * (2 * e + 8) + 2 * y * p * (1 + e * p) * (2 / torch.pi) ** 0.5 * (1 + 3 * 0.044715 * y * y)
+  over = (gx[:, 0].double() - slope).abs() - bound * STEP - (1 + 2 * y * (1 + 0.134145 * y * y)) * 2.0 ** -147
+  assert over.max() <= 0, (name, z[over.argmax()].item(), over.max().item() / STEP)
