@@ -77,10 +77,10 @@ __device__ __forceinline__ u32x4 widen(uint32_t lo, uint32_t hi) {
 }
 
 // The activations' functions for outputs of float32 (F32), and of bf16: e^x on the transcendental unit, off by up to
-// (1 + |x|) 2^-23 of itself, its reciprocal there, zero below 2^-126, and erf by Abramowitz and Stegun's 7.1.26, off by
-// up to 1e-6 in float32 (1.5e-7 without its roundings): a thousandth of what a bf16 output of that size rounds.
-// float32 outputs with bf16's functions and with their own, us of 10,242 x 768 -> 3,072: gelu 267 and 277, gelu_tanh 258 and
-// 268, silu 257 and 265.
+// (1 + |x|) 2^-23 of itself, its reciprocal there, zero below 2^-126, and erfc by Abramowitz and Stegun's 7.1.26, off by
+// up to 1e-6 in float32 (1.5e-7 without its roundings) and, where it is small itself, by up to 0.4% of it for z down to -6.2,
+// one rounding of a bf16 output. float32 outputs with bf16's functions and with their own, us of 10,242 x 768 -> 3,072: gelu 267
+// and 286, gelu_tanh 258 and 264, silu 257 and 262.
 template <bool F32>
 constexpr float kLog = F32 ? 1.f : LOG2E;
 template <bool F32>
@@ -89,15 +89,19 @@ __device__ __forceinline__ float power(float x) {  // e^(x / kLog)
   return fast_exp2(x);
 }
 
+// (1 + erf(z / sqrt 2)) / 2, formed of erfc so that the small values of negative z keep their digits: the sum leaves
+// none from z = -5.5 on.
 template <bool F32>
-__device__ __forceinline__ float erf_of(float x) {
-  if constexpr (F32) return erff(x);
+__device__ __forceinline__ float normal_cdf(float z) {
+  const float x = z * 0.7071067811865476f;
+  if constexpr (F32) return 0.5f * erfcf(-x);
   const float y = __builtin_fabsf(x), t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, y, 1.f));
   float p = fmaf(1.061405429f, t, -1.453152027f);
   p = fmaf(p, t, 1.421413741f);
   p = fmaf(p, t, -0.284496736f);
   p = fmaf(p, t, 0.254829592f);
-  return __builtin_copysignf(1.f - p * t * fast_exp2(-y * y * LOG2E), x);
+  const float c = 0.5f * p * t * fast_exp2(-y * y * LOG2E);
+  return z > 0.f ? 1.f - c : c;
 }
 
 // p = 1 / (1 + e^(x / kLog)) and q = 1 - p. float32: of e^-|x|, which leaves neither the range nor digits behind.
@@ -126,7 +130,7 @@ __device__ __forceinline__ float tanh_arg(float z, float z2) {
 template <int KIND, bool F32>
 __device__ __forceinline__ float activate(float z) {
   if constexpr (KIND == FWN_ACT_RELU) return z > 0.f || z != z ? z : 0.f;
-  if constexpr (KIND == FWN_ACT_GELU) return 0.5f * z * (1.f + erf_of<F32>(z * 0.7071067811865476f));
+  if constexpr (KIND == FWN_ACT_GELU) return z * normal_cdf<F32>(z);
   if constexpr (KIND == FWN_ACT_GELU_TANH) return z * logistic<F32>(tanh_arg<F32>(z, z * z)).p;
   if constexpr (KIND == FWN_ACT_SILU) return z * logistic<F32>(-z * kLog<F32>).p;
   return z;
@@ -137,7 +141,7 @@ template <int KIND, bool F32>
 __device__ __forceinline__ float slope(float z) {
   if constexpr (KIND == FWN_ACT_RELU) return z > 0.f ? 1.f : 0.f;
   if constexpr (KIND == FWN_ACT_GELU)
-    return 0.5f * (1.f + erf_of<F32>(z * 0.7071067811865476f)) + z * power<F32>(-0.5f * z * z * kLog<F32>) * 0.3989422804014327f;
+    return normal_cdf<F32>(z) + z * power<F32>(-0.5f * z * z * kLog<F32>) * 0.3989422804014327f;
   if constexpr (KIND == FWN_ACT_GELU_TANH) {
     // p + 2 z p (1 - p) u'; beyond 12 p is 0 or 1, and a large z^2 would meet that 0.
     const float y = z > 12.f ? 12.f : z < -12.f ? -12.f : z, y2 = y * y;
