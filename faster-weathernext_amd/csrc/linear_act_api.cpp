@@ -22,7 +22,7 @@ int check_desc(const fwn_linear_desc* d, const char* what) {
     return fail(FWN_ERR_INVALID_ARG, "%s: ins %d and outs %d must be 1 to %d", what, d->ins, d->outs, FWN_LINEAR_ACT_MAX);
   // Byte offsets stay inside 64 bits and grids inside 32.
   if (d->rows < 0 || d->rows > (INT64_C(1) << 31)) return fail(FWN_ERR_INVALID_ARG, "%s: %lld rows", what, (long long)d->rows);
-  const int64_t widest = INT64_C(1) << 30;
+  const int64_t widest = FWN_LINEAR_STRIDE_MAX;
   if (d->x_stride < 0 || d->w_stride < 0 || d->r_stride < 0 || d->x_stride > widest || d->w_stride > widest ||
       d->r_stride > FWN_LINEAR_ACT_MAX)
     return fail(FWN_ERR_INVALID_ARG, "%s: strides %lld, %lld and %lld", what, (long long)d->x_stride,

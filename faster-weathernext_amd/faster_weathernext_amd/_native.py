@@ -89,6 +89,7 @@ class LinearDesc(ctypes.Structure):
 
 ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}  # FWN_ACT_*
 LINEAR_ACT_MAX = 1 << 20  # FWN_LINEAR_ACT_MAX
+LINEAR_STRIDE_MAX = 1 << 30  # FWN_LINEAR_STRIDE_MAX
 RMS_MAX_CHANNELS = 16384  # FWN_RMS_MAX_CHANNELS
 ROWS_MAX_CHANNELS = 4096  # FWN_ROWS_MAX_CHANNELS
 COND_MAX = 64  # FWN_COND_MAX: norms of one fwn_cond_affine_launch

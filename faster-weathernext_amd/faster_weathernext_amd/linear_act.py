@@ -36,12 +36,12 @@ def _check_like(t, name, shape, dtype, x):
     raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
 
 
-def _residual(t):
-  """(t's rows, their stride) as the kernels read a residual: at most LINEAR_ACT_MAX elements apart."""
+def _rows(t, most=nat.LINEAR_STRIDE_MAX):
+  """(t's rows, their stride) as the launches take them: at most `most` elements apart (a residual's LINEAR_ACT_MAX)."""
   if t is None:
     return None, 0
   rows, stride = rows_of(t)
-  return (rows, stride) if stride <= nat.LINEAR_ACT_MAX else (rows.contiguous(), rows.shape[-1])
+  return (rows, stride) if stride <= most else (rows.contiguous(), rows.shape[-1])
 
 
 def _activation(name):
@@ -59,9 +59,9 @@ def _workspace(query, d, like, *addresses):
 def _forward(x, weight, bias, residual, activation, keep):
   """(act(x weight^T + bias) + residual, the pre-activation or None), without autograd."""
   lead, (outs, ins) = x.shape[:-1], weight.shape
-  xr, xs = rows_of(x)
-  wr, ws = rows_of(weight)
-  rr, rs = _residual(residual)
+  xr, xs = _rows(x)
+  wr, ws = _rows(weight)
+  rr, rs = _rows(residual, nat.LINEAR_ACT_MAX)
   bias = dense(bias)
   L = nat.lib()
   out = x.new_empty((*lead, outs))
@@ -126,8 +126,8 @@ class _LinearAct(torch.autograd.Function):
     if as_torch(g):
       return (*_backward_torch(x, weight, bias, g, act, needs), g_res, None)
     g = dense(g)
-    xr, xs = rows_of(x) if need_w else (None, 0)
-    wr, ws = rows_of(weight) if need_x else (None, 0)
+    xr, xs = _rows(x) if need_w else (None, 0)
+    wr, ws = _rows(weight) if need_x else (None, 0)
     d = nat.LinearDesc(g.numel() // outs, xs, ws, 0, ins, outs, _DTYPES[g.dtype], act)
     L = nat.lib()
     gx = g.new_empty(x_shape) if need_x else None
@@ -183,9 +183,9 @@ def linear_act_q8(x, x_scale, weight, weight_scale, bias=None, *, activation=Non
   _check_like(weight_scale, "weight_scale", weight.shape[:1], torch.float32, x)
   _no_grad("linear_act_q8", x, x_scale, weight, weight_scale, bias, residual)
   outs, ins = weight.shape
-  xr, xs = rows_of(x)
-  wr, ws = rows_of(weight)
-  rr, rs = _residual(residual)
+  xr, xs = _rows(x)
+  wr, ws = _rows(weight)
+  rr, rs = _rows(residual, nat.LINEAR_ACT_MAX)
   bias = dense(bias)
   x_scale, weight_scale = dense(x_scale), dense(weight_scale)
   L = nat.lib()

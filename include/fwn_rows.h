@@ -165,8 +165,8 @@ int fwn_rms_norm_bwd_launch(const fwn_rms_desc* d, const void* s, const void* we
 /* Matrix product with bias, activation and residual in its epilogue:
  *   z = x weight^T + bias,  out = act(z) + residual
  * x is [rows, ins], weight [outs, ins], residual [rows, outs], with contiguous rows x_stride, w_stride and
- * r_stride elements apart (0: one row for all; r_stride at most FWN_LINEAR_ACT_MAX); bias [outs], out and pre
- * [rows, outs] are contiguous.
+ * r_stride elements apart (0: one row for all; at most FWN_LINEAR_STRIDE_MAX, r_stride FWN_LINEAR_ACT_MAX); bias
+ * [outs], out and pre [rows, outs] are contiguous.
  * Products accumulate in float32; out, and pre (z for the backward, NULL: not stored) are rounded
  * once. bias and residual may be NULL. Every tensor is of `dtype`; float32 products keep float32's precision over
  * its whole range. No output of the launches here may overlap an input or another output. */
@@ -176,6 +176,7 @@ int fwn_rms_norm_bwd_launch(const fwn_rms_desc* d, const void* s, const void* we
 #define FWN_ACT_GELU_TANH 3 /* its tanh form */
 #define FWN_ACT_SILU 4      /* z / (1 + exp(-z)) */
 #define FWN_LINEAR_ACT_MAX (1 << 20) /* of ins and outs */
+#define FWN_LINEAR_STRIDE_MAX (1 << 30)
 
 typedef struct fwn_linear_desc {
   int64_t rows;
