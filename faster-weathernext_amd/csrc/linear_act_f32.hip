@@ -13,7 +13,7 @@
 // A workgroup is 4 waves on a 128 x 128 tile, a wave 64 x 64: per 16 k it reads 12 KB of LDS for 24 MFMAs. One
 // stage of 32 k is 48 KB of parts, so that two or three workgroups share a CU: while one splits and writes its next
 // stage, loaded a stage ahead into registers, the others multiply. A stage takes 2.0 us alone on a CU and 1.1 among
-// others (4,096 x 4,096 -> 4,096: 210 TFLOP/s). Where such tiles are too few, an inner a is taken in tiles of 64 x 128, of 1.1 us a
+// others (4,096 x 4,096 -> 4,096: 200 to 205 TFLOP/s). Where such tiles are too few, an inner a is taken in tiles of 64 x 128, of 1.1 us a
 // stage alone and 0.66 among others, us with 128 rows and with 64: 1,000 x 512 -> 512 22 and 17, 2,562 x 515 -> 1,027 43
 // and 36, 130 x 1,024 -> 1,024 16 and 13; 10,242 x 768 -> 3,072 260 and 286. Two stages in LDS (a stage split between the products
 // of the one before) were slower where tiles fill the chip: 337.

@@ -23,6 +23,9 @@ __global__ void __launch_bounds__(256) layout_kernel(LayoutArgs a) {
   }
 }
 
+// dz = g act'(pre). bf16: dz is the products' operand and so rounded to it, which costs the gradients as much again as their
+// own rounding (1,024 x 256 -> 1,024 with gelu_tanh: gx 2.34e-3 off, 1.65e-3 with dz left in float32); pre, kept in bf16 to
+// be half the bytes, adds little (2.39e-3). The sums are of dz before it is rounded.
 // 256 columns by `chunk` rows a workgroup, eight columns of every eighth row a thread: side by side where rows are whole
 // aligned eights (VEC), else 32 apart, so that a wave's accesses lie side by side. F32: the dtype is float32.
 template <int KIND, bool VEC, bool F32>

@@ -137,7 +137,8 @@ hipError_t launch(const ProductArgs& a, hipStream_t stream) {
 // 32 outputs a workgroup where 16 would be more workgroups than CUs: the rows of x are then read half as often. bf16, us
 // with 16 and with 32: 24 rows of 4,096 -> 4,096 12.5 and 15.9, of 5,120 -> 5,120 27.3 and 20.7, of 8,192 -> 8,192 40
 // and 31; one row of 3,072 -> 768 5.9 and 8.8, of 768 -> 3,072 3.5 and 4.6, of 5,120 -> 5,120 15.1 and 13.9 (3.8
-// TB/s), of 8,192 -> 8,192 23.3 (5.8 TB/s) and 26.4. From 33 rows on the tiles' kernels are quicker (48 rows
+// TB/s), of 8,192 -> 8,192 23.3 (5.8 TB/s) and 26.4: one row is quicker with 16 where they fill the chip evenly, which the rule
+// does not look at. From 33 rows on the tiles' kernels are quicker (48 rows
 // of 4,096 -> 4,096: 15.8 against 22).
 template <int OP>
 hipError_t launch_op(const ProductArgs& a, hipStream_t stream) {

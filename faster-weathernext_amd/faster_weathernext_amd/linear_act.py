@@ -144,7 +144,9 @@ def linear_act(x, weight, bias=None, *, activation=None, residual=None):
   [..., outs], all float32 or all bfloat16: a Linear layer with its activation (None, "relu", "gelu",
   "gelu_tanh" or "silu") and the residual's addition in the product's epilogue. Accumulated in float32 and
   rounded once. Rows of any stride are read where they lie if their channels are contiguous.
-  Differentiable in x, weight, bias and residual."""
+  Differentiable in x, weight, bias and residual. With an activation the backward keeps the pre-activation in the
+  tensors' dtype and rounds the gradient in front of it to that for its products: bfloat16 gradients are off by 2.4e-3
+  (relative) where the formula in float32, rounded once, is by 1.7e-3, as those of separate bfloat16 layers."""
   if not isinstance(x, torch.Tensor) or not x.is_cuda:
     raise ValueError("x must be a CUDA tensor")
   if x.dtype not in _DTYPES:
