@@ -1,14 +1,15 @@
 // The linear layers' products of float32 operands (gfx950), at float32's precision on the bf16 matrix units.
 //
-// A value times 2^16 is the exact sum of three bf16 parts: it rounded, what is left rounded, and the rest. The second is at most 2^-8
-// of the value and the third 2^-17, of either sign. Of the nine products of parts the six largest are formed and accumulated in
-// float32, small ones first; the three left out are together within 2^-24 (1 + 2^-9) of the product, as its rounding
-// to float32 would be, and without a direction. (Parts cut off rather than rounded took as long, lost up to 2^-21 of a
-// product and always towards zero.) The factor puts the last bits of the least float32 numbers, 2^-149, at bf16's own,
+// A value times 2^16 is the exact sum of three bf16 parts: it rounded, what is left rounded, and the rest. The second is at
+// most 2^-8 of the value and the third 2^-17, of either sign. Of the nine products of parts the six largest are formed and
+// accumulated in float32, small ones first; the three left out are together within 2^-24 (1 + 2^-9) of the product, as its
+// rounding to float32 would be, and without a direction. (Parts cut off rather than rounded took as long, lost up to 2^-21
+// of a product and always towards zero.) The factor puts the last bits of the least float32 numbers, 2^-149, at bf16's own,
 // 2^-133: without it what lies below is lost, 1e-4 of values of 1e-37. Sums carry 2^32, which the epilogue takes back; where
-// that or the factor leaves float32's range (sums from 2^96 on, operands from 2^111), outputs come out infinite or NaN and are
-// formed anew of the whole values, as those that an infinity feeds. Six bf16 MFMAs do what eight times as many clocks of float32 MFMAs do. The parts are
-// formed on the way from memory to LDS, so an operand of any strides and alignment is read where it lies, once a tile.
+// that or the factor leaves float32's range (sums from 2^96 on, operands from 2^111), outputs come out infinite or NaN and
+// are formed anew of the whole values, as those that an infinity feeds. Six bf16 MFMAs do what eight times as many clocks
+// of float32 MFMAs do. The parts are formed on the way from memory to LDS, so an operand of any strides and alignment is
+// read where it lies, once a tile.
 //
 // A workgroup is 4 waves on a 128 x 128 tile, a wave 64 x 64: per 16 k it reads 12 KB of LDS for 24 MFMAs. One
 // stage of 32 k is 48 KB of parts, so that two or three workgroups share a CU: while one splits and writes its next
