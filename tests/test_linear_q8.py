@@ -125,3 +125,19 @@ def test_codes_that_need_a_gradient_are_refused():
       fwn.linear_act_q8(a, one(40), b, one(24))
     with torch.no_grad():
       assert fwn.linear_act_q8(a, one(40), b, one(24)).shape == (40, 24)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("outs", [1000, 1027])
+def test_many_rows(outs, dtype):
+  """Enough rows for the largest tiles, in whole eights of outputs and not: small whole numbers, to the bit."""
+  rows, ins = 30001, 1024
+  whole = lambda shape, seed: torch.randint(-2, 3, shape, generator=_gen(seed)).float().to(DEV)
+  x, w, b, r = whole((rows, ins), 1), whole((outs, ins), 2), whole((outs,), 3).to(dtype), whole((rows, outs), 4).to(dtype)
+  one = lambda n: torch.ones(n, device=DEV)
+  z = x.double() @ w.double().t()
+  for bias, res in ((None, None), (b, None), (b, r)):
+    want = z + (0 if bias is None else bias.double()) + (0 if res is None else res.double())
+    got = fwn.linear_act_q8(x.to(E4M3), one(rows), w.to(E4M3), one(outs), bias, residual=res, dtype=dtype)
+    assert torch.equal(got, want.to(dtype))
