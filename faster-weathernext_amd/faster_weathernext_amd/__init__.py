@@ -10,6 +10,7 @@ op contract, computed by hand-written gfx950 HIP kernels behind a C ABI (include
 """
 
 from . import patch
+from .dropout import dropout
 from .hip_attn import (BLOCK_K, BLOCK_Q, TileList, attention_backward, attention_forward, tiled_flash_attention,
                        tiled_flash_attention_qkv)
 from .linear_act import linear_act, linear_act_q8
@@ -17,6 +18,7 @@ from .mesh import adjacency, build_tile_mask, hilbert_order, icosahedral_mesh, k
 from .mha import TiledMHA
 from .rms import add_rms_norm, add_rms_norm_q8, quantize_rows, rms_norm, rms_norm_q8
 from .rows import gather_layer_norm, layer_norm_scatter
+from .sandwich import sandwich_norm
 from .transformer import MeshBlock, MeshTransformer
 from .tile_cache import cached_khop_tiles, cached_tile_mask
 

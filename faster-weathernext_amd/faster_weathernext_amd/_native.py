@@ -87,9 +87,26 @@ class LinearDesc(ctypes.Structure):
               ("activation", ctypes.c_int32)]
 
 
+class Dropout(ctypes.Structure):
+  _fields_ = [("p", ctypes.c_double), ("seed", ctypes.c_uint64), ("offset", ctypes.c_uint64), ("state", ctypes.c_void_p)]
+
+
+class DropoutDesc(ctypes.Structure):
+  _fields_ = [("rows", ctypes.c_int64), ("x_stride", ctypes.c_int64), ("r_stride", ctypes.c_int64),
+              ("channels", ctypes.c_int32), ("dtype", ctypes.c_int32), ("drop", Dropout)]
+
+
+class SandwichDesc(ctypes.Structure):
+  _fields_ = [("rows", ctypes.c_int64), ("gate_rows", ctypes.c_int64), ("x_stride", ctypes.c_int64),
+              ("y_stride", ctypes.c_int64), ("channels", ctypes.c_int32), ("dtype", ctypes.c_int32),
+              ("gate_dtype", ctypes.c_int32), ("post_dtype", ctypes.c_int32), ("pre_dtype", ctypes.c_int32),
+              ("post_norm", ctypes.c_int32), ("eps", ctypes.c_float), ("scale", ctypes.c_float), ("drop", Dropout)]
+
+
 ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}  # FWN_ACT_*
 LINEAR_ACT_MAX = 1 << 20  # FWN_LINEAR_ACT_MAX
 LINEAR_STRIDE_MAX = 1 << 30  # FWN_LINEAR_STRIDE_MAX
+DROPOUT_MAX_CHANNELS = 1 << 30  # FWN_DROPOUT_MAX_CHANNELS
 RMS_MAX_CHANNELS = 16384  # FWN_RMS_MAX_CHANNELS
 ROWS_MAX_CHANNELS = 4096  # FWN_ROWS_MAX_CHANNELS
 COND_MAX = 64  # FWN_COND_MAX: norms of one fwn_cond_affine_launch
@@ -104,6 +121,8 @@ _ROWS = ctypes.POINTER(RowsDesc)
 _DS = ctypes.POINTER(DsMap)
 _RMS = ctypes.POINTER(RmsDesc)
 _LIN = ctypes.POINTER(LinearDesc)
+_DROP = ctypes.POINTER(DropoutDesc)
+_SAND = ctypes.POINTER(SandwichDesc)
 
 # name -> argtypes, every entry point of include/fwn_attn.h and include/fwn_rows.h
 SIGNATURES = {
@@ -151,6 +170,10 @@ SIGNATURES = {
     "fwn_quantize_rows_launch": [_RMS, _P, _P, _P, _P],
     "fwn_rms_norm_bwd_workspace_size": [_RMS, _P],
     "fwn_rms_norm_bwd_launch": [_RMS, _P, _P, _P, _P, _P, _P, _P, _U64, _P],
+    "fwn_dropout_launch": [_DROP, _P, _P, _P, _P],
+    "fwn_sandwich_norm_launch": [_SAND, _P, _P, _P, _P, _P, _P, _P, _P],
+    "fwn_sandwich_norm_bwd_workspace_size": [_SAND, _I32, _P],
+    "fwn_sandwich_norm_bwd_launch": [_SAND, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _U64, _P],
     "fwn_linear_act_workspace_size": [_LIN, _P, _P, _P],
     "fwn_linear_act_launch": [_LIN, _P, _P, _P, _P, _P, _P, _P, _U64, _P],
     "fwn_linear_act_bwd_workspace_size": [_LIN, _P, _P, _P, _P, _P, _P, _P],

@@ -162,6 +162,70 @@ int fwn_rms_norm_bwd_launch(const fwn_rms_desc* d, const void* s, const void* we
                             const void* g_sum, void* gx, void* gw, void* workspace, uint64_t workspace_bytes,
                             void* stream);
 
+/* Dropout of rows with a residual: out[i, c] = kept(i, c) ? x[i, c] m : 0, plus residual[i, c] (NULL: 0), in float32 and
+ * rounded once to the dtype. With T = p 2^16 to the nearest whole number, m = 2^16 / (2^16 - T) in float32, and channel c of row i is
+ * kept if its 16 random bits are T or more: the halves, low one first, of the four words of Philox-4x32-10 (Salmon, Moraes,
+ * Dror and Shaw 2011) with the seed's halves as its key and (c / 8, i, the offset's halves) as its counter. Nothing about what is kept is
+ * stored; the same launch over the gradient of out, without a residual, is the gradient of x. Dropped values are zeros, whatever
+ * they were. state, if not NULL, holds {seed, offset} in the GPU's memory, read when the kernel runs, and the two
+ * members are not used. Rows are `channels` elements with stride 1; row i of x begins at i * x_stride elements, of residual
+ * likewise, out is contiguous. out may be x or the residual where that is contiguous, and must not overlap either otherwise. */
+#define FWN_DROPOUT_MAX_CHANNELS (1 << 30)
+
+typedef struct fwn_dropout {
+  double p;              /* 0 to 1 */
+  uint64_t seed, offset;
+  const uint64_t* state; /* 8-byte aligned, or NULL */
+} fwn_dropout;
+
+typedef struct fwn_dropout_desc {
+  int64_t rows;          /* less than 2^32 */
+  int64_t x_stride, r_stride;
+  int32_t channels;      /* 1 to FWN_DROPOUT_MAX_CHANNELS */
+  int32_t dtype;
+  fwn_dropout drop;
+} fwn_dropout_desc;
+
+int fwn_dropout_launch(const fwn_dropout_desc* d, const void* x, const void* residual, void* out, void* stream);
+
+/* The root-mean-square norms after a block and before the next one, with the block's gate, the residual's scale and dropout between them.
+ * For rows x of the residual and y of the block's output,
+ *   r1 = 1 / sqrt(mean(y^2) + eps),  b = gate y r1 post_weight,  s = scale x + dropout(b)
+ *   r2 = 1 / sqrt(mean(s^2) + eps),  out = s r2 pre_weight
+ * s is formed in float32 and stored rounded once in sum; the second norm is of the stored rows. Without post_norm r1 is 1.
+ * NULL weights and a NULL gate are 1. Row i of gate [rows / gate_rows, channels] is that of the rows i gate_rows .. (i + 1)
+ * gate_rows - 1: gate_rows is `rows` for one gate, 1 for a gate of x's shape, and divides rows. Rows of x and y are
+ * `channels` elements with stride 1, x_stride and y_stride elements apart; every other tensor is contiguous. Outputs must not overlap each
+ * other or an input. */
+typedef struct fwn_sandwich_desc {
+  int64_t rows;                            /* less than 2^32 */
+  int64_t gate_rows;                       /* not read without a gate */
+  int64_t x_stride, y_stride;
+  int32_t channels;                        /* 1 to FWN_RMS_MAX_CHANNELS */
+  int32_t dtype;                           /* of x, y, sum, out and their gradients */
+  int32_t gate_dtype, post_dtype, pre_dtype; /* the dtype, or FWN_F32, also of the tensor's gradient */
+  int32_t post_norm;                       /* 0 or 1 */
+  float eps, scale;                        /* eps finite and >= 0, scale finite */
+  fwn_dropout drop;                        /* p = 0: none */
+} fwn_sandwich_desc;
+
+int fwn_sandwich_norm_launch(const fwn_sandwich_desc* d, const void* x, const void* y, const void* gate, const void* post_weight,
+                             const void* pre_weight, void* sum, void* out, void* stream);
+
+/* Its backward at the contiguous rows s = sum, with a = g_out pre_weight, g = g_sum + r2 (a - s r2^2 mean(a s)) and
+ * d = dropout(g):
+ *   gx = scale g,  gy = r1 (c - y r1^2 mean(c y)) with c = d gate post_weight (without post_norm c)
+ *   g_gate = sums of d y r1 post_weight over the rows of each row of gate
+ *   g_post = sum of d gate y r1,  g_pre = sum of g_out s r2, both over the rows
+ * g_sum and g_out may be NULL (zeros), and each output may be NULL (not wanted). The workspace
+ * (fwn_sandwich_norm_bwd_workspace_size bytes, 16-byte aligned) is needed where one of g_gate (of more than one row each),
+ * g_post and g_pre is; the query takes whether g_gate is wanted. Sums run in a fixed order. */
+int fwn_sandwich_norm_bwd_workspace_size(const fwn_sandwich_desc* d, int32_t gate_gradient, uint64_t* bytes);
+int fwn_sandwich_norm_bwd_launch(const fwn_sandwich_desc* d, const void* s, const void* y, const void* gate,
+                                 const void* post_weight, const void* pre_weight, const void* g_sum, const void* g_out, void* gx,
+                                 void* gy, void* g_gate, void* g_post, void* g_pre, void* workspace, uint64_t workspace_bytes,
+                                 void* stream);
+
 /* Matrix product with bias, activation and residual in its epilogue:
  *   z = x weight^T + bias,  out = act(z) + residual
  * x is [rows, ins], weight [outs, ins], residual [rows, outs], with contiguous rows x_stride, w_stride and
