@@ -7,6 +7,7 @@
 #include "fwn_internal.h"
 #include "fwn_rows.h"
 #include "linear_act.h"
+#include "linear_q4.h"
 
 namespace fwn {
 namespace {
@@ -282,6 +283,27 @@ struct Backward {
   }
 };
 
+// The same with a weight of 4 bits: widened in the workspace where the tiles' kernels take it, read as it is for few rows.
+struct ForwardQ4 {
+  Matrix x, w{};
+  Product z;
+  int64_t groups;
+  uint64_t bytes;
+
+  ForwardQ4(const fwn_linear_desc* d, const void* xp, void* workspace) {
+    Workspace ws{(char*)workspace};
+    const int32_t op = d->dtype == FWN_F32 ? kOpF32 : kOpBf16;
+    groups = parts(d->ins, FWN_Q4_GROUP);
+    x.place(xp, d->rows, d->ins, d->x_stride, op, ws);
+    z.shape(Operands::kInnerInner, d->rows, d->outs, d->ins, op, d->dtype, false, ws);
+    if (!z.few) {
+      w.row_bytes = groups * FWN_Q4_GROUP * op_size(op);
+      w.at = ws.take((uint64_t)d->outs * (uint64_t)w.row_bytes);
+    }
+    bytes = ws.used;
+  }
+};
+
 int size_query(const fwn_linear_desc* d, uint64_t* bytes, const char* what) {
   clear_error();
   if (!bytes) return fail(FWN_ERR_INVALID_ARG, "%s: null argument", what);
@@ -324,6 +346,72 @@ int fwn_linear_act_q8_launch(const fwn_linear_desc* d, const uint8_t* x, const f
   clear_error();
   return forward(d, kOpE4m3, x, x_scale, weight, w_scale, bias, residual, out, nullptr, workspace, workspace_bytes,
                  stream, "fwn_linear_act_q8_launch");
+}
+
+int fwn_quantize_q4_launch(int64_t rows, int32_t ins, int64_t x_stride, int32_t dtype, const void* x, uint8_t* codes,
+                           uint8_t* scales, void* stream) {
+  using namespace fwn;
+  clear_error();
+  const char* what = "fwn_quantize_q4_launch";
+  if (dtype != FWN_F32 && dtype != FWN_BF16) return fail(FWN_ERR_UNSUPPORTED, "%s: dtype must be f32 or bf16", what);
+  if (ins < 1 || ins > FWN_LINEAR_ACT_MAX) return fail(FWN_ERR_INVALID_ARG, "%s: ins %d must be 1 to %d", what, ins, FWN_LINEAR_ACT_MAX);
+  if (rows < 0 || rows > FWN_LINEAR_ACT_MAX || x_stride < 0 || x_stride > FWN_LINEAR_STRIDE_MAX)
+    return fail(FWN_ERR_INVALID_ARG, "%s: %lld rows, stride %lld", what, (long long)rows, (long long)x_stride);
+  if (rows == 0) return FWN_OK;
+  if (!x || !codes || !scales) return fail(FWN_ERR_INVALID_ARG, "%s: null argument", what);
+  const uint64_t size = size_of(dtype);
+  if (misaligned(x, size) || misaligned(codes, 16)) return fail(FWN_ERR_INVALID_ARG, "%s: a tensor is not aligned", what);
+  const int64_t groups = parts(ins, FWN_Q4_GROUP);
+  const Span in[] = {span(x, rows, x_stride, ins, size)};
+  const Span outs[] = {span(codes, rows, groups * 16, groups * 16, 1), span(scales, rows, groups, groups, 1)};
+  if (int rc = check_overlap(in, outs, what)) return rc;
+  return status(launch_quantize_q4(dtype, {x, codes, scales, rows, ins, x_stride}, (hipStream_t)stream), what);
+}
+
+int fwn_linear_act_q4_workspace_size(const fwn_linear_desc* d, const void* x, uint64_t* bytes) {
+  using namespace fwn;
+  if (int rc = size_query(d, bytes, "fwn_linear_act_q4_workspace_size")) return rc;
+  *bytes = ForwardQ4(d, x, nullptr).bytes;
+  return FWN_OK;
+}
+
+int fwn_linear_act_q4_launch(const fwn_linear_desc* d, const void* x, const uint8_t* codes, const uint8_t* scales,
+                             const void* bias, const void* residual, void* out, void* workspace, uint64_t workspace_bytes,
+                             void* stream) {
+  using namespace fwn;
+  clear_error();
+  const char* what = "fwn_linear_act_q4_launch";
+  if (int rc = check_desc(d, what)) return rc;
+  if (d->rows == 0) return FWN_OK;
+  if (!x || !codes || !scales || !out) return fail(FWN_ERR_INVALID_ARG, "%s: null argument", what);
+  const uint64_t size = size_of(d->dtype);
+  if (misaligned(x, size) || misaligned(codes, 16) || misaligned(bias, size) || misaligned(residual, size) || misaligned(out, size))
+    return fail(FWN_ERR_INVALID_ARG, "%s: a tensor is not aligned", what);
+  ForwardQ4 f(d, x, workspace);
+  if (int rc = check_workspace(workspace, workspace_bytes, f.bytes, what)) return rc;
+  const Span ins[] = {span(x, d->rows, d->x_stride, d->ins, size), span(codes, d->outs, f.groups * 16, f.groups * 16, 1),
+                      span(scales, d->outs, f.groups, f.groups, 1), span(bias, 1, 0, d->outs, size),
+                      span(residual, d->rows, d->r_stride, d->outs, size)};
+  const Span outs[] = {span(out, d->rows, d->outs, d->outs, size), {workspace, f.bytes}};
+  if (int rc = check_overlap(ins, outs, what)) return rc;
+  EpilogueArgs& e = f.z.g.e;
+  e.bias = bias;
+  e.residual = residual;
+  e.r_row = d->r_stride;
+  e.out = out;
+  e.dtype = d->dtype;
+  e.activation = d->activation;
+  const hipStream_t s = (hipStream_t)stream;
+  const bool f32 = d->dtype == FWN_F32;
+  if (int rc = status(f.x.lay_out(s), what)) return rc;
+  if (f.z.few) {
+    Q4Args a{f.z.g, codes, scales, f.groups};
+    a.p.a = f.x.at;
+    a.p.a_stride = f.x.row_bytes;
+    return status(launch_q4_rows(f32, a, s), what);
+  }
+  if (int rc = status(launch_widen(f32, {codes, scales, f.w.at, d->outs, d->ins, f.groups}, s), what)) return rc;
+  return status(f.z.launch(f.x, f.w, s), what);
 }
 
 int fwn_linear_act_bwd_workspace_size(const fwn_linear_desc* d, const void* x, const void* weight, const void* g,

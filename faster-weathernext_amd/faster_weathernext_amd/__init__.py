@@ -14,6 +14,7 @@ from .dropout import dropout
 from .hip_attn import (BLOCK_K, BLOCK_Q, TileList, attention_backward, attention_forward, tiled_flash_attention,
                        tiled_flash_attention_qkv)
 from .linear_act import linear_act, linear_act_q8
+from .linear_q4 import linear_act_q4, quantize_q4
 from .mesh import adjacency, build_tile_mask, hilbert_order, icosahedral_mesh, khop_mask, mesh_mask
 from .mha import TiledMHA
 from .rms import add_rms_norm, add_rms_norm_q8, quantize_rows, rms_norm, rms_norm_q8

@@ -104,6 +104,7 @@ class SandwichDesc(ctypes.Structure):
 
 
 ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}  # FWN_ACT_*
+Q4_GROUP = 32  # FWN_Q4_GROUP
 LINEAR_ACT_MAX = 1 << 20  # FWN_LINEAR_ACT_MAX
 LINEAR_STRIDE_MAX = 1 << 30  # FWN_LINEAR_STRIDE_MAX
 DROPOUT_MAX_CHANNELS = 1 << 30  # FWN_DROPOUT_MAX_CHANNELS
@@ -179,6 +180,9 @@ SIGNATURES = {
     "fwn_linear_act_bwd_workspace_size": [_LIN, _P, _P, _P, _P, _P, _P, _P],
     "fwn_linear_act_bwd_launch": [_LIN, _P, _P, _P, _P, _P, _P, _P, _P, _U64, _P],
     "fwn_linear_act_q8_workspace_size": [_LIN, _P, _P, _P],
+    "fwn_quantize_q4_launch": [_I64, _I32, _I64, _I32, _P, _P, _P, _P],
+    "fwn_linear_act_q4_workspace_size": [_LIN, _P, _P],
+    "fwn_linear_act_q4_launch": [_LIN, _P, _P, _P, _P, _P, _P, _P, _U64, _P],
     "fwn_linear_act_q8_launch": [_LIN, _P, _P, _P, _P, _P, _P, _P, _P, _U64, _P],
 }
 

@@ -277,6 +277,25 @@ int fwn_linear_act_q8_launch(const fwn_linear_desc* d, const uint8_t* x, const f
                              const float* w_scale, const void* bias, const void* residual, void* out,
                              void* workspace, uint64_t workspace_bytes, void* stream);
 
+/* Weights of 4 bits with a scale for each group of FWN_Q4_GROUP inputs (the 4-bit format of the OCP microscaling
+ * specification): w[o, i] = value(code) 2^(scale - 127), the code's top bit the sign, the others 0, 0.5, 1, 1.5, 2, 3, 4 and 6. With
+ * groups = ceil(ins / FWN_Q4_GROUP), codes are [outs, 16 groups] bytes, 16-byte aligned, the even input of a pair in the low
+ * half; scales are [outs, groups], 255 meaning NaN. Codes past ins are not used. A weight of 2^128 or more is infinite.
+ *
+ * fwn_quantize_q4_launch: the codes and scales of rows of x, x_stride elements apart. A group's scale is the least power of two
+ * of which its largest magnitude is at most seven (beyond six is cut to six), its codes the nearest ones, middles to even codes.
+ * Groups with NaN or infinities have the scale NaN. Codes past ins are zeros. */
+#define FWN_Q4_GROUP 32
+int fwn_quantize_q4_launch(int64_t rows, int32_t ins, int64_t x_stride, int32_t dtype, const void* x, uint8_t* codes,
+                           uint8_t* scales, void* stream);
+
+/* fwn_linear_act_launch with such a weight, without pre; w_stride is not read. Products are exact and added in float32 (float32
+ * x as in fwn_linear_act_launch). */
+int fwn_linear_act_q4_workspace_size(const fwn_linear_desc* d, const void* x, uint64_t* bytes);
+int fwn_linear_act_q4_launch(const fwn_linear_desc* d, const void* x, const uint8_t* codes, const uint8_t* scales,
+                             const void* bias, const void* residual, void* out, void* workspace, uint64_t workspace_bytes,
+                             void* stream);
+
 #ifdef __cplusplus
 }  /* extern "C" */
 #endif
