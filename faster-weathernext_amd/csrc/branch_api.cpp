@@ -90,8 +90,8 @@ Span gate_of(const fwn_sandwich_desc* d, const void* gate) {
 }
 
 // Bytes of partial sums, whichever of the weights' gradients are wanted.
-uint64_t part_bytes(const fwn_sandwich_desc* d, bool gate_gradient) {
-  const SandwichGrid g = sandwich_grid(d->rows, d->gate_rows, d->channels, gate_gradient && d->gate_rows > 1);
+uint64_t part_bytes(const fwn_sandwich_desc* d, bool gate) {
+  const SandwichGrid g = sandwich_grid(d->rows, gate ? d->gate_rows : d->rows, d->channels, d->dtype);
   return (uint64_t)g.parts * (uint64_t)g.blocks * (uint64_t)d->channels * sizeof(float);
 }
 
@@ -173,7 +173,7 @@ int fwn_sandwich_norm_launch(const fwn_sandwich_desc* d, const void* x, const vo
   return status(launch_sandwich(d->dtype, a, (hipStream_t)stream), what);
 }
 
-int fwn_sandwich_norm_bwd_workspace_size(const fwn_sandwich_desc* d, int32_t gate_gradient, uint64_t* bytes) {
+int fwn_sandwich_norm_bwd_workspace_size(const fwn_sandwich_desc* d, int32_t gate, uint64_t* bytes) {
   using namespace fwn;
   clear_error();
   const char* what = "fwn_sandwich_norm_bwd_workspace_size";
@@ -181,9 +181,9 @@ int fwn_sandwich_norm_bwd_workspace_size(const fwn_sandwich_desc* d, int32_t gat
   *bytes = 0;
   DropoutArgs draw;
   if (int rc = check_sandwich(d, draw, what)) return rc;
-  if (gate_gradient)
+  if (gate)
     if (int rc = check_gate(d, what)) return rc;
-  *bytes = part_bytes(d, gate_gradient != 0);
+  *bytes = part_bytes(d, gate != 0);
   return FWN_OK;
 }
 
@@ -210,7 +210,7 @@ int fwn_sandwich_norm_bwd_launch(const fwn_sandwich_desc* d, const void* s, cons
     return fail(FWN_ERR_INVALID_ARG, "%s: a tensor is not aligned to its elements", what);
   const auto rows = [&](const void* p, int64_t stride) { return rows_of(p, d->rows, stride, d->channels, size); };
   const bool part = g_post || g_pre || (g_gate && d->gate_rows > 1);
-  const uint64_t need = part ? part_bytes(d, g_gate != nullptr) : 0;
+  const uint64_t need = part ? part_bytes(d, gate != nullptr) : 0;
   if (need > 0 && (!workspace || misaligned(workspace, 16) || workspace_bytes < need))
     return fail(FWN_ERR_INVALID_ARG, "%s: a 16-byte aligned workspace of %llu bytes is needed", what, (unsigned long long)need);
   const Span ins[] = {rows(s, d->channels), rows(y, d->y_stride), gate_of(d, gate), {post_weight, c * post_size},

@@ -69,14 +69,14 @@ struct SandwichBwdArgs {
   bool stream;  // set by the launch: non-temporal stores
   DropoutArgs draw;
 };
-// The workgroups of the backward pass: groups of rows that share a gate's row (one group if the sums of the gate's gradient
-// are not wanted) go to `per` workgroups each, or several to one.
+// The workgroups of the backward pass: groups of rows that share a gate's row (one group without a gate, and with one of x's
+// shape: gate_rows 1) go to `per` workgroups each, or several to one.
 struct SandwichGrid {
   int64_t groups, group_rows;
   int32_t blocks, per, of_block;  // workgroups a group, groups a workgroup; one of the two is 1
   int32_t parts;                  // partial sums a workgroup leaves: of pre_weight's, post_weight's and the gate's gradients
 };
-SandwichGrid sandwich_grid(int64_t rows, int64_t gate_rows, int32_t channels, bool gate_sums);
+SandwichGrid sandwich_grid(int64_t rows, int64_t gate_rows, int32_t channels, int32_t dtype);
 hipError_t launch_sandwich_bwd(int dtype, const SandwichBwdArgs& a, hipStream_t stream);
 
 }  // namespace fwn

@@ -40,18 +40,26 @@ struct Draw {
     }
   }
 
-  // f of the channels col .. col + E - 1 (a vector of the row: col is a multiple of E): times `keep`, or zero whatever it was.
+  // f of the channels col .. col + E - 1 (a vector of the row: col is a multiple of E): itself, or zero whatever it was.
   template <int E>
-  __device__ __forceinline__ void apply(uint32_t row, uint32_t col, float (&f)[E]) const {
+  __device__ __forceinline__ void select(uint32_t row, uint32_t col, float (&f)[E]) const {
     uint32_t c[4];
     block(row, col / 8, c);
     // A vector of four has one half of the words, chosen by value (an index that varies would put them into memory).
     const uint32_t w[4] = {E == 4 && (col & 4) ? c[2] : c[0], E == 4 && (col & 4) ? c[3] : c[1], c[2], c[3]};
 #pragma unroll
     for (int e = 0; e < E; e += 2) {
-      f[e] = (w[e / 2] & 0xffffu) >= border ? f[e] * keep : 0.f;
-      f[e + 1] = (w[e / 2] >> 16) >= border ? f[e + 1] * keep : 0.f;
+      f[e] = (w[e / 2] & 0xffffu) >= border ? f[e] : 0.f;
+      f[e + 1] = (w[e / 2] >> 16) >= border ? f[e + 1] : 0.f;
     }
+  }
+
+  // The same times `keep`.
+  template <int E>
+  __device__ __forceinline__ void apply(uint32_t row, uint32_t col, float (&f)[E]) const {
+#pragma unroll
+    for (int e = 0; e < E; ++e) f[e] *= keep;
+    select(row, col, f);
   }
 };
 

@@ -27,6 +27,53 @@ struct Bits<float> {
   typedef uint32_t type;
 };
 
+// Sums over the TPR threads of a row, by every one of them; fixed order. Within 16 lanes by rotations, beyond by swaps of rows and
+// halves of the wave, none of which takes a trip through LDS as __shfl_xor does (40,968 x 768 bf16 with dropout, backward: 97 us, with
+// __shfl_xor 103; forward of 40,962 x 768 57 and 60).
+template <int ROTATE>
+__device__ __forceinline__ float rotated(float v) {
+  return as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)as_bits(v), 0x120 + ROTATE, 0xf, 0xf, false));
+}
+template <int TPR>
+__device__ __forceinline__ float wave_sum(float v) {
+  v += rotated<8>(v);
+  v += rotated<4>(v);
+  v += rotated<2>(v);
+  v += rotated<1>(v);
+  if constexpr (TPR >= 32) {
+    const auto r = __builtin_amdgcn_permlane16_swap(as_bits(v), as_bits(v), false, false);
+    const uint32_t a = r[0], b = r[1];
+    v = as_float(a) + as_float(b);
+  }
+  if constexpr (TPR >= 64) {
+    const auto r = __builtin_amdgcn_permlane32_swap(as_bits(v), as_bits(v), false, false);
+    const uint32_t a = r[0], b = r[1];
+    v = as_float(a) + as_float(b);
+  }
+  return v;
+}
+template <int TPR, int N>
+__device__ __forceinline__ void all_sums(float (&v)[N], float* red) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = wave_sum<TPR>(v[i]);
+  if constexpr (TPR > 64) {
+    constexpr int WAVES = TPR / 64;
+    const int wave = (int)threadIdx.x >> 6, first = wave / WAVES * WAVES;  // of the row
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) red[N * wave + i] = v[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      v[i] = red[N * first + i];
+#pragma unroll
+      for (int w = 1; w < WAVES; ++w) v[i] += red[N * (first + w) + i];
+    }
+  }
+}
+
 // A gate's row of a row: 32-bit division, rows being fewer than 2^32.
 __device__ __forceinline__ int64_t gate_row(int64_t row, int64_t gate_rows, int64_t rows) {
   return gate_rows == 1 ? row : gate_rows >= rows ? 0 : (int64_t)((uint32_t)row / (uint32_t)gate_rows);
@@ -74,15 +121,16 @@ __global__ void __launch_bounds__(kThreads<TPR>) sandwich_kernel(SandwichArgs a)
     }
     float r = 1.f;
     if (a.post_norm) {
-      float sq = 0.f;
+      float sq[1] = {0.f};
 #pragma unroll
       for (int k = 0; k < VPT; ++k)
 #pragma unroll
-        for (int e = 0; e < E; ++e) sq = fmaf(b[k][e], b[k][e], sq);
-      r = 1.f / sqrtf(row_sum<TPR>(sq, red) * inv_c + a.eps);
+        for (int e = 0; e < E; ++e) sq[0] = fmaf(b[k][e], b[k][e], sq[0]);
+      all_sums<TPR>(sq, red);
+      r = 1.f / sqrtf(sq[0] * inv_c + a.eps);
     }
     const int64_t gate_at = a.gate && ok ? gate_row(row, a.gate_rows, a.rows) * a.channels : 0;
-    float sq = 0.f;
+    float sq[1] = {0.f};
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
       const int c = (t + TPR * k) * E;
@@ -102,9 +150,10 @@ __global__ void __launch_bounds__(kThreads<TPR>) sandwich_kernel(SandwichArgs a)
           if (e >= a.channels - c) f[k][e] = 0.f;
       }
 #pragma unroll
-      for (int e = 0; e < E; ++e) sq = fmaf(f[k][e], f[k][e], sq);
+      for (int e = 0; e < E; ++e) sq[0] = fmaf(f[k][e], f[k][e], sq[0]);
     }
-    r = 1.f / sqrtf(row_sum<TPR>(sq, red) * inv_c + a.eps);
+    all_sums<TPR>(sq, red);
+    r = 1.f / sqrtf(sq[0] * inv_c + a.eps);
     if (!ok) continue;
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
@@ -118,20 +167,22 @@ __global__ void __launch_bounds__(kThreads<TPR>) sandwich_kernel(SandwichArgs a)
   }
 }
 
-// Adds the sums that the workgroup's threads hold over the rows that it holds at once, in a fixed order, and hands
-// each to its channel's thread: give(channel, value).
+// Adds the sums that the workgroup's threads hold over the rows that it holds at once, in a fixed order, and hands them out: a
+// thread's own vectors where the workgroup has one row, else a channel a thread. give(channel, channels left, values).
 template <int TPR, int VPT, int E, typename Give>
 __device__ __forceinline__ void over_rows(const float (&v)[VPT][E], float* sums, int channels, const Give& give) {
   constexpr int RPW = kThreads<TPR> / TPR;
   const int t = (int)threadIdx.x % TPR, own = (int)threadIdx.x / TPR;
   if constexpr (RPW == 1) {
 #pragma unroll
-    for (int k = 0; k < VPT; ++k)
+    for (int k = 0; k < VPT; ++k) {
+      const int c = (t + TPR * k) * E;
+      float f[E];
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const int c = (t + TPR * k) * E + e;
-        if (c < channels) give(c, v[k][e]);
-      }
+      for (int e = 0; e < E; ++e) f[e] = v[k][e];
+      if (c < channels) give(c, channels - c, f);
+      __builtin_amdgcn_sched_barrier(0);
+    }
   } else {
     __syncthreads();
     for (int g = 0; g < RPW; ++g) {
@@ -146,7 +197,10 @@ __device__ __forceinline__ void over_rows(const float (&v)[VPT][E], float* sums,
       }
       __syncthreads();
     }
-    for (int c = threadIdx.x; c < channels; c += kThreads<TPR>) give(c, sums[c]);
+    for (int c = threadIdx.x; c < channels; c += kThreads<TPR>) {
+      float f[1] = {sums[c]};
+      give(c, channels - c, f);
+    }
   }
 }
 
@@ -173,29 +227,71 @@ __device__ __forceinline__ u32x4 take(const T* p, int left) {
   return load_raw<T, true>(p);
 }
 
-// SUMS: the gate's gradient is summed over rows. The sums of a workgroup's rows stay in its threads' registers; those of
-// the gate are handed on at the end of each group of rows.
-template <typename T, int TPR, int VPT, bool SUMS, bool TAIL>
-__global__ void __launch_bounds__(kThreads<TPR>) sandwich_bwd_kernel(SandwichBwdArgs a, SandwichGrid grid) {
+// The first `left` of N sums.
+template <int N>
+__device__ __forceinline__ void put_sums(float* p, int left, const float (&f)[N]) {
+  if constexpr (N % 4 == 0) {
+    if (left >= N) {
+#pragma unroll
+      for (int h = 0; h < N; h += 4) *(f32x4_any*)(p + h) = f32x4_any{as_bits(f[h]), as_bits(f[h + 1]), as_bits(f[h + 2]), as_bits(f[h + 3])};
+      return;
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < N; ++e)
+    if (e < left) p[e] = f[e];
+}
+
+// E weights from channel c times v; NULL: v.
+template <typename T, int E, bool TAIL>
+__device__ __forceinline__ void weights(const void* w, bool f32, int64_t c, int left, float v, float (&f)[E]) {
+#pragma unroll
+  for (int e = 0; e < E; ++e) f[e] = v;
+  times<T, E, TAIL>(w, f32, c, left, f);
+}
+
+// Waves a SIMD that the backward's registers leave room for.
+template <typename T, int TPR, int VPT>
+constexpr int kWaves = TPR == 1024 ? 4 : 16 / (int)sizeof(T) * VPT <= 8 ? 4 : 16 / (int)sizeof(T) * VPT <= 16 ? 3 : 2;
+
+// EACH: the gate is of x's shape. Else the rows go by groups that share a row of the gate (one group without a gate), whose
+// sum of db y r1 is both the gate's gradient but for post_weight and the group's share of post_weight's but for the gate: one sum in
+// registers, beside pre_weight's. What dropout multiplies by is part of the weights, not of db.
+template <typename T, int TPR, int VPT, bool EACH, bool TAIL>
+__global__ void __launch_bounds__(kThreads<TPR>) __attribute__((amdgpu_waves_per_eu(kWaves<T, TPR, VPT>))) sandwich_bwd_kernel(SandwichBwdArgs a, SandwichGrid grid) {
   constexpr int E = 16 / sizeof(T), RPW = kThreads<TPR> / TPR;
   __shared__ float red[32];
   __shared__ float sums[RPW > 1 ? TPR * VPT * E : 1];
   const int t = (int)threadIdx.x % TPR, own = (int)threadIdx.x / TPR;
   const float inv_c = 1.f / (float)a.channels;
   const Draw draw(a.draw);
-  float g_pre[VPT][E], g_post[VPT][E], g_gate[SUMS ? VPT : 1][E];
+  const float keep = a.drop ? draw.keep : 1.f;
+  float g_pre[VPT][E], q[VPT][E], pre[VPT][E], w[VPT][E];
 #pragma unroll
-  for (int k = 0; k < VPT; ++k)
+  for (int k = 0; k < VPT; ++k) {
+    const int c = (t + TPR * k) * E;
 #pragma unroll
-    for (int e = 0; e < E; ++e) g_pre[k][e] = g_post[k][e] = 0.f;
+    for (int e = 0; e < E; ++e) g_pre[k][e] = q[k][e] = pre[k][e] = w[k][e] = 0.f;
+    if (c >= a.channels) continue;
+    weights<T, E, TAIL>(a.pre_weight, a.pre_f32, c, a.channels - c, 1.f, pre[k]);
+    if (EACH) weights<T, E, TAIL>(a.post_weight, a.post_f32, c, a.channels - c, keep, w[k]);
+  }
+  float* const part_pre = a.part + (int64_t)blockIdx.x * a.channels;
+  float* const part_post = part_pre + (a.g_pre ? (int64_t)grid.blocks * a.channels : 0);
+  float* const part_gate = part_post + (a.g_post ? (int64_t)grid.blocks * a.channels : 0);
   const int64_t first = (int64_t)((int)blockIdx.x / grid.per) * grid.of_block;
   const int sub = (int)blockIdx.x % grid.per;
   for (int64_t group = first; group < first + grid.of_block && group < grid.groups; ++group) {
-    if constexpr (SUMS) {
+    if constexpr (!EACH) {
 #pragma unroll
-      for (int k = 0; k < VPT; ++k)
+      for (int k = 0; k < VPT; ++k) {
+        const int c = (t + TPR * k) * E;
 #pragma unroll
-        for (int e = 0; e < E; ++e) g_gate[k][e] = 0.f;
+        for (int e = 0; e < E; ++e) q[k][e] = 0.f;
+        if (c >= a.channels) continue;
+        weights<T, E, TAIL>(a.post_weight, a.post_f32, c, a.channels - c, keep, w[k]);
+        times<T, E, TAIL>(a.gate, a.gate_f32, group * a.channels + c, a.channels - c, w[k]);
+      }
     }
     const int64_t begin = group * grid.group_rows, end = begin + grid.group_rows;
     for (int64_t row0 = begin + sub * RPW; row0 < end; row0 += grid.per * RPW) {
@@ -216,127 +312,127 @@ __global__ void __launch_bounds__(kThreads<TPR>) sandwich_bwd_kernel(SandwichBwd
       }
       float r2 = 0.f, k2 = 0.f;
       if (a.g_out) {
-        float sq = 0.f, as = 0.f;  // of s^2, and of a s
+        float m[2] = {0.f, 0.f};  // s^2, and a s
 #pragma unroll
         for (int k = 0; k < VPT; ++k) {
-          const int c = (t + TPR * k) * E;
           float s[E], h[E];
           unpack<T>(vs[k], s);
           unpack<T>(vo[k], h);
-          if (ok && c < a.channels) times<T, E, TAIL>(a.pre_weight, a.pre_f32, c, a.channels - c, h);
 #pragma unroll
           for (int e = 0; e < E; ++e) {
-            sq = fmaf(s[e], s[e], sq);
-            as = fmaf(h[e], s[e], as);
+            m[0] = fmaf(s[e], s[e], m[0]);
+            m[1] = fmaf(h[e] * pre[k][e], s[e], m[1]);
           }
         }
-        row_sums<TPR>(sq, as, red);
-        r2 = 1.f / sqrtf(sq * inv_c + a.eps);
-        k2 = as * inv_c * r2 * r2;
+        all_sums<TPR>(m, red);
+        r2 = 1.f / sqrtf(m[0] * inv_c + a.eps);
+        k2 = m[1] * inv_c * r2 * r2;
       }
-      const int64_t gate_at = a.gate && ok ? gate_row(row, a.gate_rows, a.rows) * a.channels : 0;
-      float db[VPT][E], yy = 0.f, cy = 0.f;  // of y^2, and of c y
+      float db[VPT][E], m[2] = {0.f, 0.f};  // y^2, and c y
 #pragma unroll
       for (int k = 0; k < VPT; ++k) {
         const int c = (t + TPR * k) * E, left = a.channels - c;
 #pragma unroll
         for (int e = 0; e < E; ++e) db[k][e] = 0.f;
         if (!ok || left <= 0) continue;
-        float ds[E];
-        unpack<T>(vg[k], ds);
+        unpack<T>(vg[k], db[k]);
         if (a.g_out) {
           float s[E], h[E];
           unpack<T>(vs[k], s);
           unpack<T>(vo[k], h);
 #pragma unroll
-          for (int e = 0; e < E; ++e) g_pre[k][e] = fmaf(h[e], s[e] * r2, g_pre[k][e]);
-          times<T, E, TAIL>(a.pre_weight, a.pre_f32, c, left, h);
-#pragma unroll
-          for (int e = 0; e < E; ++e) ds[e] = fmaf(r2, h[e] - s[e] * k2, ds[e]);
+          for (int e = 0; e < E; ++e) {
+            g_pre[k][e] = fmaf(h[e], s[e] * r2, g_pre[k][e]);
+            db[k][e] = fmaf(r2, fmaf(-k2, s[e], h[e] * pre[k][e]), db[k][e]);
+          }
         }
         if (a.gx) {
           float o[E];
 #pragma unroll
-          for (int e = 0; e < E; ++e) o[e] = a.scale * ds[e];
+          for (int e = 0; e < E; ++e) o[e] = a.scale * db[k][e];
           put<T, E, TAIL>(a.stream, (T*)a.gx + at + c, left, o);
         }
-        if (a.drop) draw.template apply<E>((uint32_t)row, (uint32_t)c, ds);
-#pragma unroll
-        for (int e = 0; e < E; ++e) db[k][e] = ds[e];
-        if (!a.post_norm) continue;
-        float y[E];
+        if (a.drop) draw.template select<E>((uint32_t)row, (uint32_t)c, db[k]);
+        float y[E], g[E];
         unpack<T>(vy[k], y);
-        times<T, E, TAIL>(a.gate, a.gate_f32, gate_at + c, left, ds);
-        times<T, E, TAIL>(a.post_weight, a.post_f32, c, left, ds);
+        if constexpr (EACH) {
+#pragma unroll
+          for (int e = 0; e < E; ++e) g[e] = w[k][e];
+          times<T, E, TAIL>(a.gate, a.gate_f32, at + c, left, g);
+        }
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-          yy = fmaf(y[e], y[e], yy);
-          cy = fmaf(ds[e], y[e], cy);
+          m[0] = fmaf(y[e], y[e], m[0]);
+          m[1] = fmaf(db[k][e] * (EACH ? g[e] : w[k][e]), y[e], m[1]);
         }
       }
       float r1 = 1.f, k1 = 0.f;
       if (a.post_norm) {
-        row_sums<TPR>(yy, cy, red);
-        r1 = 1.f / sqrtf(yy * inv_c + a.eps);
-        k1 = cy * inv_c * r1 * r1;
+        all_sums<TPR>(m, red);
+        r1 = 1.f / sqrtf(m[0] * inv_c + a.eps);
+        k1 = m[1] * inv_c * r1 * r1;
       }
       if (!ok) continue;
 #pragma unroll
       for (int k = 0; k < VPT; ++k) {
         const int c = (t + TPR * k) * E, left = a.channels - c;
         if (left <= 0) continue;
-        float unit[E], d[E], o[E];
-        unpack<T>(vy[k], unit);
+        float y[E], o[E];
+        unpack<T>(vy[k], y);
+        if constexpr (EACH) {
+          // The gate's gradient, and db times the gate in place of db.
+          float g[E];
+          weights<T, E, TAIL>(a.gate, a.gate_f32, at + c, left, 1.f, g);
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          o[e] = unit[e] * k1;
-          unit[e] *= r1;
-          d[e] = db[k][e];
-        }
-        times<T, E, TAIL>(a.gate, a.gate_f32, gate_at + c, left, d);
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          g_post[k][e] = fmaf(d[e], unit[e], g_post[k][e]);
-          if constexpr (SUMS) g_gate[k][e] = fmaf(db[k][e], unit[e], g_gate[k][e]);
-        }
-        if (a.gy) {
-          times<T, E, TAIL>(a.post_weight, a.post_f32, c, left, d);
-          if (a.post_norm) {
-#pragma unroll
-            for (int e = 0; e < E; ++e) d[e] = r1 * (d[e] - o[e]);
+          for (int e = 0; e < E; ++e) {
+            o[e] = db[k][e] * w[k][e] * (y[e] * r1);
+            db[k][e] *= g[e];
           }
-          put<T, E, TAIL>(a.stream, (T*)a.gy + at + c, left, d);
-        }
-        if (!SUMS && a.g_gate) {
+          if (a.g_gate) {
+            if (sizeof(T) == 4 || !a.gate_f32) {
+              put<T, E, TAIL>(a.stream, (T*)a.g_gate + at + c, left, o);
+            } else {
 #pragma unroll
-          for (int e = 0; e < E; ++e) unit[e] *= db[k][e];
-          times<T, E, TAIL>(a.post_weight, a.post_f32, c, left, unit);
-          if (sizeof(T) == 4 || !a.gate_f32) {
-            put<T, E, TAIL>(a.stream, (T*)a.g_gate + at + c, left, unit);
-          } else {
-#pragma unroll
-            for (int e = 0; e < E; ++e)
-              if (!TAIL || e < left) ((float*)a.g_gate)[at + c + e] = unit[e];
+              for (int e = 0; e < E; ++e)
+                if (!TAIL || e < left) ((float*)a.g_gate)[at + c + e] = o[e];
+            }
           }
         }
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          q[k][e] = fmaf(db[k][e], y[e] * r1, q[k][e]);
+          o[e] = db[k][e] * w[k][e];
+          if (a.post_norm) o[e] = r1 * fmaf(-k1, y[e], o[e]);
+        }
+        if (a.gy) put<T, E, TAIL>(a.stream, (T*)a.gy + at + c, left, o);
       }
     }
-    if constexpr (SUMS) {
-      float* const part = a.part + ((int64_t)(grid.parts - 1) * grid.blocks + blockIdx.x) * a.channels;
-      over_rows<TPR>(g_gate, sums, a.channels, [&](int c, float v) {
-        if (grid.per > 1)
-          part[c] = v;
-        else
-          put_weight(a.g_gate, a.gate_f32, group * a.channels + c, a.post_weight ? v * weight_at(a.post_weight, a.post_f32, c) : v);
+    if (!EACH && (a.g_post || a.g_gate)) {
+      over_rows<TPR>(q, sums, a.channels, [&](int c, int left, auto& v) {
+        constexpr int N = sizeof(v) / sizeof(float);
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[e] *= keep;
+        if (a.g_gate && grid.per > 1) put_sums<N>(part_gate + c, left, v);
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          if (e >= left) break;
+          if (a.g_gate && grid.per == 1)
+            put_weight(a.g_gate, a.gate_f32, group * a.channels + c + e,
+                       a.post_weight ? v[e] * weight_at(a.post_weight, a.post_f32, c + e) : v[e]);
+          if (a.gate) v[e] *= weight_at(a.gate, a.gate_f32, group * a.channels + c + e);
+          if (a.g_post && group > first) v[e] += part_post[c + e];
+        }
+        if (a.g_post) put_sums<N>(part_post + c, left, v);
       });
     }
   }
-  float* part = a.part + (int64_t)blockIdx.x * a.channels;
-  if (a.g_pre) {
-    over_rows<TPR>(g_pre, sums, a.channels, [&](int c, float v) { part[c] = v; });
-    part += (int64_t)grid.blocks * a.channels;
-  }
-  if (a.g_post) over_rows<TPR>(g_post, sums, a.channels, [&](int c, float v) { part[c] = v; });
+  if (a.g_pre) over_rows<TPR>(g_pre, sums, a.channels, [&](int c, int left, auto& v) { put_sums<sizeof(v) / 4>(part_pre + c, left, v); });
+  if (a.g_post && (EACH || first >= grid.groups))
+    over_rows<TPR>(q, sums, a.channels, [&](int c, int left, auto& v) {
+#pragma unroll
+      for (int e = 0; e < (int)(sizeof(v) / 4); ++e) v[e] *= keep;
+      put_sums<sizeof(v) / 4>(part_post + c, left, v);
+    });
 }
 
 constexpr int kSumCols = 16, kShares = 64;  // columns of a workgroup, and shares of the rows that it adds in parallel
@@ -391,6 +487,39 @@ __global__ void __launch_bounds__(kSumCols * kShares) sandwich_sums_kernel(Sandw
   put_weight(out, f32, (int64_t)what * a.channels + c, s * weight);
 }
 
+// The instance of the backward pass for `n` vectors of E elements: few vectors a thread.
+template <int E, typename F>
+hipError_t choose_bwd(int n, F&& f) {
+  if (n <= 16) return f.template operator()<16, 1>();
+  if (n <= 32) return f.template operator()<32, 1>();
+  if (n <= 64) return f.template operator()<64, 1>();
+  if (n <= 128) return f.template operator()<128, 1>();
+  if (n <= 256) return f.template operator()<256, 1>();
+  if (n <= 512) return f.template operator()<512, 1>();
+  if (n <= 1024) return f.template operator()<1024, 1>();
+  if (n <= 2048) return f.template operator()<1024, 2>();
+  if constexpr (E == 4) {
+    if (n <= 4096) return f.template operator()<1024, 4>();
+  }
+  return hipErrorInvalidValue;
+}
+
+template <int E, typename F>
+hipError_t choose_fwd(int n, F&& f) {
+  if (n <= 16) return f.template operator()<16, 1>();
+  if (n <= 32) return f.template operator()<32, 1>();
+  if (n <= 64) return f.template operator()<64, 1>();
+  if (n <= 128) return f.template operator()<128, 1>();
+  if (n <= 256) return f.template operator()<256, 1>();
+  if (n <= 512) return f.template operator()<256, 2>();
+  if (n <= 1024) return f.template operator()<512, 2>();
+  if (n <= 2048) return f.template operator()<1024, 2>();
+  if constexpr (E == 4) {
+    if (n <= 4096) return f.template operator()<1024, 4>();
+  }
+  return hipErrorInvalidValue;
+}
+
 template <typename T, bool TAIL>
 struct Forward {
   const SandwichArgs& a;
@@ -405,14 +534,14 @@ struct Forward {
   }
 };
 
-template <typename T, bool SUMS, bool TAIL>
+template <typename T, bool EACH, bool TAIL>
 struct Backward {
   const SandwichBwdArgs& a;
   const SandwichGrid& grid;
   hipStream_t stream;
   template <int TPR, int VPT>
   hipError_t operator()() const {
-    hipLaunchKernelGGL((sandwich_bwd_kernel<T, TPR, VPT, SUMS, TAIL>), dim3((unsigned)grid.blocks), dim3(kThreads<TPR>), 0, stream, a,
+    hipLaunchKernelGGL((sandwich_bwd_kernel<T, TPR, VPT, EACH, TAIL>), dim3((unsigned)grid.blocks), dim3(kThreads<TPR>), 0, stream, a,
                        grid);
     return hipGetLastError();
   }
@@ -422,18 +551,16 @@ template <typename T>
 hipError_t forward_as(const SandwichArgs& a, hipStream_t stream) {
   constexpr int E = 16 / sizeof(T);
   const int n = (a.channels + E - 1) / E;
-  return a.channels % E ? choose<E>(n, Forward<T, true>{a, stream}) : choose<E>(n, Forward<T, false>{a, stream});
+  return a.channels % E ? choose_fwd<E>(n, Forward<T, true>{a, stream}) : choose_fwd<E>(n, Forward<T, false>{a, stream});
 }
 
-template <typename T, bool SUMS>
+template <typename T, bool EACH>
 hipError_t backward_as(const SandwichBwdArgs& a, const SandwichGrid& grid, hipStream_t stream) {
   constexpr int E = 16 / sizeof(T);
   const int n = (a.channels + E - 1) / E;
-  return a.channels % E ? choose<E>(n, Backward<T, SUMS, true>{a, grid, stream})
-                        : choose<E>(n, Backward<T, SUMS, false>{a, grid, stream});
+  return a.channels % E ? choose_bwd<E>(n, Backward<T, EACH, true>{a, grid, stream})
+                        : choose_bwd<E>(n, Backward<T, EACH, false>{a, grid, stream});
 }
-
-bool gate_sums(const SandwichBwdArgs& a) { return a.g_gate && a.gate_rows > 1; }
 
 }  // namespace
 
@@ -443,12 +570,14 @@ hipError_t launch_sandwich(int dtype, const SandwichArgs& args, hipStream_t stre
   return dtype == FWN_F32 ? forward_as<float>(a, stream) : forward_as<uint16_t>(a, stream);
 }
 
-// At most 1,024 workgroups, four a CU, with eight rows each at least (32 where rows share waves), as each leaves its partial sums.
-SandwichGrid sandwich_grid(int64_t rows, int64_t gate_rows, int32_t channels, bool sums) {
+// As many workgroups as the chip holds at once, 1,024 threads a CU, with four rows each at least (32 where rows share waves), as
+// each leaves its partial sums.
+constexpr int64_t kCus = 256;
+SandwichGrid sandwich_grid(int64_t rows, int64_t gate_rows, int32_t channels, int32_t dtype) {
   SandwichGrid g;
-  constexpr int64_t most = 1024;
-  const int64_t least = channels <= 256 ? 32 : 8;
-  g.group_rows = sums ? gate_rows : rows;
+  const int n = (channels * (dtype == FWN_F32 ? 4 : 2) + 15) / 16, threads = n <= 256 ? 256 : n <= 512 ? 512 : 1024;
+  const int64_t most = kCus * 1024 / threads, least = n <= 32 ? 32 : 4;
+  g.group_rows = gate_rows > 1 ? gate_rows : rows;
   g.groups = g.group_rows > 0 ? rows / g.group_rows : 0;
   const int64_t want = (g.group_rows + least - 1) / least, room = g.groups < most ? most / (g.groups > 0 ? g.groups : 1) : 1;
   g.per = (int32_t)(want < 1 ? 1 : want < room ? want : room);
@@ -456,22 +585,22 @@ SandwichGrid sandwich_grid(int64_t rows, int64_t gate_rows, int32_t channels, bo
   if (g.of_block < 1) g.of_block = 1;
   g.blocks = (int32_t)(g.per > 1 ? g.groups * g.per : (g.groups + g.of_block - 1) / g.of_block);
   if (g.blocks < 1) g.blocks = 1;
-  g.parts = 2 + (sums && g.per > 1);
+  g.parts = 2 + (gate_rows > 1 && g.per > 1);
   return g;
 }
 
 hipError_t launch_sandwich_bwd(int dtype, const SandwichBwdArgs& args, hipStream_t stream) {
   SandwichBwdArgs a = args;
   a.stream = 2 * (uint64_t)a.rows * a.channels * (dtype == FWN_F32 ? 4 : 2) >= kStreamBytes;
-  const bool sums = gate_sums(a);
-  SandwichGrid grid = sandwich_grid(a.rows, a.gate_rows, a.channels, sums);
-  const bool gates = sums && grid.per > 1;
+  const bool each = a.gate && a.gate_rows == 1;
+  SandwichGrid grid = sandwich_grid(a.rows, a.gate ? a.gate_rows : a.rows, a.channels, dtype);
+  const bool gates = a.g_gate && !each && grid.per > 1;
   grid.parts = (a.g_pre != nullptr) + (a.g_post != nullptr) + gates;
   hipError_t rc;
   if (dtype == FWN_F32)
-    rc = sums ? backward_as<float, true>(a, grid, stream) : backward_as<float, false>(a, grid, stream);
+    rc = each ? backward_as<float, true>(a, grid, stream) : backward_as<float, false>(a, grid, stream);
   else
-    rc = sums ? backward_as<uint16_t, true>(a, grid, stream) : backward_as<uint16_t, false>(a, grid, stream);
+    rc = each ? backward_as<uint16_t, true>(a, grid, stream) : backward_as<uint16_t, false>(a, grid, stream);
   if (rc != hipSuccess || grid.parts == 0) return rc;
   const unsigned roles = (unsigned)((a.g_pre != nullptr) + (a.g_post != nullptr) + (gates ? grid.groups : 0));
   hipLaunchKernelGGL(sandwich_sums_kernel, dim3((unsigned)((a.channels + kSumCols - 1) / kSumCols), roles),

@@ -87,7 +87,7 @@ def _backward(s, y, post, pre, gate, state, call, g_sum, g_out, needs):
   ws, size = None, ctypes.c_uint64(0)
   summed = need_gate and call.gate_rows > 1 and s.numel() > 0
   if need_post or need_pre or summed:
-    nat.check(L.fwn_sandwich_norm_bwd_workspace_size(d, summed, ctypes.byref(size)))
+    nat.check(L.fwn_sandwich_norm_bwd_workspace_size(d, gate is not None, ctypes.byref(size)))
     ws = torch.empty(size.value, dtype=torch.uint8, device=s.device)
   launch(s, L.fwn_sandwich_norm_bwd_launch, d, _addr(s), _addr(yr), _addr(gate), _addr(post), _addr(pre), _addr(g_sum),
          _addr(g_out), _addr(gx), _addr(gy), _addr(g_gate) if s.numel() else None, _addr(g_post), _addr(g_pre), _addr(ws),

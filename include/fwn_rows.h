@@ -219,8 +219,8 @@ int fwn_sandwich_norm_launch(const fwn_sandwich_desc* d, const void* x, const vo
  *   g_post = sum of d gate y r1,  g_pre = sum of g_out s r2, both over the rows
  * g_sum and g_out may be NULL (zeros), and each output may be NULL (not wanted). The workspace
  * (fwn_sandwich_norm_bwd_workspace_size bytes, 16-byte aligned) is needed where one of g_gate (of more than one row each),
- * g_post and g_pre is; the query takes whether g_gate is wanted. Sums run in a fixed order. */
-int fwn_sandwich_norm_bwd_workspace_size(const fwn_sandwich_desc* d, int32_t gate_gradient, uint64_t* bytes);
+ * g_post and g_pre is; the query takes whether there is a gate. Sums run in a fixed order. */
+int fwn_sandwich_norm_bwd_workspace_size(const fwn_sandwich_desc* d, int32_t gate, uint64_t* bytes);
 int fwn_sandwich_norm_bwd_launch(const fwn_sandwich_desc* d, const void* s, const void* y, const void* gate,
                                  const void* post_weight, const void* pre_weight, const void* g_sum, const void* g_out, void* gx,
                                  void* gy, void* g_gate, void* g_post, void* g_pre, void* workspace, uint64_t workspace_bytes,
