@@ -7,6 +7,11 @@
 namespace fwn {
 namespace {
 
+// One instruction where the compiler makes two of ^ (40,968 x 768 bf16, backward of the norms around a block with dropout: 87 us, with ^ 96).
+__device__ __forceinline__ uint32_t xor3(uint32_t a, uint32_t b, uint32_t c) {
+  return (uint32_t)__builtin_amdgcn_bitop3_b32((int)a, (int)b, (int)c, 0x96);
+}
+
 // The state of a launch: of its arguments, or as the GPU's memory holds it when the kernel runs.
 struct Draw {
   uint32_t key[2], offset[2];
@@ -31,9 +36,9 @@ struct Draw {
 #pragma unroll
     for (int i = 0; i < 10; ++i) {
       const uint64_t a = (uint64_t)c[0] * 0xD2511F53u, b = (uint64_t)c[2] * 0xCD9E8D57u;
-      c[0] = (uint32_t)(b >> 32) ^ c[1] ^ k0;
+      c[0] = xor3((uint32_t)(b >> 32), c[1], k0);
       c[1] = (uint32_t)b;
-      c[2] = (uint32_t)(a >> 32) ^ c[3] ^ k1;
+      c[2] = xor3((uint32_t)(a >> 32), c[3], k1);
       c[3] = (uint32_t)a;
       k0 += 0x9E3779B9u;
       k1 += 0xBB67AE85u;
