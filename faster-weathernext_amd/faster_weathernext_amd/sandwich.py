@@ -9,6 +9,7 @@ for the residual x and the output y of an attention or feed-forward block, as bl
 one HIP pass forward and one, plus the small reductions of the weights' and the gate's gradients, backward.
 """
 import ctypes
+import functools
 
 import torch
 
@@ -46,56 +47,52 @@ def _gate_rows(gate, x):
                    f"[members, ..., channels], got {tuple(gate.shape)}")
 
 
-class _Call:
-  """What a call's passes share beside their tensors."""
-  __slots__ = ("scale", "post_norm", "p", "eps", "gate_rows", "seed", "offset")
-
-  def desc(self, x, x_stride, y_stride, gate, post, pre, state):
-    c, dtype = x.shape[-1], _DTYPES[x.dtype]
-    kind = lambda t: dtype if t is None else _DTYPES[t.dtype]
-    return nat.SandwichDesc(x.numel() // c, self.gate_rows, x_stride, y_stride, c, dtype, kind(gate), kind(post), kind(pre),
-                            self.post_norm, self.eps, self.scale, nat.Dropout(self.p, self.seed, self.offset, _addr(state)))
+def _kind(t, dtype):
+  return dtype if t is None else _DTYPES[t.dtype]
 
 
-def _forward(x, y, post, pre, gate, state, call):
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(rows, gate_rows, channels, dtype, gate):
+  """The backward's workspace, a function of the sizes alone (the query takes 3 us of host time)."""
+  d = nat.SandwichDesc(rows, gate_rows, channels, channels, channels, dtype, dtype, dtype, dtype, 1, 0.0, 1.0, nat.Dropout(0.0, 0, 0, None))
+  size = ctypes.c_uint64(0)
+  nat.check(nat.lib().fwn_sandwich_norm_bwd_workspace_size(d, gate, ctypes.byref(size)))
+  return size.value
+
+
+def _forward(x, y, post, pre, gate, state, d):
   """(s, out): one HIP pass (no autograd)."""
-  xr, xs = rows_of(x)
-  yr, ys = rows_of(y)
+  xr, d.x_stride = rows_of(x)
+  yr, d.y_stride = rows_of(y)
   post, pre, gate = dense(post), dense(pre), dense(gate)
   s, out = new_like(x), new_like(x)
-  d = call.desc(x, xs, ys, gate, post, pre, state)
   launch(x, nat.lib().fwn_sandwich_norm_launch, d, _addr(xr), _addr(yr), _addr(gate), _addr(post), _addr(pre), _addr(s),
          _addr(out))
   return s, out
 
 
-def _backward(s, y, post, pre, gate, state, call, g_sum, g_out, needs):
+def _backward(s, y, post, pre, gate, state, d, g_sum, g_out, needs):
   """The gradients that `needs` asks for of x, y, post, pre and gate: fwn_sandwich_norm_bwd_launch."""
-  yr, ys = rows_of(y)
-  s, post, pre, gate, g_sum, g_out = (dense(t) for t in (s, post, pre, gate, g_sum, g_out))
+  if not s.numel():
+    return tuple(torch.zeros_like(t) if n else None for t, n in zip((s, y, post, pre, gate), needs))
+  yr, d.y_stride = rows_of(y)
+  s, post, pre, gate, g_sum, g_out = dense(s), dense(post), dense(pre), dense(gate), dense(g_sum), dense(g_out)
   need_x, need_y, need_post, need_pre, need_gate = needs
-  c = s.shape[-1]
-  d = call.desc(s, c, ys, gate, post, pre, state)
-  L = nat.lib()
   gx = torch.empty_like(s) if need_x else None
   gy = torch.empty_like(s) if need_y else None
   g_post = torch.empty_like(post) if need_post else None
   g_pre = torch.empty_like(pre) if need_pre else None
-  g_gate = None
-  if need_gate:
-    g_gate = torch.empty_like(gate) if s.numel() else torch.zeros_like(gate)
-  ws, size = None, ctypes.c_uint64(0)
-  summed = need_gate and call.gate_rows > 1 and s.numel() > 0
-  if need_post or need_pre or summed:
-    nat.check(L.fwn_sandwich_norm_bwd_workspace_size(d, gate is not None, ctypes.byref(size)))
-    ws = torch.empty(size.value, dtype=torch.uint8, device=s.device)
-  launch(s, L.fwn_sandwich_norm_bwd_launch, d, _addr(s), _addr(yr), _addr(gate), _addr(post), _addr(pre), _addr(g_sum),
-         _addr(g_out), _addr(gx), _addr(gy), _addr(g_gate) if s.numel() else None, _addr(g_post), _addr(g_pre), _addr(ws),
-         size.value)
+  g_gate = torch.empty_like(gate) if need_gate else None
+  ws, size = None, 0
+  if need_post or need_pre or (need_gate and d.gate_rows > 1):
+    size = _workspace_bytes(d.rows, d.gate_rows, d.channels, d.dtype, gate is not None)
+    ws = torch.empty(size, dtype=torch.uint8, device=s.device)
+  launch(s, nat.lib().fwn_sandwich_norm_bwd_launch, d, _addr(s), _addr(yr), _addr(gate), _addr(post), _addr(pre), _addr(g_sum),
+         _addr(g_out), _addr(gx), _addr(gy), _addr(g_gate), _addr(g_post), _addr(g_pre), _addr(ws), size)
   return gx, gy, g_post, g_pre, g_gate
 
 
-def _backward_torch(s, y, post, pre, gate, state, call, g_sum, g_out, needs):
+def _backward_torch(s, y, post, pre, gate, state, d, g_sum, g_out, needs):
   """The same gradients as torch operations, for backwards under create_graph or of batched gradients."""
   c = s.shape[-1]
   one = torch.ones((), device=s.device)
@@ -106,16 +103,16 @@ def _backward_torch(s, y, post, pre, gate, state, call, g_sum, g_out, needs):
   if per_member:
     w_gate = w_gate.reshape(gate.shape[0], *[1] * (s.dim() - 2), c)
   ds = torch.zeros_like(f) if g_sum is None else g_sum.float()
-  r2 = torch.rsqrt(f.square().mean(-1, keepdim=True) + call.eps)
+  r2 = torch.rsqrt(f.square().mean(-1, keepdim=True) + d.eps)
   if g_out is not None:
     a = g_out.float() * w_pre
     ds = ds + r2 * (a - f * r2.square() * (a * f).mean(-1, keepdim=True))
   db = ds
-  if call.p > 0:
-    db = dropped(ds, multipliers(s.shape, s, call.p, (state, call.seed, call.offset)))
-  r1 = torch.rsqrt(z.square().mean(-1, keepdim=True) + call.eps) if call.post_norm else one
+  if d.drop.p > 0:
+    db = dropped(ds, multipliers(s.shape, s, d.drop.p, (state, d.drop.seed, d.drop.offset)))
+  r1 = torch.rsqrt(z.square().mean(-1, keepdim=True) + d.eps) if d.post_norm else one
   unit, q = z * r1, db * w_gate * w_post
-  gy = r1 * (q - z * r1.square() * (q * z).mean(-1, keepdim=True)) if call.post_norm else q
+  gy = r1 * (q - z * r1.square() * (q * z).mean(-1, keepdim=True)) if d.post_norm else q
   need_x, need_y, need_post, need_pre, need_gate = needs
   g_post = (db * w_gate * unit).reshape(-1, c).sum(0).to(post.dtype) if need_post else None
   g_pre = None
@@ -129,7 +126,7 @@ def _backward_torch(s, y, post, pre, gate, state, call, g_sum, g_out, needs):
     elif gate.shape != s.shape:
       g_gate = g_gate.reshape(-1, c).sum(0)
     g_gate = g_gate.to(gate.dtype)
-  return (call.scale * ds).to(s.dtype) if need_x else None, gy.to(s.dtype) if need_y else None, g_post, g_pre, g_gate
+  return (d.scale * ds).to(s.dtype) if need_x else None, gy.to(s.dtype) if need_y else None, g_post, g_pre, g_gate
 
 
 class _Sandwich(torch.autograd.Function):
@@ -137,11 +134,11 @@ class _Sandwich(torch.autograd.Function):
   miss what comes through it."""
 
   @staticmethod
-  def forward(ctx, x, y, post, pre, gate, state, call):
-    s, out = _forward(x, y, post, pre, gate, state, call)
+  def forward(ctx, x, y, post, pre, gate, state, d):
+    s, out = _forward(x, y, post, pre, gate, state, d)
     ctx.save_for_backward(s, y, post, pre, gate, state)
     ctx.set_materialize_grads(False)
-    ctx.call = call
+    ctx.desc = d
     return s, out
 
   @staticmethod
@@ -149,7 +146,7 @@ class _Sandwich(torch.autograd.Function):
     if g_sum is None and g_out is None:
       return (None,) * 7
     run = _backward_torch if as_torch(g_sum, g_out) else _backward
-    return (*run(*ctx.saved_tensors, ctx.call, g_sum, g_out, ctx.needs_input_grad[:5]), None, None)
+    return (*run(*ctx.saved_tensors, ctx.desc, g_sum, g_out, ctx.needs_input_grad[:5]), None, None)
 
 
 def sandwich_norm(x, y, post_weight=None, pre_weight=None, *, gate=None, scale=1.0, post_norm=True, p=0.0, rng=None, eps=1e-6):
@@ -167,14 +164,15 @@ def sandwich_norm(x, y, post_weight=None, pre_weight=None, *, gate=None, scale=1
   _check_weight(pre_weight, "pre_weight", x)
   if post_weight is not None and not post_norm:
     raise ValueError("post_weight is the norm's: there is none without post_norm")
-  call = _Call()
-  call.gate_rows = _gate_rows(gate, x)
-  call.scale, call.post_norm, call.p, call.eps = float(scale), bool(post_norm), check_p(p), float(eps)
-  state, call.seed, call.offset = None, 0, 0
-  if call.p > 0:
+  p, state, seed, offset = check_p(p), None, 0, 0
+  if p > 0:
     if rng is None:
       raise ValueError("dropout needs rng, its state")
-    state, call.seed, call.offset = rng_of(rng, x)
+    state, seed, offset = rng_of(rng, x)
+  c, dtype = x.shape[-1], _DTYPES[x.dtype]
+  # The strides are filled in where the rows are taken; the backward pass takes the same descriptor, of tensors it keeps.
+  d = nat.SandwichDesc(x.numel() // c, _gate_rows(gate, x), 0, 0, c, dtype, _kind(gate, dtype), _kind(post_weight, dtype),
+                       _kind(pre_weight, dtype), bool(post_norm), eps, scale, nat.Dropout(p, seed, offset, _addr(state)))
   if _needs(x, y, post_weight, pre_weight, gate):
-    return _Sandwich.apply(x, y, post_weight, pre_weight, gate, state, call)
-  return _forward(x, y, post_weight, pre_weight, gate, state, call)
+    return _Sandwich.apply(x, y, post_weight, pre_weight, gate, state, d)
+  return _forward(x, y, post_weight, pre_weight, gate, state, d)
