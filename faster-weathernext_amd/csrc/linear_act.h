@@ -54,6 +54,8 @@ enum class Operands { kInnerInner, kInnerOuter, kOuterOuter };  // how a and b l
 // kInnerInner alone.
 hipError_t launch_product(Operands how, int32_t op, int tile, const ProductArgs& a, hipStream_t stream);
 hipError_t launch_product_f32(Operands how, int tile, const ProductArgs& a, hipStream_t stream);
+// The partial products of a split product with bf16 outputs added in order, and its epilogue.
+hipError_t launch_join(const ProductArgs& a, hipStream_t stream);
 // One product of inner operands with at most kFewRows rows of a, unsplit.
 hipError_t launch_product_rows(int32_t op, const ProductArgs& a, hipStream_t stream);
 constexpr int64_t kFewRows = 32;

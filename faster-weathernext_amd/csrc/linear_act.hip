@@ -11,56 +11,10 @@
 // with both, of which the main loop has 160 and 92. One workgroup a CU (its two stages are 128 KB of LDS, its sums half
 // of the registers): 8 waves of 128 x 64 outputs, so that a byte of a in LDS is read four times and one of b twice.
 #include "linear_act_device.h"
+#include "linear_act_stage.h"
 
 namespace fwn {
 namespace {
-
-// ------------------------------------------------------------------------------------------
-// Copies of an operand's stages into LDS, 1 KB a wave instruction, a few a wave and stage.
-//   inner: 8 rows of 128 bytes; 16-byte chunk c of row r lies at c ^ (r / 2 % 8), so that a chunk of sixteen
-//          rows, which a ds_read_b128 serves at once, lies in sixteen different parts of a 256-byte line (4 clocks
-//          a read measured, 256 bytes a clock). Whole 128-byte lines: with 64-byte rows each line was fetched
-//          twice, the L1 holding less than a stage, and the product ran at two thirds of its rate;
-//   outer: 4 rows of k by 128 columns, in the swizzled layout of the transpose reads.
-// Rows and columns past the operand, k past the sum and stages past the range are copied as zeros: their
-// offsets lie past the buffer's end.
-template <bool OUTER, int WAVES, int COUNT>
-struct Copy {
-  const char* base;  // of the tile
-  int64_t step;      // bytes from one stage to the next
-  uint32_t off[COUNT], tail[COUNT];  // of this lane's 16 bytes, and kNowhere where they lie past the sum in its last stage
-
-  // Tile from row (or column) `first` of `rows`; `k` elements of `size` bytes in the sum, whose last stage is `last`.
-  __device__ __forceinline__ void init(const char* p, int64_t stride, int64_t first, int64_t rows,
-                                       int64_t k, int size, int64_t last, int w, int lane) {
-    base = p + (OUTER ? first * 2 : first * stride);
-    step = OUTER ? kStageRows * stride : kStageBytes;
-#pragma unroll
-    for (int h = 0; h < COUNT; ++h) {
-      const int q = w + WAVES * h;
-      if constexpr (OUTER) {
-        const int row = 4 * (q & 15) + lane / 16, chunk = (lane % 16) ^ swz<16>(row), col = (q >> 4) * 128 + chunk * 8;
-        off[h] = first + col < rows ? (uint32_t)row * (uint32_t)stride + (uint32_t)col * 2 : kNowhere;
-        tail[h] = last * kStageRows + row < k ? 0 : kNowhere;
-      } else {
-        const int row = 8 * q + lane / 8, chunk = (lane % 8) ^ (row / 2 % 8);
-        off[h] = first + row < rows ? (uint32_t)row * (uint32_t)stride + (uint32_t)chunk * 16 : kNowhere;
-        tail[h] = last * kStageBytes + chunk * 16 < k * size ? 0 : kNowhere;
-      }
-    }
-  }
-
-  // Stage `t` to `dst`; `last` all ones: the sum's last stage; `none` kNowhere: zeros.
-  __device__ __forceinline__ void issue(lds_char* dst, int64_t t, uint32_t last, uint32_t none, int w) const {
-    const rsrc_t r = make_rsrc(base + t * step, kBuffer);
-#pragma unroll
-    for (int h = 0; h < COUNT; ++h) {
-      const uint32_t o = off[h] | (tail[h] & last) | none;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(dst + (w + WAVES * h) * 1024),
-                                               16, (int)o, 0, 0, 0);
-    }
-  }
-};
 
 // LDS byte offsets of an operand's 32-row blocks for one wave: quarter c of a stage is 16 bf16 k.
 template <bool OUTER, int BLOCKS>
@@ -96,14 +50,6 @@ struct Reads {
     }
   }
 };
-
-// This wave's copies have landed and its LDS reads have returned, and so have every other wave's.
-__device__ __forceinline__ void stage_barrier() {
-  __builtin_amdgcn_s_waitcnt(0x0070);
-  asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_barrier();
-  asm volatile("" ::: "memory");
-}
 
 constexpr int threads_of(int bm) { return 2 * bm; }
 
@@ -283,17 +229,22 @@ __global__ void __launch_bounds__(256) join_kernel(ProductArgs g) {
   join<PLAIN, F32, N>(g, MendNothing());
 }
 
+template <bool PLAIN, bool F32>
+hipError_t join_parts(const ProductArgs& g, hipStream_t stream) {
+  if (g.e.vec)
+    hipLaunchKernelGGL((join_kernel<PLAIN, F32, 8>), join_grid(g), dim3(256), 0, stream, g);
+  else
+    hipLaunchKernelGGL((join_kernel<PLAIN, F32, 1>), join_grid(g), dim3(256), 0, stream, g);
+  return hipGetLastError();
+}
+
 template <bool OA, bool OB, Form FORM, int TILE>
 hipError_t launch_tile(const ProductArgs& g, hipStream_t stream) {
   const int64_t tiles = ((g.e.m + TILE - 1) / TILE) * ((g.e.n + TILE - 1) / TILE);
   hipLaunchKernelGGL((product_kernel<OA, OB, FORM, TILE, TILE>), dim3((unsigned)(tiles * g.splits)), dim3(threads_of(TILE)), 0,
                      stream, g);
   if (hipError_t e = hipGetLastError(); e != hipSuccess || !g.part) return e;
-  if (g.e.vec)
-    hipLaunchKernelGGL((join_kernel<OB, FORM == Form::kWidened, 8>), join_grid(g), dim3(256), 0, stream, g);
-  else
-    hipLaunchKernelGGL((join_kernel<OB, FORM == Form::kWidened, 1>), join_grid(g), dim3(256), 0, stream, g);
-  return hipGetLastError();
+  return join_parts<OB, FORM == Form::kWidened>(g, stream);
 }
 
 template <bool OA, bool OB, Form FORM>
@@ -302,6 +253,8 @@ hipError_t launch_operands(int tile, const ProductArgs& g, hipStream_t stream) {
 }
 
 }  // namespace
+
+hipError_t launch_join(const ProductArgs& g, hipStream_t stream) { return join_parts<false, false>(g, stream); }
 
 hipError_t launch_product(Operands how, int32_t op, int tile, const ProductArgs& a, hipStream_t stream) {
   if (op == kOpF32) return launch_product_f32(how, tile, a, stream);

@@ -128,6 +128,7 @@ struct Matrix {
 struct Plan {
   int tile;
   int32_t splits, chunk;
+  double time = 0;
 };
 
 struct Cost {
@@ -154,7 +155,40 @@ Plan plan(Operands how, int64_t m, int64_t n, int64_t k, int32_t op, bool widene
       const double time = load * (chunk * (load == 1 ? c.alone : c.full) * (widened ? 2 : 1) + c.ends) + join;
       if (least < 0 || time < least) {
         least = time;
-        best = {c.tile, (int32_t)splits, (int32_t)chunk};
+        best = {c.tile, (int32_t)splits, (int32_t)chunk, time};
+      }
+    }
+  }
+  return best;
+}
+
+// How a product of bf16 rows with a 4-bit weight is formed, by an estimate of its time in us: the few rows' kernel (tile -1), tiles
+// that take the codes (tile: their waves), or a widened weight and its plan (tile 0). Measured and estimated: 24 rows of 5,120 ->
+// 8,192 16 in few rows, 21 in tiles; 32 of 16,384 -> 4,096 38 and 24; 512 of 4,096 -> 8,192 36 in tiles of four waves, 39 of two, 62
+// widened; 2,048 of 2,048 -> 4,096 41 in tiles, 40 widened.
+Plan plan_q4(int64_t m, int64_t n, int64_t k) {
+  Plan best{0, 1, 0};
+  const double weights = (double)n * k;
+  double least = plan(Operands::kInnerInner, m, n, k, kOpBf16, false).time + 3.0 + weights * 2.53 / 4.6e6;
+  if (m <= kFewRows) {
+    // Each workgroup of 16 or 32 outputs reads all rows.
+    const double reads = (double)parts(n, n > 16 * kCus ? 32 : 16) * m * k * 2;
+    least = 3.0 + std::max(weights * 0.53 / 4e6, reads / 6e6);
+    best.tile = -1;
+  }
+  const int64_t spans = std::max<int64_t>(1, parts(k, kQ4Span));
+  for (int waves = 2; waves <= 4; waves += 2) {
+    const int64_t tiles = parts(m, 64) * parts(n, 64 * waves), at_once = waves == 2 ? 2 * kCus : kCus;
+    for (int64_t want = 1; want <= 16; ++want) {
+      const int64_t chunk = parts(spans, want), splits = parts(spans, chunk), load = tiles * splits;
+      if (splits != want) continue;
+      if (want > 1 && (chunk < 2 || load > 2 * at_once)) break;
+      const double span = waves == 2 ? (load <= kCus ? 0.8 : 1.08) : (load <= kCus / 2 ? 0.86 : 1.0);
+      const double join = splits > 1 ? 5.0 + (double)(splits + 1) * m * n * 4 / 2.5e6 : 0;
+      const double time = parts(load, at_once) * (chunk * span + 4.0) + join;
+      if (time < least) {
+        least = time;
+        best = {waves, (int32_t)splits, (int32_t)chunk};
       }
     }
   }
@@ -170,10 +204,12 @@ struct Product {
   bool few;  // rows: no tiles
 
   // `sums`: the column sums of a are wanted. `dtype`: of the outputs.
-  void shape(Operands h, int64_t m, int64_t n, int64_t k, int32_t o, int32_t dtype, bool sums, Workspace& ws) {
+  // `given`: the plan, of a kernel of its own.
+  void shape(Operands h, int64_t m, int64_t n, int64_t k, int32_t o, int32_t dtype, bool sums, Workspace& ws,
+             const Plan* given = nullptr) {
     how = h, op = o;
-    few = how == Operands::kInnerInner && m <= kFewRows;
-    p = few ? Plan{0, 1, 0} : plan(how, m, n, k, op, op == kOpE4m3 && dtype == FWN_F32);
+    few = !given && how == Operands::kInnerInner && m <= kFewRows;
+    p = given ? *given : few ? Plan{0, 1, 0} : plan(how, m, n, k, op, op == kOpE4m3 && dtype == FWN_F32);
     g.k = k;
     g.splits = p.splits;
     g.chunk = p.chunk;
@@ -187,10 +223,15 @@ struct Product {
   hipError_t launch(const Matrix& a, const Matrix& b, hipStream_t stream) {
     g.a = a.at, g.a_stride = a.row_bytes;
     g.b = b.at, g.b_stride = b.row_bytes;
+    finish();
+    return few ? launch_product_rows(op, g, stream) : launch_product(how, op, p.tile, g, stream);
+  }
+
+  // What the epilogue's arguments imply.
+  void finish() {
     const EpilogueArgs& e = g.e;
     g.e.vec = e.n % 8 == 0 && (!e.residual || e.r_row % 8 == 0) &&
               (((uintptr_t)e.out | (uintptr_t)e.pre | (uintptr_t)e.residual) & 15) == 0;
-    return few ? launch_product_rows(op, g, stream) : launch_product(how, op, p.tile, g, stream);
   }
 };
 
@@ -283,20 +324,26 @@ struct Backward {
   }
 };
 
-// The same with a weight of 4 bits: widened in the workspace where the tiles' kernels take it, read as it is for few rows.
+// The same with a weight of 4 bits: read as it is for few rows and by the tiles of bf16, widened in the workspace for float32's.
 struct ForwardQ4 {
-  Matrix x, w{};
+  Matrix x, w{}, scales{};
   Product z;
   int64_t groups;
+  int waves = 0;  // of a tile that takes the codes
   uint64_t bytes;
 
-  ForwardQ4(const fwn_linear_desc* d, const void* xp, void* workspace) {
+  ForwardQ4(const fwn_linear_desc* d, const void* xp, const uint8_t* sp, void* workspace) {
     Workspace ws{(char*)workspace};
     const int32_t op = d->dtype == FWN_F32 ? kOpF32 : kOpBf16;
     groups = parts(d->ins, FWN_Q4_GROUP);
     x.place(xp, d->rows, d->ins, d->x_stride, op, ws);
-    z.shape(Operands::kInnerInner, d->rows, d->outs, d->ins, op, d->dtype, false, ws);
-    if (!z.few) {
+    const Plan p = op == kOpBf16 && d->rows > 16 ? plan_q4(d->rows, d->outs, d->ins) : Plan{0, 1, 0};
+    waves = p.tile > 0 ? p.tile : 0;
+    z.shape(Operands::kInnerInner, d->rows, d->outs, d->ins, op, d->dtype, false, ws, waves ? &p : nullptr);
+    scales.at = (char*)sp;
+    scales.row_bytes = groups;
+    if (waves && (groups % 4 || ((uintptr_t)sp & 3))) scales.place(sp, d->outs, groups, groups, kOpE4m3, ws, true);
+    if (!z.few && !waves) {
       w.row_bytes = groups * FWN_Q4_GROUP * op_size(op);
       w.at = ws.take((uint64_t)d->outs * (uint64_t)w.row_bytes);
     }
@@ -368,10 +415,10 @@ int fwn_quantize_q4_launch(int64_t rows, int32_t ins, int64_t x_stride, int32_t 
   return status(launch_quantize_q4(dtype, {x, codes, scales, rows, ins, x_stride}, (hipStream_t)stream), what);
 }
 
-int fwn_linear_act_q4_workspace_size(const fwn_linear_desc* d, const void* x, uint64_t* bytes) {
+int fwn_linear_act_q4_workspace_size(const fwn_linear_desc* d, const void* x, const uint8_t* scales, uint64_t* bytes) {
   using namespace fwn;
   if (int rc = size_query(d, bytes, "fwn_linear_act_q4_workspace_size")) return rc;
-  *bytes = ForwardQ4(d, x, nullptr).bytes;
+  *bytes = ForwardQ4(d, x, scales, nullptr).bytes;
   return FWN_OK;
 }
 
@@ -387,7 +434,7 @@ int fwn_linear_act_q4_launch(const fwn_linear_desc* d, const void* x, const uint
   const uint64_t size = size_of(d->dtype);
   if (misaligned(x, size) || misaligned(codes, 16) || misaligned(bias, size) || misaligned(residual, size) || misaligned(out, size))
     return fail(FWN_ERR_INVALID_ARG, "%s: a tensor is not aligned", what);
-  ForwardQ4 f(d, x, workspace);
+  ForwardQ4 f(d, x, scales, workspace);
   if (int rc = check_workspace(workspace, workspace_bytes, f.bytes, what)) return rc;
   const Span ins[] = {span(x, d->rows, d->x_stride, d->ins, size), span(codes, d->outs, f.groups * 16, f.groups * 16, 1),
                       span(scales, d->outs, f.groups, f.groups, 1), span(bias, 1, 0, d->outs, size),
@@ -404,11 +451,13 @@ int fwn_linear_act_q4_launch(const fwn_linear_desc* d, const void* x, const uint
   const hipStream_t s = (hipStream_t)stream;
   const bool f32 = d->dtype == FWN_F32;
   if (int rc = status(f.x.lay_out(s), what)) return rc;
-  if (f.z.few) {
-    Q4Args a{f.z.g, codes, scales, f.groups};
+  if (f.z.few || f.waves) {
+    f.z.finish();
+    if (int rc = status(f.scales.lay_out(s), what)) return rc;
+    Q4Args a{f.z.g, codes, (const uint8_t*)f.scales.at, f.groups, f.scales.row_bytes};
     a.p.a = f.x.at;
     a.p.a_stride = f.x.row_bytes;
-    return status(launch_q4_rows(f32, a, s), what);
+    return status(f.waves ? launch_q4_tiles(f.waves, a, s) : launch_q4_rows(f32, a, s), what);
   }
   if (int rc = status(launch_widen(f32, {codes, scales, f.w.at, d->outs, d->ins, f.groups}, s), what)) return rc;
   return status(f.z.launch(f.x, f.w, s), what);

@@ -181,7 +181,7 @@ SIGNATURES = {
     "fwn_linear_act_bwd_launch": [_LIN, _P, _P, _P, _P, _P, _P, _P, _P, _U64, _P],
     "fwn_linear_act_q8_workspace_size": [_LIN, _P, _P, _P],
     "fwn_quantize_q4_launch": [_I64, _I32, _I64, _I32, _P, _P, _P, _P],
-    "fwn_linear_act_q4_workspace_size": [_LIN, _P, _P],
+    "fwn_linear_act_q4_workspace_size": [_LIN, _P, _P, _P],
     "fwn_linear_act_q4_launch": [_LIN, _P, _P, _P, _P, _P, _P, _P, _U64, _P],
     "fwn_linear_act_q8_launch": [_LIN, _P, _P, _P, _P, _P, _P, _P, _P, _U64, _P],
 }

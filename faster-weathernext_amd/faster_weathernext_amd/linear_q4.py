@@ -85,7 +85,7 @@ def linear_act_q4(x, weight, weight_scale, bias=None, *, activation=None, residu
   L = nat.lib()
   out = x.new_empty((*lead, outs))
   d = nat.LinearDesc(x.numel() // ins, xs, 0, rs, ins, outs, _DTYPES[x.dtype], act)
-  xa = _addr(xr)
-  work, size = _workspace(L.fwn_linear_act_q4_workspace_size, d, x, xa)
-  launch(x, L.fwn_linear_act_q4_launch, d, xa, _addr(codes), _addr(scales), _addr(bias), _addr(rr), _addr(out), _addr(work), size)
+  xa, sa = _addr(xr), _addr(scales)
+  work, size = _workspace(L.fwn_linear_act_q4_workspace_size, d, x, xa, sa)
+  launch(x, L.fwn_linear_act_q4_launch, d, xa, _addr(codes), sa, _addr(bias), _addr(rr), _addr(out), _addr(work), size)
   return out

@@ -291,7 +291,7 @@ int fwn_quantize_q4_launch(int64_t rows, int32_t ins, int64_t x_stride, int32_t 
 
 /* fwn_linear_act_launch with such a weight, without pre; w_stride is not read. Products are exact and added in float32 (float32
  * x as in fwn_linear_act_launch). */
-int fwn_linear_act_q4_workspace_size(const fwn_linear_desc* d, const void* x, uint64_t* bytes);
+int fwn_linear_act_q4_workspace_size(const fwn_linear_desc* d, const void* x, const uint8_t* scales, uint64_t* bytes);
 int fwn_linear_act_q4_launch(const fwn_linear_desc* d, const void* x, const uint8_t* codes, const uint8_t* scales,
                              const void* bias, const void* residual, void* out, void* workspace, uint64_t workspace_bytes,
                              void* stream);

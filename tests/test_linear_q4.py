@@ -351,7 +351,7 @@ def _desc(rows=4, ins=64, outs=32, x_stride=64, r_stride=32, dtype=nat.BF16, act
                                       (dict(activation=9), 2), (dict(rows=1 << 31, ins=1 << 20), 1)])
 def test_bad_descriptors(bad, code):
   L, d, size = nat.lib(), _desc(**bad), ctypes.c_uint64()
-  assert L.fwn_linear_act_q4_workspace_size(d, F, ctypes.byref(size)) == code
+  assert L.fwn_linear_act_q4_workspace_size(d, F, 3 * F, ctypes.byref(size)) == code
   assert L.fwn_linear_act_q4_launch(d, F, 2 * F, 3 * F, None, None, 4 * F, 8 * F, 1 << 30, None) == code
 
 
@@ -364,7 +364,7 @@ def test_bad_pointers():
     args[at] = value
     assert L.fwn_linear_act_q4_launch(d, *args, None, 0, None) == nat.ERR_INVALID_ARG, (at, value)
   d, size = _desc(rows=40), ctypes.c_uint64()
-  assert L.fwn_linear_act_q4_workspace_size(d, F, ctypes.byref(size)) == nat.OK and size.value >= 32 * 64 * 2
+  assert L.fwn_linear_act_q4_workspace_size(d, F, 3 * F, ctypes.byref(size)) == nat.OK and size.value >= 32 * 16
   for work, n in ((None, 0), (8 * F, 16), (8 * F + 16, 1 << 20), (F, 1 << 20), (6 * F, 1 << 20)):
     assert L.fwn_linear_act_q4_launch(d, *good, work, n, None) == nat.ERR_INVALID_ARG
   assert L.fwn_linear_act_q4_launch(_desc(rows=0), *[None] * 7, 0, None) == nat.OK
