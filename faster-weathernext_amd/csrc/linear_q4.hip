@@ -454,26 +454,25 @@ hipError_t launch(const Q4Args& a, hipStream_t stream) {
 // 4,096 -> 4,096 11.0, 12.9 and 16.9, of 5,120 -> 8,192 24.3, 16.2 and 20.3, 20 of 1,024 -> 16,384 16.1, 10.9 and 7.4. float32 products
 // take their time, so that few lines on their way suffice, and long rows take 16 waves: 24 rows of 1,283 -> 2,051 11.4 with 8
 // and 14.6 with 16, of 4,096 -> 4,096 24.1 and 20.6.
-template <bool F32>
-hipError_t launch_as(const Q4Args& a, hipStream_t stream) {
-  const bool few = a.p.e.m <= 16, long_rows = a.p.k > 16 * LINE;
-  if (a.p.e.n > 48 * 256 && !F32) return few ? launch<F32, 1, 4, 8, 2>(a, stream) : launch<F32, 2, 4, 8, 1>(a, stream);
-  if (a.p.e.n > 16 * 256) {
-    if constexpr (F32) return few ? launch<F32, 1, 2, 16, 1>(a, stream) : launch<F32, 2, 2, 16, 1>(a, stream);
-    return few ? launch<F32, 1, 2, 8, 2>(a, stream) : launch<F32, 2, 2, 16, 1>(a, stream);
-  }
-  if constexpr (F32) {
-    if (few) return launch<F32, 1, 1, 8, 1>(a, stream);
-    return long_rows ? launch<F32, 2, 1, 16, 1>(a, stream) : launch<F32, 2, 1, 8, 1>(a, stream);
-  }
-  if (few) return long_rows ? launch<F32, 1, 1, 8, 2>(a, stream) : launch<F32, 1, 1, 16, 1>(a, stream);
-  return launch<F32, 2, 1, 8, 2>(a, stream);
+hipError_t launch_bf16(const Q4Args& a, hipStream_t stream) {
+  const bool few = a.p.e.m <= 16;
+  if (a.p.e.n > 48 * 256) return few ? launch<false, 1, 4, 8, 2>(a, stream) : launch<false, 2, 4, 8, 1>(a, stream);
+  if (a.p.e.n > 16 * 256) return few ? launch<false, 1, 2, 8, 2>(a, stream) : launch<false, 2, 2, 16, 1>(a, stream);
+  if (few) return a.p.k > 16 * LINE ? launch<false, 1, 1, 8, 2>(a, stream) : launch<false, 1, 1, 16, 1>(a, stream);
+  return launch<false, 2, 1, 8, 2>(a, stream);
+}
+
+hipError_t launch_f32(const Q4Args& a, hipStream_t stream) {
+  const bool few = a.p.e.m <= 16;
+  if (a.p.e.n > 16 * 256) return few ? launch<true, 1, 2, 16, 1>(a, stream) : launch<true, 2, 2, 16, 1>(a, stream);
+  if (few) return launch<true, 1, 1, 8, 1>(a, stream);
+  return a.p.k > 16 * LINE ? launch<true, 2, 1, 16, 1>(a, stream) : launch<true, 2, 1, 8, 1>(a, stream);
 }
 
 }  // namespace
 
 hipError_t launch_q4_rows(bool f32, const Q4Args& a, hipStream_t stream) {
-  return f32 ? launch_as<true>(a, stream) : launch_as<false>(a, stream);
+  return f32 ? launch_f32(a, stream) : launch_bf16(a, stream);
 }
 
 hipError_t launch_q4_tiles(int waves, const Q4Args& a, hipStream_t stream) {

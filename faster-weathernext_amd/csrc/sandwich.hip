@@ -18,15 +18,6 @@
 namespace fwn {
 namespace {
 
-template <typename T>
-struct Bits {
-  typedef uint16_t type;
-};
-template <>
-struct Bits<float> {
-  typedef uint32_t type;
-};
-
 // Sums over the TPR threads of a row, by every one of them; fixed order. Within 16 lanes by rotations, beyond by swaps of rows and
 // halves of the wave, none of which takes a trip through LDS as __shfl_xor does (40,968 x 768 bf16 with dropout, backward: 97 us, with
 // __shfl_xor 103; forward of 40,962 x 768 57 and 60).
@@ -88,11 +79,49 @@ __device__ __forceinline__ void put(bool stream, T* p, int left, const float (&f
     store<T, E, false, TAIL>(p, left, f);
 }
 
+// A vector of a row of `channels` with `left` of them from p on, as it lies in memory. With TAIL the row's last vector is read from
+// E elements before the row's end, and fit moves it to its place, with zeros behind: loads of single elements, and any
+// load whose values are changed before the branches of the two meet, are waited for one by one (24,512 x 1,283 bf16, forward and
+// backward: 119 and 193 us so, 82 and 152 without).
+template <typename T, int E, bool TAIL, bool NT = true>
+__device__ __forceinline__ u32x4 ask(const T* p, int left, int channels) {
+  if constexpr (TAIL) {
+    if (channels < E) {  // no row to read before it
+      uint32_t d[E];
+#pragma unroll
+      for (int e = 0; e < E; ++e) d[e] = e < left ? as_bits(load_one(p + e)) : 0u;
+      u32x4 v = {0, 0, 0, 0};
+#pragma unroll
+      for (int e = 0; e < E; ++e) v[e * (int)sizeof(T) / 4] |= (sizeof(T) == 4 ? d[e] : d[e] >> 16) << 8 * (e * (int)sizeof(T) % 4);
+      return v;
+    }
+    return load_raw<T, NT>(left < E ? p + (left - E) : p);
+  }
+  return load_raw<T, NT>(p);
+}
 template <typename T, int E, bool TAIL>
-__device__ __forceinline__ void times(const void* w, bool f32, int64_t at, int left, float (&f)[E]) {
+__device__ __forceinline__ u32x4 fit(const u32x4& v, int left, int channels) {
+  if constexpr (TAIL) {
+    if (channels < E || !__any(left < E)) return v;
+    const int bytes = (E - channels % E) * (int)sizeof(T);
+    u32x4 u = v;
+    if (bytes & 8) u = u32x4{u[2], u[3], 0, 0};
+    if (bytes & 4) u = u32x4{u[1], u[2], u[3], 0};
+    if (bytes & 2) u = u32x4{u[0] >> 16 | u[1] << 16, u[1] >> 16 | u[2] << 16, u[2] >> 16 | u[3] << 16, u[3] >> 16};
+    return left < E ? u : v;
+  }
+  return v;
+}
+
+// f times the E weights from channel c of row `row` of w (of T, or of float); NULL: as it is.
+template <typename T, int E, bool TAIL>
+__device__ __forceinline__ void times(const void* w, bool f32, int64_t row, int c, int channels, float (&f)[E]) {
   if (!w) return;
   float g[E];
-  load_weight<T, E, TAIL>(w, f32, at, left, g);
+  if (sizeof(T) == 4 || !f32)
+    unpack<T>(fit<T, E, TAIL>(ask<T, E, TAIL, false>((const T*)w + row + c, channels - c, channels), channels - c, channels), g);
+  else
+    load_weight<T, E, TAIL>(w, true, row + c, channels - c, g);
 #pragma unroll
   for (int e = 0; e < E; ++e) f[e] *= g[e];
 }
@@ -109,15 +138,21 @@ __global__ void __launch_bounds__(kThreads<TPR>) sandwich_kernel(SandwichArgs a)
     const bool ok = row < a.rows;
     const T* const x = (const T*)a.x + row * a.x_stride;
     const T* const y = (const T*)a.y + row * a.y_stride;
-    float f[VPT][E], b[VPT][E];
+    u32x4 vx[VPT], vy[VPT];
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
       const int c = (t + TPR * k) * E;
-#pragma unroll
-      for (int e = 0; e < E; ++e) f[k][e] = b[k][e] = 0.f;
+      vx[k] = vy[k] = u32x4{0, 0, 0, 0};
       if (!ok || c >= a.channels) continue;
-      load<T, E, true, TAIL>(y + c, a.channels - c, b[k]);
-      load<T, E, true, TAIL>(x + c, a.channels - c, f[k]);
+      vy[k] = ask<T, E, TAIL>(y + c, a.channels - c, a.channels);
+      vx[k] = ask<T, E, TAIL>(x + c, a.channels - c, a.channels);
+    }
+    float f[VPT][E], b[VPT][E];
+#pragma unroll
+    for (int k = 0; k < VPT; ++k) {
+      const int left = a.channels - (t + TPR * k) * E;
+      unpack<T>(fit<T, E, TAIL>(vy[k], left, a.channels), b[k]);
+      unpack<T>(fit<T, E, TAIL>(vx[k], left, a.channels), f[k]);
     }
     float r = 1.f;
     if (a.post_norm) {
@@ -137,8 +172,8 @@ __global__ void __launch_bounds__(kThreads<TPR>) sandwich_kernel(SandwichArgs a)
       if (!ok || c >= a.channels) continue;
 #pragma unroll
       for (int e = 0; e < E; ++e) b[k][e] *= r;
-      times<T, E, TAIL>(a.gate, a.gate_f32, gate_at + c, a.channels - c, b[k]);
-      times<T, E, TAIL>(a.post_weight, a.post_f32, c, a.channels - c, b[k]);
+      times<T, E, TAIL>(a.gate, a.gate_f32, gate_at, c, a.channels, b[k]);
+      times<T, E, TAIL>(a.post_weight, a.post_f32, 0, c, a.channels, b[k]);
       if (a.drop) draw.template apply<E>((uint32_t)row, (uint32_t)c, b[k]);
 #pragma unroll
       for (int e = 0; e < E; ++e) f[k][e] = fmaf(a.scale, f[k][e], b[k][e]);
@@ -161,7 +196,7 @@ __global__ void __launch_bounds__(kThreads<TPR>) sandwich_kernel(SandwichArgs a)
       if (c >= a.channels) continue;
 #pragma unroll
       for (int e = 0; e < E; ++e) f[k][e] *= r;
-      times<T, E, TAIL>(a.pre_weight, a.pre_f32, c, a.channels - c, f[k]);
+      times<T, E, TAIL>(a.pre_weight, a.pre_f32, 0, c, a.channels, f[k]);
       put<T, E, TAIL>(a.stream, (T*)a.out + row * a.channels + c, a.channels - c, f[k]);
     }
   }
@@ -214,19 +249,6 @@ __device__ __forceinline__ void put_weight(void* w, bool f32, int64_t i, float v
     store_one((uint16_t*)w + i, v);
 }
 
-// A vector as it lies in memory; with TAIL its first `left` elements, and zeros.
-template <typename T, int E, bool TAIL>
-__device__ __forceinline__ u32x4 take(const T* p, int left) {
-  if (TAIL && left < E) {
-    u32x4 v = {0, 0, 0, 0};
-#pragma unroll
-    for (int e = 0; e < E; ++e)
-      if (e < left) v[e * (int)sizeof(T) / 4] |= (uint32_t)((const typename Bits<T>::type*)p)[e] << 8 * (e * (int)sizeof(T) % 4);
-    return v;
-  }
-  return load_raw<T, true>(p);
-}
-
 // The first `left` of N sums.
 template <int N>
 __device__ __forceinline__ void put_sums(float* p, int left, const float (&f)[N]) {
@@ -244,10 +266,10 @@ __device__ __forceinline__ void put_sums(float* p, int left, const float (&f)[N]
 
 // E weights from channel c times v; NULL: v.
 template <typename T, int E, bool TAIL>
-__device__ __forceinline__ void weights(const void* w, bool f32, int64_t c, int left, float v, float (&f)[E]) {
+__device__ __forceinline__ void weights(const void* w, bool f32, int64_t row, int c, int channels, float v, float (&f)[E]) {
 #pragma unroll
   for (int e = 0; e < E; ++e) f[e] = v;
-  times<T, E, TAIL>(w, f32, c, left, f);
+  times<T, E, TAIL>(w, f32, row, c, channels, f);
 }
 
 // Waves a SIMD that the backward's registers leave room for.
@@ -273,8 +295,8 @@ __global__ void __launch_bounds__(kThreads<TPR>) __attribute__((amdgpu_waves_per
 #pragma unroll
     for (int e = 0; e < E; ++e) g_pre[k][e] = q[k][e] = pre[k][e] = w[k][e] = 0.f;
     if (c >= a.channels) continue;
-    weights<T, E, TAIL>(a.pre_weight, a.pre_f32, c, a.channels - c, 1.f, pre[k]);
-    if (EACH) weights<T, E, TAIL>(a.post_weight, a.post_f32, c, a.channels - c, keep, w[k]);
+    weights<T, E, TAIL>(a.pre_weight, a.pre_f32, 0, c, a.channels, 1.f, pre[k]);
+    if (EACH) weights<T, E, TAIL>(a.post_weight, a.post_f32, 0, c, a.channels, keep, w[k]);
   }
   float* const part_pre = a.part + (int64_t)blockIdx.x * a.channels;
   float* const part_post = part_pre + (a.g_pre ? (int64_t)grid.blocks * a.channels : 0);
@@ -289,8 +311,8 @@ __global__ void __launch_bounds__(kThreads<TPR>) __attribute__((amdgpu_waves_per
 #pragma unroll
         for (int e = 0; e < E; ++e) q[k][e] = 0.f;
         if (c >= a.channels) continue;
-        weights<T, E, TAIL>(a.post_weight, a.post_f32, c, a.channels - c, keep, w[k]);
-        times<T, E, TAIL>(a.gate, a.gate_f32, group * a.channels + c, a.channels - c, w[k]);
+        weights<T, E, TAIL>(a.post_weight, a.post_f32, 0, c, a.channels, keep, w[k]);
+        times<T, E, TAIL>(a.gate, a.gate_f32, group * a.channels, c, a.channels, w[k]);
       }
     }
     const int64_t begin = group * grid.group_rows, end = begin + grid.group_rows;
@@ -305,10 +327,20 @@ __global__ void __launch_bounds__(kThreads<TPR>) __attribute__((amdgpu_waves_per
         vs[k] = vy[k] = vo[k] = vg[k] = u32x4{0, 0, 0, 0};
         if (!ok || c >= a.channels) continue;
         const int left = a.channels - c;
-        vs[k] = take<T, E, TAIL>((const T*)a.s + at + c, left);
-        if (a.g_out) vo[k] = take<T, E, TAIL>((const T*)a.g_out + at + c, left);
-        if (a.g_sum) vg[k] = take<T, E, TAIL>((const T*)a.g_sum + at + c, left);
-        vy[k] = take<T, E, TAIL>((const T*)a.y + row * a.y_stride + c, left);
+        vs[k] = ask<T, E, TAIL>((const T*)a.s + at + c, left, a.channels);
+        if (a.g_out) vo[k] = ask<T, E, TAIL>((const T*)a.g_out + at + c, left, a.channels);
+        if (a.g_sum) vg[k] = ask<T, E, TAIL>((const T*)a.g_sum + at + c, left, a.channels);
+        vy[k] = ask<T, E, TAIL>((const T*)a.y + row * a.y_stride + c, left, a.channels);
+      }
+      if constexpr (TAIL) {
+#pragma unroll
+        for (int k = 0; k < VPT; ++k) {
+          const int left = a.channels - (t + TPR * k) * E;
+          vs[k] = fit<T, E, TAIL>(vs[k], left, a.channels);
+          vo[k] = fit<T, E, TAIL>(vo[k], left, a.channels);
+          vg[k] = fit<T, E, TAIL>(vg[k], left, a.channels);
+          vy[k] = fit<T, E, TAIL>(vy[k], left, a.channels);
+        }
       }
       float r2 = 0.f, k2 = 0.f;
       if (a.g_out) {
@@ -358,7 +390,7 @@ __global__ void __launch_bounds__(kThreads<TPR>) __attribute__((amdgpu_waves_per
         if constexpr (EACH) {
 #pragma unroll
           for (int e = 0; e < E; ++e) g[e] = w[k][e];
-          times<T, E, TAIL>(a.gate, a.gate_f32, at + c, left, g);
+          times<T, E, TAIL>(a.gate, a.gate_f32, at, c, a.channels, g);
         }
 #pragma unroll
         for (int e = 0; e < E; ++e) {
@@ -382,7 +414,7 @@ __global__ void __launch_bounds__(kThreads<TPR>) __attribute__((amdgpu_waves_per
         if constexpr (EACH) {
           // The gate's gradient, and db times the gate in place of db.
           float g[E];
-          weights<T, E, TAIL>(a.gate, a.gate_f32, at + c, left, 1.f, g);
+          weights<T, E, TAIL>(a.gate, a.gate_f32, at, c, a.channels, 1.f, g);
 #pragma unroll
           for (int e = 0; e < E; ++e) {
             o[e] = db[k][e] * w[k][e] * (y[e] * r1);
