@@ -1,7 +1,8 @@
 // Dropout of rows with the residual's addition (gfx950): out = rnd(kept x 2^16 / (2^16 - T) + residual), its backward pass the same
 // over the gradient. Nothing about what is kept is stored: see dropout_device.h.
 //
-// Bound by HBM, a streaming pass of one 16-byte vector of each tensor a thread and step, two steps at a time.
+// Bound by HBM, a streaming pass of one 16-byte vector of each tensor a thread and step, two steps at a time: 40,962 x 768 bf16 with a
+// residual 34 us (5.6 TB/s), without 26; 10,242 x 1,283 float32 21 (5.0). The generator takes about half of that time beside it.
 #include "dropout_device.h"
 
 #include "fwn_attn.h"

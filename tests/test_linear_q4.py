@@ -175,6 +175,20 @@ def test_normal_numbers(rows, ins, outs, dtype, activation):
 
 
 @gpu
+@pytest.mark.parametrize("rows,ins,outs", [(512, 1100, 8200), (300, 4096, 2056), (33, 8192, 300), (700, 2000, 3000), (32, 16384, 515),
+                                           (17, 16384, 4104), (64, 1024, 16384), (2100, 640, 4097), (20, 900, 12800), (3, 700, 12900)])
+def test_tiles_and_ranges(rows, ins, outs):
+  """Whole numbers over sizes that take tiles of both widths, sums in several ranges, and many outputs a workgroup."""
+  codes, scales = _random_codes(outs, ins, 1, 127, 129)
+  x = torch.randint(-1, 2, (rows, ins), generator=_gen(3)).bfloat16().to(DEV)
+  r = torch.randint(-2, 3, (rows, outs), generator=_gen(5)).bfloat16().to(DEV)
+  z = x.double() @ _values(codes, scales, ins).t()  # below 2^18 in steps of a half: exact in float32
+  for _ in range(2):
+    assert torch.equal(fwn.linear_act_q4(x, codes, scales), z.bfloat16())
+    assert torch.equal(fwn.linear_act_q4(x, codes, scales, residual=r), (z + r.double()).bfloat16())
+
+
+@gpu
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rows", [1, 20, 40])
 def test_every_code_and_scale(rows, dtype):
