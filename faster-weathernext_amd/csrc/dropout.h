@@ -59,7 +59,7 @@ struct SandwichBwdArgs {
   void* g_gate;
   void* g_post;
   void* g_pre;
-  float* part;  // [sandwich_parts, blocks, channels], or null
+  float* part;  // [parts, blocks, channels] of the launch's SandwichGrid, or null
   int64_t rows, gate_rows, y_stride;
   int32_t channels;
   float eps, scale;

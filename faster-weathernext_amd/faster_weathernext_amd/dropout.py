@@ -13,6 +13,8 @@ that should drop independently need another offset (or seed) each; two calls wit
 The tensor is kept for the backward pass, so it must not change before that (autograd refuses one that did):
 a call's offset is a new tensor, or written after the backward pass.
 """
+import operator
+
 import torch
 
 from . import _native as nat
@@ -31,7 +33,7 @@ def rng_of(rng, x):
       raise ValueError("rng must be on the device of x")
     return dense(rng), 0, 0
   try:
-    seed, offset = (int(v) for v in rng)
+    seed, offset = (operator.index(v) for v in rng)
   except (TypeError, ValueError):
     raise ValueError("rng must be a pair (seed, offset) or an int64 tensor of the two") from None
   return None, seed & _WORD, offset & _WORD

@@ -9,10 +9,13 @@ float32 sums and the output's rounding stand between the result and the exact pr
 are one pass over the codes; more rows widen the weight into a workspace first, for the kernels of ``linear_act``. No
 derivative.
 """
+import ctypes
+import functools
+
 import torch
 
 from . import _native as nat
-from .linear_act import _activation, _check_like, _rows, _workspace
+from .linear_act import _activation, _check_like, _rows
 from .rms import _no_grad, dense, launch
 from .rows import _DTYPES, _addr
 
@@ -51,6 +54,14 @@ def _bytes(t, aligned):
   return t.clone(memory_format=torch.contiguous_format)
 
 
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(rows, x_stride, ins, outs, dtype, x_at, scales_at):
+  """A call's workspace, a function of its sizes and of how x and the scales lie to 16 bytes (the query takes 2 us of host time)."""
+  d, size = nat.LinearDesc(rows, x_stride, 0, 0, ins, outs, dtype, 0), ctypes.c_uint64()
+  nat.check(nat.lib().fwn_linear_act_q4_workspace_size(d, 4096 + x_at, 4096 + scales_at, ctypes.byref(size)))
+  return size.value
+
+
 def linear_act_q4(x, weight, weight_scale, bias=None, *, activation=None, residual=None):
   """act(x w^T + bias) + residual with the 4-bit weight w of codes `weight` [outs, 16 groups] (torch.float4_e2m1fn_x2) and
   scales `weight_scale` [outs, groups] (torch.float8_e8m0fnu), as ``quantize_q4`` gives them, groups = ceil(ins / 32). x [..., ins],
@@ -82,10 +93,11 @@ def linear_act_q4(x, weight, weight_scale, bias=None, *, activation=None, residu
   xr, xs = _rows(x)
   rr, rs = _rows(residual, nat.LINEAR_ACT_MAX)
   bias, codes, scales = dense(bias), _bytes(weight, True), _bytes(weight_scale, False)
-  L = nat.lib()
   out = x.new_empty((*lead, outs))
-  d = nat.LinearDesc(x.numel() // ins, xs, 0, rs, ins, outs, _DTYPES[x.dtype], act)
+  rows, dtype = x.numel() // ins, _DTYPES[x.dtype]
+  d = nat.LinearDesc(rows, xs, 0, rs, ins, outs, dtype, act)
   xa, sa = _addr(xr), _addr(scales)
-  work, size = _workspace(L.fwn_linear_act_q4_workspace_size, d, x, xa, sa)
-  launch(x, L.fwn_linear_act_q4_launch, d, xa, _addr(codes), sa, _addr(bias), _addr(rr), _addr(out), _addr(work), size)
+  size = _workspace_bytes(rows, xs, ins, outs, dtype, xa % 16, sa % 16) if rows else 0
+  work = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
+  launch(x, nat.lib().fwn_linear_act_q4_launch, d, xa, _addr(codes), sa, _addr(bias), _addr(rr), _addr(out), _addr(work), size)
   return out

@@ -248,7 +248,7 @@ def test_refusals():
                lambda: fwn.dropout(x, 1.1, (1, 2)), lambda: fwn.dropout(x, float("nan"), (1, 2)),
                lambda: fwn.dropout(x, 0.1, (1, 2), residual=x[:2]), lambda: fwn.dropout(x, 0.1, (1, 2), residual=x.bfloat16()),
                lambda: fwn.dropout(x, 0.1, (1, 2), residual=torch.zeros(4, 64)), lambda: fwn.dropout(x, 0.1, (1,)),
-               lambda: fwn.dropout(x, 0.1, (1, 2, 3)), lambda: fwn.dropout(x, 0.1, None), lambda: fwn.dropout(x, 0.1, 5),
+               lambda: fwn.dropout(x, 0.1, (1, 2, 3)), lambda: fwn.dropout(x, 0.1, (1.5, 2)), lambda: fwn.dropout(x, 0.1, "12"), lambda: fwn.dropout(x, 0.1, None), lambda: fwn.dropout(x, 0.1, 5),
                lambda: fwn.dropout(x, 0.1, torch.tensor([1, 2])), lambda: fwn.dropout(x, 0.1, torch.tensor([1., 2.], device=DEV)),
                lambda: fwn.dropout(x, 0.1, torch.tensor([1, 2, 3], device=DEV))):
     with pytest.raises(ValueError):
