@@ -60,10 +60,19 @@ def _workspace_bytes(rows, gate_rows, channels, dtype, gate):
   return size.value
 
 
+def _for_launch(d, x_stride, y_stride, state):
+  """d for one launch: a copy of its own, as passes over one graph may run at once, with the address of the state that the launch
+  holds. What autograd gives back of a saved state may be another tensor than the forward pass had (hooks, checkpoints)."""
+  d = nat.SandwichDesc.from_buffer_copy(d)
+  d.x_stride, d.y_stride, d.drop.state = x_stride, y_stride, _addr(state)
+  return d
+
+
 def _forward(x, y, post, pre, gate, state, d):
   """(s, out): one HIP pass (no autograd)."""
-  xr, d.x_stride = rows_of(x)
-  yr, d.y_stride = rows_of(y)
+  xr, xs = rows_of(x)
+  yr, ys = rows_of(y)
+  d = _for_launch(d, xs, ys, state)
   post, pre, gate = dense(post), dense(pre), dense(gate)
   s, out = new_like(x), new_like(x)
   launch(x, nat.lib().fwn_sandwich_norm_launch, d, _addr(xr), _addr(yr), _addr(gate), _addr(post), _addr(pre), _addr(s),
@@ -75,7 +84,9 @@ def _backward(s, y, post, pre, gate, state, d, g_sum, g_out, needs):
   """The gradients that `needs` asks for of x, y, post, pre and gate: fwn_sandwich_norm_bwd_launch."""
   if not s.numel():
     return tuple(torch.zeros_like(t) if n else None for t, n in zip((s, y, post, pre, gate), needs))
-  yr, d.y_stride = rows_of(y)
+  yr, ys = rows_of(y)
+  state = dense(state)
+  d = _for_launch(d, 0, ys, state)
   s, post, pre, gate, g_sum, g_out = dense(s), dense(post), dense(pre), dense(gate), dense(g_sum), dense(g_out)
   need_x, need_y, need_post, need_pre, need_gate = needs
   gx = torch.empty_like(s) if need_x else None
@@ -170,9 +181,9 @@ def sandwich_norm(x, y, post_weight=None, pre_weight=None, *, gate=None, scale=1
       raise ValueError("dropout needs rng, its state")
     state, seed, offset = rng_of(rng, x)
   c, dtype = x.shape[-1], _DTYPES[x.dtype]
-  # The strides are filled in where the rows are taken; the backward pass takes the same descriptor, of tensors it keeps.
+  # Strides and the state's address are each launch's own (_for_launch): autograd keeps the descriptor without them.
   d = nat.SandwichDesc(x.numel() // c, _gate_rows(gate, x), 0, 0, c, dtype, _kind(gate, dtype), _kind(post_weight, dtype),
-                       _kind(pre_weight, dtype), bool(post_norm), eps, scale, nat.Dropout(p, seed, offset, _addr(state)))
+                       _kind(pre_weight, dtype), bool(post_norm), eps, scale, nat.Dropout(p, seed, offset, None))
   if _needs(x, y, post_weight, pre_weight, gate):
     return _Sandwich.apply(x, y, post_weight, pre_weight, gate, state, d)
   return _forward(x, y, post_weight, pre_weight, gate, state, d)

@@ -1,0 +1,167 @@
+"""Dropout's state tensor where autograd keeps it by hooks (``torch.utils.checkpoint``, ``save_on_cpu``, a program's own): the
+backward pass has to read the tensor that the hooks give back, as nothing else holds the one of the forward pass.
+
+Gradients through hooks are the same launches over the same values and are compared bit by bit. The pass as torch operations
+(create_graph) adds in another order: float32 rows of 72 channels, chains below 200 operations on terms of one size, within
+2^-16 of the gradients' norms."""
+import ctypes
+import importlib
+
+import pytest
+import torch
+from torch.utils.checkpoint import checkpoint
+
+import faster_weathernext_amd as fwn
+from oracle import dropout as oracle
+
+DEV = "cuda"
+gpu = pytest.mark.gpu
+WORDS = {"first": (5, 6), "second": (7, 1 << 40)}
+
+
+def _normal(shape, seed, dtype=torch.float32, device=DEV):
+  return torch.randn(shape, generator=torch.Generator().manual_seed(seed)).to(dtype).to(device)
+
+
+def _state(words, device=DEV, strided=False):
+  state = torch.tensor(words, device=device)
+  return torch.stack([state, state + 9], 1)[:, 0] if strided else state
+
+
+class _Recorder:
+  """Takes the launches' place: notes the state that a kernel would read."""
+
+  def __init__(self):
+    self.read = []
+
+  def __call__(self, t, fn, d, *args):
+    self.read.append(tuple((ctypes.c_int64 * 2).from_address(d.drop.state)))
+
+
+def _branch(name, record, monkeypatch):
+  """A call of the operator for tensors on the host, the launches recorded."""
+  module = importlib.import_module("faster_weathernext_amd." + name)
+  monkeypatch.setattr(module, "launch", record)
+  if name == "dropout":
+    return lambda x, state: module._Dropout.apply(x, None, 0.5, state, 0, 0)
+  monkeypatch.setattr(module, "_check", lambda *args: None)
+  monkeypatch.setattr(module, "rng_of", lambda rng, x: (rng, 0, 0))
+  return lambda x, state: module.sandwich_norm(x, x, p=0.5, rng=state)[1]
+
+
+@pytest.mark.parametrize("name,strided", [("dropout", False), ("sandwich", False), ("sandwich", True)])
+def test_the_backward_reads_the_unpacked_state(name, strided, monkeypatch):
+  record = _Recorder()
+  call = _branch(name, record, monkeypatch)
+  x, state = _normal((3, 64), 1, device="cpu").requires_grad_(), _state(WORDS["first"], "cpu")
+  other = _state(WORDS["second"], "cpu", strided)
+  with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: other if t.dtype == torch.int64 else t):
+    out = call(x, state)
+  held = getattr(out.grad_fn, "desc", None)
+  before = held and bytes(held)
+  for _ in range(2):
+    torch.autograd.grad(out, x, torch.ones_like(out), retain_graph=True)
+  assert record.read == [WORDS["first"]] + 2 * [WORDS["second"]]
+  # Passes that run at once over one graph write to nothing that they share, and nothing holds an address without its tensor.
+  if held:
+    assert bytes(held) == before and held.drop.state is None
+
+
+def _leaves(seed=0, dtype=torch.float32):
+  """x, y, post_weight, pre_weight and gate."""
+  shapes = ((2, 9, 72), (2, 9, 72), (72,), (72,), (2, 72))
+  return [_normal(s, seed + k, dtype).requires_grad_() for k, s in enumerate(shapes)]
+
+
+def _sandwich(leaves, state):
+  x, y, post, pre, gate = leaves
+  return fwn.sandwich_norm(x, y, post, pre, gate=gate, scale=0.5, p=0.4, rng=state)
+
+
+def _dropout(leaves, state):
+  x, y = leaves[:2]
+  return (fwn.dropout(x, 0.4, state, residual=y),)
+
+
+OPERATORS = {"sandwich": (_sandwich, 5), "dropout": (_dropout, 2)}
+
+
+def _grads(name, leaves, outs):
+  n = OPERATORS[name][1]
+  gs = tuple(_normal(o.shape, 30 + k, o.dtype) for k, o in enumerate(outs))
+  return torch.autograd.grad(outs, leaves[:n], gs)
+
+
+def _churn():
+  """Fills memory that was given back: as much as the call's small tensors, over and over."""
+  return [torch.full((2,), -1, device=DEV) for _ in range(512)]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("strided", [False, True])
+@pytest.mark.parametrize("name", OPERATORS)
+def test_checkpoint(name, strided, dtype):
+  """A block that is recomputed, with a state made inside it, against the block that is not; a model of two blocks."""
+  fn, leaves = OPERATORS[name][0], _leaves(0, dtype)
+  want = _grads(name, leaves, fn(leaves, _state(WORDS["first"])))
+  block = lambda *t: fn(t, _state(WORDS["first"], strided=strided))
+  outs = checkpoint(block, *leaves, use_reentrant=False)
+  held = _churn()
+  for a, b in zip(_grads(name, leaves, outs), want):
+    assert torch.equal(a, b)
+  del held
+  def two(leaves, again):
+    x = leaves[0]
+    for k in range(2):
+      inner = lambda x, k=k: fn([x, *leaves[1:]], _state((5, k), strided=strided))[0]
+      x = checkpoint(inner, x, use_reentrant=False) if again else inner(x)
+    return (x,)
+  plain, again = two(leaves, False), two(leaves, True)
+  held = _churn()
+  used = leaves[:1]
+  g = _normal(plain[0].shape, 9, dtype)
+  assert torch.equal(torch.autograd.grad(again, used, g)[0], torch.autograd.grad(plain, used, g)[0])
+  del held
+
+
+@gpu
+@pytest.mark.parametrize("strided", [False, True])
+@pytest.mark.parametrize("name", OPERATORS)
+def test_saved_on_the_host(name, strided):
+  fn, leaves = OPERATORS[name][0], _leaves()
+  want = _grads(name, leaves, fn(leaves, _state(WORDS["first"])))
+  with torch.autograd.graph.save_on_cpu():
+    outs = fn(leaves, _state(WORDS["first"], strided=strided))
+  held = _churn()
+  for a, b in zip(_grads(name, leaves, outs), want):
+    assert torch.equal(a, b)
+  del held
+
+
+@gpu
+@pytest.mark.parametrize("name", OPERATORS)
+def test_gradients_follow_the_unpacked_state(name):
+  """Hooks that give back another state: the passes by kernels and as torch operations drop by that one."""
+  fn, n = OPERATORS[name]
+  leaves, first = _leaves(), _state(WORDS["first"])
+  other = _state(WORDS["second"])
+  with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: other if t.dtype == torch.int64 else t):
+    outs = fn(leaves, first)
+  got = _grads(name, leaves, outs)
+  gs = tuple(_normal(o.shape, 30 + k) for k, o in enumerate(outs))
+  wide = torch.autograd.grad(outs, leaves[:n], gs, create_graph=True)
+  for a, b in zip(got, wide):
+    assert (a - b).norm() <= 2.0 ** -16 * b.norm()
+  if name == "dropout":
+    kept = torch.from_numpy(oracle.kept(18, 72, 0.4, *WORDS["second"])).to(DEV).view(2, 9, 72)
+    assert torch.equal(got[0], gs[0] * kept * float(oracle.multiplier(0.4)))
+
+
+@gpu
+def test_state_changed_before_the_backward_pass():
+  leaves, state = _leaves(), _state(WORDS["first"])
+  outs = _sandwich(leaves, state)
+  state += 1
+  with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+    _grads("sandwich", leaves, outs)
