@@ -86,10 +86,10 @@ def _dropout(leaves, state):
 OPERATORS = {"sandwich": (_sandwich, 5), "dropout": (_dropout, 2)}
 
 
-def _grads(name, leaves, outs):
+def _grads(name, leaves, outs, **keep):
   n = OPERATORS[name][1]
   gs = tuple(_normal(o.shape, 30 + k, o.dtype) for k, o in enumerate(outs))
-  return torch.autograd.grad(outs, leaves[:n], gs)
+  return torch.autograd.grad(outs, leaves[:n], gs, **keep)
 
 
 def _churn():
@@ -148,7 +148,7 @@ def test_gradients_follow_the_unpacked_state(name):
   other = _state(WORDS["second"])
   with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: other if t.dtype == torch.int64 else t):
     outs = fn(leaves, first)
-  got = _grads(name, leaves, outs)
+  got = _grads(name, leaves, outs, retain_graph=True)
   gs = tuple(_normal(o.shape, 30 + k) for k, o in enumerate(outs))
   wide = torch.autograd.grad(outs, leaves[:n], gs, create_graph=True)
   for a, b in zip(got, wide):
