@@ -47,12 +47,13 @@ def check_p(p):
 
 
 def _forward(x, residual, p, rng):
-  """One HIP pass (no autograd); rng as rng_of gives it."""
+  """One HIP pass (no autograd); rng as rng_of gives it, or with the state as autograd gives it back."""
   c = x.shape[-1]
   xr, xs = rows_of(x)
   rr, rs = rows_of(residual) if residual is not None else (None, 0)
   out = new_like(x)
   state, seed, offset = rng
+  state = dense(state)
   d = nat.DropoutDesc(x.numel() // c, xs, rs, c, _DTYPES[x.dtype], nat.Dropout(p, seed, offset, _addr(state)))
   launch(x, nat.lib().fwn_dropout_launch, d, _addr(xr), _addr(rr), _addr(out))
   return out

@@ -49,7 +49,8 @@ def _branch(name, record, monkeypatch):
   return lambda x, state: module.sandwich_norm(x, x, p=0.5, rng=state)[1]
 
 
-@pytest.mark.parametrize("name,strided", [("dropout", False), ("sandwich", False), ("sandwich", True)])
+@pytest.mark.parametrize("strided", [False, True])
+@pytest.mark.parametrize("name", ["dropout", "sandwich"])
 def test_the_backward_reads_the_unpacked_state(name, strided, monkeypatch):
   record = _Recorder()
   call = _branch(name, record, monkeypatch)
@@ -140,12 +141,13 @@ def test_saved_on_the_host(name, strided):
 
 
 @gpu
+@pytest.mark.parametrize("strided", [False, True])
 @pytest.mark.parametrize("name", OPERATORS)
-def test_gradients_follow_the_unpacked_state(name):
+def test_gradients_follow_the_unpacked_state(name, strided):
   """Hooks that give back another state: the passes by kernels and as torch operations drop by that one."""
   fn, n = OPERATORS[name]
   leaves, first = _leaves(), _state(WORDS["first"])
-  other = _state(WORDS["second"])
+  other = _state(WORDS["second"], strided=strided)
   with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: other if t.dtype == torch.int64 else t):
     outs = fn(leaves, first)
   got = _grads(name, leaves, outs, retain_graph=True)
