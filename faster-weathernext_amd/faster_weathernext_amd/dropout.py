@@ -39,8 +39,15 @@ def rng_of(rng, x):
   return None, seed & _WORD, offset & _WORD
 
 
+def check_number(v, name):
+  """v, refused as a tensor: it would be copied to the host, and get no gradient."""
+  if isinstance(v, torch.Tensor):
+    raise TypeError(f"{name} must be a number, got a tensor")
+  return v
+
+
 def check_p(p):
-  p = float(p)
+  p = float(check_number(p, "p"))
   if not 0 <= p <= 1:
     raise ValueError(f"p must be 0 to 1, got {p}")
   return p

@@ -14,7 +14,7 @@ import functools
 import torch
 
 from . import _native as nat
-from .dropout import check_p, dropped, multipliers, rng_of
+from .dropout import check_number, check_p, dropped, multipliers, rng_of
 from .rms import _check, _needs, dense, launch, new_like, rows_of
 from .rows import _DTYPES, _addr, as_torch
 
@@ -165,16 +165,17 @@ def sandwich_norm(x, y, post_weight=None, pre_weight=None, *, gate=None, scale=1
   and y [..., channels] of one shape, float32 or bfloat16 on a GPU, with 1 to 16,384 channels and fewer than 2^32 rows.
 
   Weights [channels] and the gate are in x's dtype or float32, None is 1. The gate is [channels], [members, channels] for
-  x of [members, ..., channels], or of x's shape. Without `post_norm` y is gated as it is, and there is no post_weight. `scale` is
-  a number. With p > 0 the gated branch is dropped as ``dropout`` drops it, by the state `rng`. s is formed in float32
-  and stored rounded once; statistics are float32 and those of s are the stored rows'. Rows of any stride are read where they lie if their
-  channels are contiguous. Differentiable in x, y, the weights and the gate; the gradient of s adds to the norm's."""
+  x of [members, ..., channels], or of x's shape. Without `post_norm` y is gated as it is, and there is no post_weight. `scale`, `p`
+  and `eps` are numbers: a learned scale is applied to x before the call. With p > 0 the gated branch is dropped as
+  ``dropout`` drops it, by the state `rng`. s is formed in float32 and stored rounded once; statistics are float32 and
+  those of s are the stored rows'. Rows of any stride are read where they lie if their channels are contiguous. Differentiable in x, y, the weights and the gate; the gradient of s adds to the norm's."""
   _check(x, "x")
   _check(y, "y", x)
   _check_weight(post_weight, "post_weight", x)
   _check_weight(pre_weight, "pre_weight", x)
   if post_weight is not None and not post_norm:
     raise ValueError("post_weight is the norm's: there is none without post_norm")
+  scale, eps = check_number(scale, "scale"), check_number(eps, "eps")
   p, state, seed, offset = check_p(p), None, 0, 0
   if p > 0:
     if rng is None:
