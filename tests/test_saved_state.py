@@ -167,3 +167,16 @@ def test_state_changed_before_the_backward_pass():
   state += 1
   with pytest.raises(RuntimeError, match="modified by an inplace operation"):
     _grads("sandwich", leaves, outs)
+
+
+@gpu
+def test_two_calls_of_a_step():
+  """Rows of one tensor of states, an offset for each call: both drop by their own, and so do their backward passes."""
+  first, second = torch.tensor([[5, 12], [5, 13]], device=DEV)
+  (x, y, *_), g = _leaves(), _normal((2, 9, 72), 40)
+  keep = [torch.from_numpy(oracle.kept(18, 72, 0.5, 5, k)).to(DEV).view(2, 9, 72) * 2.0 for k in (12, 13)]
+  branch = fwn.dropout(y, 0.5, first, residual=x)
+  s, _ = fwn.sandwich_norm(branch, y, post_norm=False, p=0.5, rng=second)
+  assert torch.equal(s.detach(), (y * keep[0] + x + y * keep[1]).detach())
+  gx, gy = torch.autograd.grad(s, (x, y), g)
+  assert torch.equal(gx, g) and torch.equal(gy, g * keep[0] + g * keep[1])
