@@ -5,9 +5,12 @@
 The format is the 4-bit one of the OCP microscaling specification: e2m1 codes (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their
 negatives), two a byte with the even input in the low half, and e8m0 scales, 4.25 bits a weight. ``quantize_q4`` makes them of a layer's
 weight once; ``linear_act_q4`` is ``linear_act`` with them. Such a weight is exact in bfloat16, so that only x's own type, the
-float32 sums and the output's rounding stand between the result and the exact product with the quantised weight. Up to 32 rows of x
-are one pass over the codes; more rows widen the weight into a workspace first, for the kernels of ``linear_act``. No
-derivative.
+float32 sums and the output's rounding stand between the result and the exact product with the quantised weight. Up to 16 rows of x
+are one pass over the codes. More rows of bfloat16 go by an estimate of the time: up to 32 in that pass too, or any number in tiles
+that read the codes, with partial sums in a workspace where the sum is split, or over the weight widened into a workspace by the
+kernels of ``linear_act``. float32 takes the one pass up to 32 rows and the widened weight beyond. Rows of bfloat16 that are not
+whole aligned 16 bytes, and for the tiles scales whose groups are not whole aligned fours, are laid out in the workspace by
+each call. No derivative.
 """
 import ctypes
 import functools
