@@ -163,9 +163,9 @@ Plan plan(Operands how, int64_t m, int64_t n, int64_t k, int32_t op, bool widene
 }
 
 // How a product of bf16 rows with a 4-bit weight is formed, by an estimate of its time in us: the few rows' kernel (tile -1), tiles
-// that take the codes (tile: their waves), or a widened weight and its plan (tile 0). Measured and estimated: 24 rows of 5,120 ->
-// 8,192 16 in few rows, 21 in tiles; 32 of 16,384 -> 4,096 38 and 24; 512 of 4,096 -> 8,192 36 in tiles of four waves, 39 of two, 62
-// widened; 2,048 of 2,048 -> 4,096 41 in tiles, 40 widened.
+// that take the codes (tile: their waves), or a widened weight and its plan (tile 0). Measured on one machine, from captured graphs,
+// and estimated: 24 rows of 5,120 -> 8,192 16 in few rows, 21 in tiles; 32 of 16,384 -> 4,096 38 and 24; 512 of 4,096 -> 8,192 36 in
+// tiles of four waves (38 to 40 on others), 39 of two, 62 widened; 2,048 of 2,048 -> 4,096 41 in tiles, 40 widened.
 Plan plan_q4(int64_t m, int64_t n, int64_t k) {
   Plan best{0, 1, 0};
   const double weights = (double)n * k;

@@ -2,11 +2,12 @@
 // w = value(code) 2^(e - 127), the codes OCP e2m1 (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives) and e the group's
 // OCP e8m0 scale. Such a weight is exact in bfloat16, so that products of widened weights are exact and added in float32.
 //
-// Few rows of x: bound by the weight's trip from memory and the rows' from L2, one pass over the weight with no partial products
-// to join. A workgroup has 16 to 64 outputs, its waves share the sum, 128 inputs at a time: a lane's 16 bytes of codes are one
+// Few rows of x: bound by the weight's trip from memory and the waits for the rows' from L2, one pass over the weight with no
+// partial products to join. A workgroup has 16 to 64 outputs, its waves share the sum, 128 inputs at a time: a lane's 16 bytes of codes are one
 // group of one weight row, exchanged between the four lanes of a row so that each has eight inputs of each group and widened in
-// registers by the groups' scales to the MFMAs' operands; the waves' sums meet in LDS. One row of 4,096 -> 4,096 takes 5.8 us, of
-// 8,192 -> 8,192 12.4 (2.9 TB/s; as bf16 33), 24 rows of 5,120 -> 8,192 16.
+// registers by the groups' scales to the MFMAs' operands; the waves' sums meet in LDS. From a captured graph one row of
+// 4,096 -> 4,096 takes 5.5 to 5.9 us, of 8,192 -> 8,192 12.4 to 14 (2.5 to 2.9 TB/s; as bf16 33 to 35), 24 rows of 5,120 -> 8,192 16 to 17;
+// with a profiler 7.0 and 18 for the first and the last.
 // More rows of bf16: tiles that read the codes (q4_tile_kernel); float32, and rows enough to pay for it: the weight is widened
 // into the workspace for the kernels of linear_act.
 #include "linear_act_device.h"
@@ -255,9 +256,10 @@ struct CopyCodes {
 // by direct copies, the weight as codes; a wave has 64 outputs of its own, so that each code is widened once a tile. All stages
 // but the one that is multiplied are on their way.
 // Bound by the copies: 34 KB a stage of four waves, 0.75 us alone and 0.85 to 1.0 with the products (0.43 of the matrix units)
-// where every CU has a workgroup. 512 rows of 4,096 -> 8,192: 36 us (950 TFLOP/s), with the weight widened first 19 and 43.
-// Codes from memory straight to the registers that widen them took 51 us (a lane's 16 bytes lie in another line than its
-// neighbours'), two stages of 256 inputs 37, the next stage's first reads before the last products of a stage 39.
+// where every CU has a workgroup. 512 rows of 4,096 -> 8,192 from a captured graph: 38 to 40 us (860 to 900 TFLOP/s), with GELU and a
+// residual 41 to 47 (48 with a profiler); with the weight widened first 19 and 43. Beside 36 us on the machine of these
+// comparisons: codes from memory straight to the registers that widen them took 51 us (a lane's 16 bytes lie in another line
+// than its neighbours'), two stages of 256 inputs 37, the next stage's first reads before the last products of a stage 39.
 template <int WAVES, int STAGES>
 __global__ void __launch_bounds__(64 * WAVES, 1) q4_tile_kernel(Q4Args a) {
   constexpr int SUBS = kSpan * 2 / kStageBytes, BN = 64 * WAVES, ROWS_STAGE = kRows * kSpan * 2, STAGE = ROWS_STAGE + BN * 64;

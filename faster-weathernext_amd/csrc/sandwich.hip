@@ -10,9 +10,9 @@
 //
 // Streaming passes bound by HBM: a row is held in registers from its only load to its outputs, and the backward forms
 // both r and what is dropped anew from s, y and the counter. TPR threads share a row, each with VPT vectors of E elements.
-// 40,962 x 768 bf16: forward 55 us (4.6 TB/s), with a gate for each member and dropout 64; backward with both 87 and 6 for the sums
+// 40,962 x 768 bf16: forward 55 to 57 us (4.4 to 4.6 TB/s), with a gate for each member and dropout 64; backward with both 87 and 6 for the sums
 // (without dropout 81: the generator's multiplications run at a quarter of the other instructions' rate). 5,124 x 4,096 bf16 with a
-// gate an element: 43 and 68 (4.9 TB/s). 20,480 x 768 float32: 48 and 75 (5.3, 5.0).
+// gate an element: 45 and 69 (4.7 and 4.9 TB/s). 20,480 x 768 float32: 48 and 75 (5.3, 5.0).
 #include "dropout_device.h"
 
 #include "fwn_attn.h"
